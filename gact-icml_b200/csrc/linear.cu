@@ -1,0 +1,659 @@
+// Linear layers on the 5th-generation tensor cores:
+//
+//   forward        z = x W^T + b,  y = act(z) + residual;  z is kept as an 8-bit checkpoint made in the epilogue
+//   act backward   dz = dy act'(z'),  db = sum over rows of dz   (z' restored from the checkpoint)
+//   data gradient  dx = dz W
+//   weight grad.   dW = dz^T x'
+//
+// One matrix-product kernel serves all three products (the operands are read in the layout they have in memory: K-major or
+// MN-major tiles), persistent, one block per SM: warp 0 feeds a ring of operand tiles with tensor-map copies, one thread of
+// warp 1 issues tcgen05.mma into one of two TMEM accumulators, eight warps work on the other one (epilogue).
+#include "blocks8.cuh"
+#include "tcgen05.cuh"
+
+namespace gact {
+
+__device__ int g_linear_error = 0;
+
+constexpr int kBM = 128, kBK = 64;            // tile rows, reduction per stage (64 16-bit elements = one 128-byte swizzle row)
+constexpr int kGThreads = 384;                // warps: 0 copies, 1 products, 2 TMEM, 3 idle, 4..11 epilogue
+constexpr int kEpiWarps = 8;
+
+enum { kEpiStore = 0, kEpiLinear = 1, kEpiPartial = 2 };
+
+struct GemmArgs {
+    int64_t M, N; int ktiles;                 // output rows, columns, reduction in stages
+    int tiles_m, tiles_n, splits, per_split;  // stages per split
+    // epilogue
+    void* out; int64_t ldo; int ovec;         // bytes per store: 32, 16 or 2
+    const void* bias; int bvec;
+    const void* res; int64_t ldr; int rvec;
+    int act;
+    void* z; int zvec;                        // pre-activation in the operand type (row pitch N), or
+    int8_t* zcodes; uint8_t* zscales; int64_t zpitch;   // as 8-bit checkpoint
+    int stochastic; PhiloxKeys rk;
+    float* partial;                           // [splits][M][pitchN] fp32
+    int64_t ldp;
+};
+
+__device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// ---- activations ----------------------------------------------------------------------------------------------------
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 through Abramowitz & Stegun 7.1.26 (|error| of erf <= 1.5e-7): with
+// t = 1 / (1 + 0.3275911 |z| / sqrt 2), erfc(|z| / sqrt 2) = t (a1 + t (a2 + ...)) exp(-z^2 / 2).  One exponential serves
+// Phi and the density.  The tail keeps its relative precision (no cancellation against 1 for negative z).
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& gauss) {
+    const float az = fabsf(z);
+    gauss = __expf(-0.5f * z * z);
+    const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678118654752f, az, 1.0f));
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(t, p, 1.421413741f);
+    p = fmaf(t, p, -0.284496736f);
+    p = fmaf(t, p, 0.254829592f);
+    const float half_tail = 0.5f * p * t * gauss;
+    cdf = z < 0.0f ? half_tail : 1.0f - half_tail;
+}
+__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+constexpr float kTanhA = 1.5957691216057308f;       // 2 sqrt(2 / pi): (1 + tanh u) / 2 = sigmoid(2 u)
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == GACT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+    if (act == GACT_ACT_GELU) {
+        float c, g;
+        normal_cdf(z, c, g);
+        return z * c;
+    }
+    if (act == GACT_ACT_GELU_TANH) return z * sigmoid(kTanhA * fmaf(0.044715f * z * z, z, z));
+    if (act == GACT_ACT_SILU) return z * sigmoid(z);
+    return z;
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == GACT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    if (act == GACT_ACT_GELU) {
+        float c, g;
+        normal_cdf(z, c, g);
+        return fmaf(z * 0.39894228040143268f, g, c);
+    }
+    if (act == GACT_ACT_GELU_TANH) {
+        const float p = sigmoid(kTanhA * fmaf(0.044715f * z * z, z, z));
+        return fmaf(z * p * (1.0f - p), kTanhA * fmaf(3.0f * 0.044715f, z * z, 1.0f), p);
+    }
+    if (act == GACT_ACT_SILU) {
+        const float p = sigmoid(z);
+        return fmaf(z * p, 1.0f - p, p);
+    }
+    return 1.0f;
+}
+
+// ---- epilogue of 32 consecutive columns of one row -------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, const float (&v)[32]) {
+    using T = typename Elem<DT>::T;
+    T* p = (T*)base + row * ld + n;
+    if (n + 32 <= N && vec >= 16) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+        if (vec == 32) {
+            const uint32_t a[8] = {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, b[8] = {w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]};
+            st_v8(p, a);
+            st_v8(p + 16, b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) *(uint4*)(p + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (n + j < N) p[j] = Elem<DT>::from_float(v[j]);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, float (&v)[32]) {
+    using T = typename Elem<DT>::T;
+    const T* p = (const T*)base + row * ld + n;
+    if (n + 32 <= N && vec >= 16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 u = __ldg((const uint4*)(p + 8 * i));
+            const uint32_t raw[4] = {u.x, u.y, u.z, u.w};
+            float f[8];
+            raw_to_float<DT>(raw, f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[8 * i + j] += f[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (n + j < N) v[j] += Elem<DT>::to_float(p[j]);
+    }
+}
+
+// z = v + bias -> checkpoint of z, y = act(z) + residual -> out.  Called by threads that own (row, n .. n+31).
+template <int DT>
+__device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row, int64_t n, float (&v)[32]) {
+    if (a.bias) add32<DT>(a.bias, 0, a.bvec, 0, n, a.N, v);
+    if (a.zcodes) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            if (n + j >= a.N) v[j] = 0.0f;
+            m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        const uint32_t byte = scale_byte8(m);
+        const float up = scale_up8(byte);
+        const uint64_t at = (uint64_t)row * a.zpitch + n;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            uint32_t c[4];
+            uint4 r;
+            if (a.stochastic) r = noise8(a.rk, at / 8 + i / 2);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float z = v[4 * i + j];
+                c[j] = a.stochastic ? code8_noise(z, up, noise8_at(r, (i & 1) * 4 + j)) : code8(z, up);
+                // ReLU's slope is decided by the sign of z: a positive z keeps a positive code
+                if (a.act == GACT_ACT_RELU && z > 0.0f && (c[j] & 0xffu) == 0u) c[j] = 1u;
+            }
+            w[i] = pack4(c[0], c[1], c[2], c[3]);
+        }
+        if (byte >= top_byte8<GACT_F32>()) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = byte == 255u ? 0u : clamp_codes63(w[i]);
+        }
+        st_v8(a.zcodes + at, w);
+        a.zscales[at >> 5] = (uint8_t)byte;
+    }
+    if (a.z) store32<DT>(a.z, a.N, a.zvec, row, n, a.N, v);
+    if (a.act != GACT_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = act_value(v[j], a.act);
+    }
+    if (a.res) add32<DT>(a.res, a.ldr, a.rvec, row, n, a.N, v);
+    store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
+}
+
+// ---- the matrix product ----------------------------------------------------------------------------------------------
+template <int BN> struct Ring {
+    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kBytes = kStages * kStage + 1024 /* alignment */ + 256 /* barriers */;
+};
+
+struct Unit { int64_t m0, n0; int k0, k1, split; };
+
+// Units (tile x split of the reduction) in an order that keeps concurrently running tiles close together: bands of 16 tile
+// rows, inside a band row by row of columns.
+template <int BN> __device__ __forceinline__ Unit unit_at(const GemmArgs& a, int64_t u) {
+    constexpr int kBand = 16;
+    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+    Unit x;
+    x.split = (int)(u / tiles);
+    const int64_t t = u - x.split * tiles;
+    const int64_t band = t / ((int64_t)kBand * a.tiles_n);
+    const int rows = (int)min((int64_t)kBand, (int64_t)a.tiles_m - band * kBand);
+    const int64_t in = t - band * kBand * a.tiles_n;
+    x.m0 = (band * kBand + in % rows) * kBM;
+    x.n0 = (in / rows) * BN;
+    x.k0 = x.split * a.per_split;
+    x.k1 = min(a.ktiles, x.k0 + a.per_split);
+    return x;
+}
+
+template <int DT, bool A_MN, bool B_MN, int BN, int EPI>
+__global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                            const __grid_constant__ GemmArgs a) {
+    using R = Ring<BN>;
+    constexpr int S = R::kStages;
+    constexpr uint32_t kTmem = 2 * BN < 32 ? 32 : 2 * BN;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t ring = smem_addr(base);
+    uint64_t* bars = (uint64_t*)(base + S * R::kStage);
+    const uint32_t full = smem_addr(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16, drain = acc_empty + 16;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int dead;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        dead = 0;
+        for (int i = 0; i < S; i++) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kEpiWarps); }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+    }
+    if (warp == 2) tmem_alloc(smem_addr(&tmem_slot), kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int64_t u = blockIdx.x; u < units && !dead; u += gridDim.x) {
+                const Unit x = unit_at<BN>(a, u);
+                for (int k = x.k0; k < x.k1; k++, it++) {
+                    const uint32_t s = it % S, ph = (it / S) & 1;
+                    if (!mbar_wait(empty + 8 * s, ph ^ 1, &dead)) break;
+                    const uint32_t bar = full + 8 * s, da = ring + s * R::kStage, db = da + R::kA;
+                    mbar_expect_tx(bar, R::kStage);
+                    if (A_MN) {
+#pragma unroll
+                        for (int i = 0; i < kBM / 64; i++) tma_load_2d(da + i * 8192, &map_a, (int)x.m0 + 64 * i, k * kBK, bar);
+                    } else {
+                        tma_load_2d(da, &map_a, k * kBK, (int)x.m0, bar);
+                    }
+                    if (B_MN) {
+#pragma unroll
+                        for (int i = 0; i < BN / 64; i++) tma_load_2d(db + i * 8192, &map_b, (int)x.n0 + 64 * i, k * kBK, bar);
+                    } else {
+                        tma_load_2d(db, &map_b, k * kBK, (int)x.n0, bar);
+                    }
+                }
+            }
+            if (dead) {
+                // give up in order: the copies that were issued (at most one per stage) land before the block ends
+                atomicExch(&g_linear_error, 1);
+                for (uint32_t j = it > (uint32_t)S ? it - S : 0; j < it; j++)
+                    for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full + 8 * (j % S), (j / S) & 1); i++) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = mma_idesc(kBM, BN, DT == GACT_BF16, A_MN, B_MN);
+            uint32_t it = 0, n = 0;
+            for (int64_t u = blockIdx.x; u < units && !dead; u += gridDim.x, n++) {
+                const Unit x = unit_at<BN>(a, u);
+                const uint32_t acc = n & 1;
+                if (!mbar_wait(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, &dead)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * BN;
+                for (int k = x.k0; k < x.k1; k++, it++) {
+                    const uint32_t s = it % S, ph = (it / S) & 1;
+                    if (!mbar_wait(full + 8 * s, ph, &dead)) break;
+                    tc_fence_after();
+                    const uint32_t sa = ring + s * R::kStage, sb = sa + R::kA;
+#pragma unroll
+                    for (int j = 0; j < kBK / 16; j++) {
+                        const uint64_t da = smem_desc(sa + j * (A_MN ? 2048 : 32), A_MN ? 8192 : 16);
+                        const uint64_t db = smem_desc(sb + j * (B_MN ? 2048 : 32), B_MN ? 8192 : 16);
+                        mma_f16(d, da, db, idesc, (k > x.k0 || j > 0) ? 1u : 0u);
+                    }
+                    mma_commit(empty + 8 * s);
+                }
+                mma_commit(acc_full + 8 * acc);
+            }
+            // every product has finished before TMEM is given back
+            mma_commit(drain);
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(drain, 0); i++) {}
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        uint32_t n = 0;
+        for (int64_t u = blockIdx.x; u < units; u += gridDim.x, n++) {
+            const Unit x = unit_at<BN>(a, u);
+            const uint32_t acc = n & 1;
+            const bool ok = mbar_wait(acc_full + 8 * acc, (n >> 1) & 1, &dead);
+            if (!__all_sync(kFull, ok)) break;
+            tc_fence_after();
+            const int64_t row = x.m0 + q * 32 + lane;
+            constexpr int kSpan = BN / 2;             // columns per warp
+#pragma unroll 1
+            for (int c = 0; c < kSpan; c += 32) {
+                const int64_t col = x.n0 + half * kSpan + c;
+                if (col >= a.N) break;
+                uint32_t r[32];
+                tmem_load32(tmem + ((uint32_t)(q * 32) << 16) + acc * BN + half * kSpan + c, r);
+                if (row < a.M) {
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
+                    if constexpr (EPI == kEpiLinear) {
+                        linear_epilogue32<DT>(a, row, col, v);
+                    } else if constexpr (EPI == kEpiStore) {
+                        store32<DT>(a.out, a.ldo, a.ovec, row, col, a.N, v);
+                    } else {
+                        float* p = a.partial + ((int64_t)x.split * a.M + row) * a.ldp + col;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t w[8] = {r[8 * i], r[8 * i + 1], r[8 * i + 2], r[8 * i + 3], r[8 * i + 4], r[8 * i + 5], r[8 * i + 6], r[8 * i + 7]};
+                            st_v8(p + 8 * i, w);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 2) tmem_free(tmem, kTmem);
+}
+
+// Adds the partial sums of the splits in order and runs the epilogue: one thread per 32 columns of a row.
+template <int DT, int EPI>
+__global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ GemmArgs a) {
+    const int64_t per_row = a.ldp / 32;
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (i >= a.M * per_row) return;
+    const int64_t row = i / per_row, n = (i - row * per_row) * 32;
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = 0.0f;
+    for (int s = 0; s < a.splits; s++) {
+        const float4* p = (const float4*)(a.partial + ((int64_t)s * a.M + row) * a.ldp + n);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float4 f = p[j];
+            v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+        }
+    }
+    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, v);
+    else store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+    static std::atomic<void*> cached{nullptr};
+    void* f = cached.load(std::memory_order_acquire);
+    if (!f) {
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        cached.store(f, std::memory_order_release);
+    }
+    return (EncodeTiled)f;
+}
+
+// rows x cols elements, row pitch ld; tile of 64 elements x `box` rows, 128-byte swizzle, zeros outside
+static bool make_map(CUtensorMap* m, int dtype, const void* p, int64_t rows, int64_t cols, int64_t ld, int box) {
+    EncodeTiled f = encode_tiled();
+    if (!f) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box};
+    const cuuint32_t ones[2] = {1, 1};
+    return f(m, dtype == GACT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)p, dims, strides, boxes, ones,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan { int bn, splits, per_split; int64_t tiles_m, tiles_n; };
+
+// Tile width and splits of the reduction.  (First version: the widest tile, reduction split until the SMs are busy.)
+static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
+    Plan p;
+    const int sms = sm_count();
+    const int64_t kt = (K + kBK - 1) / kBK;
+    p.bn = 256;
+    p.tiles_m = (M + kBM - 1) / kBM;
+    p.tiles_n = (N + p.bn - 1) / p.bn;
+    const int64_t tiles = p.tiles_m * p.tiles_n;
+    int64_t splits = 1;
+    if (tiles * 2 <= sms) {
+        splits = sms / tiles;
+        if (splits > kt / 4) splits = kt / 4;
+        if (splits < 1) splits = 1;
+        if (splits > 16) splits = 16;
+    }
+    p.per_split = (int)((kt + splits - 1) / splits);
+    if (p.per_split < 1) p.per_split = 1;
+    p.splits = (int)((kt + p.per_split - 1) / p.per_split);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+static int64_t gemm_scratch(int64_t M, int64_t N, int64_t K) {
+    const Plan p = plan_gemm(M, N, K);
+    return p.splits > 1 ? (int64_t)p.splits * M * pitch8(N) * 4 : 0;
+}
+
+static int vec_bytes(const void* p, int64_t ld) {
+    const uintptr_t v = (uintptr_t)p | (uintptr_t)(ld * 2);
+    return (v & 31) == 0 ? 32 : (v & 15) == 0 ? 16 : 2;
+}
+
+template <int DT, bool A_MN, bool B_MN, int BN, int EPI>
+static int launch_gemm_kernel(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& a, cudaStream_t s) {
+    auto* k = gemm_kernel<DT, A_MN, B_MN, BN, EPI>;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<BN>::kBytes) != cudaSuccess) return GACT_ERR_LAUNCH;
+    const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+    const int64_t grid = units < sm_count() ? units : sm_count();
+    k<<<(unsigned)grid, kGThreads, Ring<BN>::kBytes, s>>>(ma, mb, a);
+    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+
+// C (M x N) = A B with the reduction over K.  A: K-major (M rows of K) or MN-major (K rows of M); B likewise with N.
+template <int DT, bool A_MN, bool B_MN, bool LINEAR>
+static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, GemmArgs a, void* scratch, cudaStream_t s) {
+    const Plan p = plan_gemm(a.M, a.N, K);
+    CUtensorMap ma, mb;
+    const bool ok = make_map(&ma, DT, A, A_MN ? K : a.M, A_MN ? a.M : K, lda, A_MN ? 64 : kBM) &&
+                    make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn);
+    if (!ok) return GACT_ERR_LAUNCH;
+    a.ktiles = (int)((K + kBK - 1) / kBK);
+    a.tiles_m = (int)p.tiles_m; a.tiles_n = (int)p.tiles_n; a.splits = p.splits; a.per_split = p.per_split;
+    constexpr int kEpi = LINEAR ? kEpiLinear : kEpiStore;
+    if (p.splits == 1) return launch_gemm_kernel<DT, A_MN, B_MN, 256, kEpi>(ma, mb, a, s);
+    a.partial = (float*)scratch;
+    a.ldp = pitch8(a.N);
+    const int st = launch_gemm_kernel<DT, A_MN, B_MN, 256, kEpiPartial>(ma, mb, a, s);
+    if (st != GACT_OK) return st;
+    const int64_t threads = a.M * (a.ldp / 32);
+    gemm_join_kernel<DT, kEpi><<<(unsigned)((threads + 127) / 128), 128, 0, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+
+// ---- dz = dy act'(z'), db = sum dz --------------------------------------------------------------------------------------
+struct ActBwdArgs {
+    const void* dy; int64_t ldy;
+    const void* z; int64_t ldz; const int8_t* codes; const uint8_t* scales; int chunks;
+    int act; int64_t rows; int cols;
+    void* dz; int64_t ldo;
+    float* partial; int width;
+};
+constexpr int kAWarps = 8;
+
+// A warp owns 256 columns (8 per lane) and walks rows; eight warps of a block take eight rows at a time.
+template <int DT, bool VEC, bool COMP, bool ACT>
+__global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid_constant__ ActBwdArgs a) {
+    using T = typename Elem<DT>::T;
+    __shared__ float fold[kAWarps][8][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int col = (blockIdx.x * 32 + lane) * 8;
+    float db[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) db[j] = 0.0f;
+    const int64_t step = (int64_t)gridDim.y * kAWarps;
+    constexpr int U = 2;
+    for (int64_t r = (int64_t)blockIdx.y * kAWarps + warp; r < a.rows; r += U * step) {
+        float g[U][8], z[U][8];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t row = r + u * step;
+            const int cols = row < a.rows ? a.cols : 0;
+            load_row8<DT, VEC>((const T*)a.dy + row * a.ldy, col, cols, g[u]);
+            if constexpr (ACT) {
+                if constexpr (COMP) {
+                    uint2 q = make_uint2(0u, 0u);
+                    uint32_t byte = 1;
+                    if (col < cols) {
+                        const int64_t chunk = row * a.chunks + (col >> 3);
+                        q = ld_stream_u2(a.codes + chunk * 8);
+                        byte = a.scales[chunk >> 2];
+                    }
+                    restore8(q, scale_down8(byte), z[u]);
+                } else {
+                    load_row8<DT, VEC>((const T*)a.z + row * a.ldz, col, cols, z[u]);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t row = r + u * step;
+            if constexpr (ACT) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) g[u][j] *= act_slope(z[u][j], a.act);
+                store_row8<DT, VEC>((T*)a.dz + row * a.ldo, col, row < a.rows ? a.cols : 0, g[u]);
+            }
+            if (row < a.rows) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) db[j] += g[u][j];
+            }
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int j = 0; j < 8; j++) fold[warp][j][lane] = db[j];
+    __syncthreads();
+    // thread (j, lane): column blockIdx.x * 256 + lane * 8 + j
+    const int j = threadIdx.x & 7, l = threadIdx.x >> 3;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAWarps; w++) sum += fold[w][j][l];
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < a.width) a.partial[(int64_t)blockIdx.y * a.width + c] = sum;
+}
+
+static int64_t act_bwd_parts(int64_t rows, int64_t cols) {
+    const int64_t strips = (cols + 255) / 256;
+    int64_t parts = ((int64_t)sm_count() * 8 + strips - 1) / strips;
+    const int64_t most = (rows + kAWarps - 1) / kAWarps;
+    if (parts > most) parts = most;
+    return parts < 1 ? 1 : parts > 65535 ? 65535 : parts;
+}
+
+template <int DT> static void dispatch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
+    const int block = kAWarps * 32;
+    if (a.act == GACT_ACT_NONE) {
+        if (vec) act_backward_kernel<DT, true, false, false><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, false><<<grid, block, 0, s>>>(a);
+    } else if (a.codes) {
+        if (vec) act_backward_kernel<DT, true, true, true><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, true, true><<<grid, block, 0, s>>>(a);
+    } else {
+        if (vec) act_backward_kernel<DT, true, false, true><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, true><<<grid, block, 0, s>>>(a);
+    }
+}
+
+static bool dims_ok(int64_t rows, int64_t cin, int64_t cout) {
+    return rows >= 0 && cin >= 1 && cout >= 1 && cin <= GACT_MAX_COLS && cout <= GACT_MAX_COLS && rows <= (1LL << 30) &&
+           rows <= GACT_MAX_ELEMENTS / pitch8(cin) && rows <= GACT_MAX_ELEMENTS / pitch8(cout);
+}
+// operands of the products are read by tensor maps: 16-byte aligned base and row pitch
+static bool map_ok(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+
+int linear_error_word() {
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_linear_error, sizeof(int)) == cudaSuccess ? v : -1;
+}
+int linear_error_clear() {
+    const int zero = 0;
+    return cudaMemcpyToSymbol(g_linear_error, &zero, sizeof(int)) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+
+}  // namespace gact
+
+using namespace gact;
+
+extern "C" int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t cout, int direction) {
+    if (!dims_ok(rows, cin, cout) || direction < 0 || direction > 2) return -1;
+    if (rows == 0) return 0;
+    return direction == 0 ? gemm_scratch(rows, cout, cin) : direction == 1 ? gemm_scratch(rows, cin, cout) : gemm_scratch(cout, cin, rows);
+}
+
+extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
+                           int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* z, void* zcodes, void* zscales,
+                           int stochastic, uint64_t seed, void* scratch, void* stream) {
+    if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
+    if (act < GACT_ACT_NONE || act > GACT_ACT_SILU) return GACT_ERR_MODE;
+    if (!dims_ok(rows, cin, cout) || ld_x < cin || ld_w < cin || (residual && ld_res < cout)) return GACT_ERR_SIZE;
+    if (rows == 0) return GACT_OK;
+    if (!x || !weight || !y || (zcodes && !zscales)) return GACT_ERR_NULL;
+    if (!map_ok(x, ld_x) || !map_ok(weight, ld_w) || (((uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)residual) & 1) ||
+        ((uintptr_t)zcodes & 31) || ((uintptr_t)scratch & 31))
+        return GACT_ERR_ALIGN;
+    if (gemm_scratch(rows, cout, cin) && !scratch) return GACT_ERR_NULL;
+    GemmArgs a = {};
+    a.M = rows; a.N = cout; a.out = y; a.ldo = cout; a.ovec = vec_bytes(y, cout);
+    a.bias = bias; a.bvec = vec_bytes(bias, 0);
+    a.res = residual; a.ldr = ld_res; a.rvec = vec_bytes(residual, ld_res);
+    a.act = act; a.z = z; a.zvec = vec_bytes(z, cout);
+    a.zcodes = (int8_t*)zcodes; a.zscales = (uint8_t*)zscales; a.zpitch = pitch8(cout);
+    a.stochastic = stochastic; a.rk = philox_round_keys(seed);
+    cudaStream_t s = (cudaStream_t)stream;
+    return dtype == GACT_F16 ? run_gemm<GACT_F16, false, false, true>(x, ld_x, weight, ld_w, cin, a, scratch, s)
+                             : run_gemm<GACT_BF16, false, false, true>(x, ld_x, weight, ld_w, cin, a, scratch, s);
+}
+
+extern "C" int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weight, int64_t ld_w, int dtype, int64_t rows, int64_t cin, int64_t cout,
+                                 void* dx, void* scratch, void* stream) {
+    if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
+    if (!dims_ok(rows, cin, cout) || ld_dz < cout || ld_w < cin) return GACT_ERR_SIZE;
+    if (rows == 0) return GACT_OK;
+    if (!dz || !weight || !dx || (gemm_scratch(rows, cin, cout) && !scratch)) return GACT_ERR_NULL;
+    if (!map_ok(dz, ld_dz) || !map_ok(weight, ld_w) || ((uintptr_t)dx & 1) || ((uintptr_t)scratch & 31)) return GACT_ERR_ALIGN;
+    GemmArgs a = {};
+    a.M = rows; a.N = cin; a.out = dx; a.ldo = cin; a.ovec = vec_bytes(dx, cin);
+    cudaStream_t s = (cudaStream_t)stream;
+    return dtype == GACT_F16 ? run_gemm<GACT_F16, false, true, false>(dz, ld_dz, weight, ld_w, cout, a, scratch, s)
+                             : run_gemm<GACT_BF16, false, true, false>(dz, ld_dz, weight, ld_w, cout, a, scratch, s);
+}
+
+extern "C" int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cin, int64_t cout,
+                                 void* dweight, void* scratch, void* stream) {
+    if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
+    if (!dims_ok(rows, cin, cout) || ld_dz < cout || ld_x < cin) return GACT_ERR_SIZE;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (!dweight) return GACT_ERR_NULL;
+    if (rows == 0) return cudaMemsetAsync(dweight, 0, (size_t)(cin * cout * 2), s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+    if (!dz || !x || (gemm_scratch(cout, cin, rows) && !scratch)) return GACT_ERR_NULL;
+    if (!map_ok(dz, ld_dz) || !map_ok(x, ld_x) || ((uintptr_t)dweight & 1) || ((uintptr_t)scratch & 31)) return GACT_ERR_ALIGN;
+    GemmArgs a = {};
+    a.M = cout; a.N = cin; a.out = dweight; a.ldo = cin; a.ovec = vec_bytes(dweight, cin);
+    return dtype == GACT_F16 ? run_gemm<GACT_F16, true, true, false>(dz, ld_dz, x, ld_x, rows, a, scratch, s)
+                             : run_gemm<GACT_BF16, true, true, false>(dz, ld_dz, x, ld_x, rows, a, scratch, s);
+}
+
+extern "C" int64_t gact_act_backward_scratch_bytes(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 1 || cols > GACT_MAX_COLS) return -1;
+    return act_bwd_parts(rows, cols) * ((cols + 7) / 8 * 8) * (int64_t)sizeof(float);
+}
+
+extern "C" int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, int act, const void* z, int64_t ld_z,
+                                 const void* zcodes, const void* zscales, void* dz, int64_t ld_dz, void* dbias, void* scratch, void* stream) {
+    if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
+    if (act < GACT_ACT_NONE || act > GACT_ACT_SILU) return GACT_ERR_MODE;
+    if (rows < 0 || cols < 1 || cols > GACT_MAX_COLS || rows > GACT_MAX_ELEMENTS / pitch8(cols) || ld_dy < cols || (z && ld_z < cols) ||
+        (dz && ld_dz < cols))
+        return GACT_ERR_SIZE;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (rows == 0) return !dbias || cudaMemsetAsync(dbias, 0, (size_t)cols * 2, s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+    if (!dy || (act != GACT_ACT_NONE && (!dz || (!z && (!zcodes || !zscales)))) || (dbias && !scratch)) return GACT_ERR_NULL;
+    if (act == GACT_ACT_NONE && !dbias) return GACT_OK;
+    if ((((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)dbias) & 1) || ((uintptr_t)zcodes & 31) || ((uintptr_t)scratch & 15)) return GACT_ERR_ALIGN;
+    ActBwdArgs a;
+    a.dy = dy; a.ldy = ld_dy; a.z = z; a.ldz = ld_z; a.codes = z ? nullptr : (const int8_t*)zcodes; a.scales = (const uint8_t*)zscales;
+    a.chunks = (int)(pitch8(cols) / 8); a.act = act; a.rows = rows; a.cols = (int)cols; a.dz = dz; a.ldo = ld_dz;
+    a.partial = dbias ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
+    const bool vec = rows_aligned(dy, ld_dy, cols, 2) && (act == GACT_ACT_NONE || ((!z || rows_aligned(z, ld_z, cols, 2)) && rows_aligned(dz, ld_dz, cols, 2)));
+    const int64_t parts = act_bwd_parts(rows, cols);
+    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)parts);
+    if (dtype == GACT_F16) dispatch_act_bwd<GACT_F16>(a, vec, grid, s);
+    else dispatch_act_bwd<GACT_BF16>(a, vec, grid, s);
+    if (cudaGetLastError() != cudaSuccess) return GACT_ERR_LAUNCH;
+    return dbias ? reduce_columns((const float*)scratch, (int)parts, a.width, dbias, cols, nullptr, 0, dtype, s) : GACT_OK;
+}

@@ -720,6 +720,10 @@ int launch_quantize16(const QuantArgs& a, int dtype, int bits, int rng, cudaStre
     return dtype == GACT_F16 ? dispatch_bits16<GACT_F16>(a, bits, rng, s) : dispatch_bits16<GACT_BF16>(a, bits, rng, s);
 }
 
+// the error word of the linear layers' pipeline (linear.cu)
+int linear_error_word();
+int linear_error_clear();
+
 }  // namespace gact
 
 using namespace gact;
@@ -727,10 +731,11 @@ using namespace gact;
 extern "C" int gact_pipeline_error(void) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_pipeline_error, sizeof(int)) != cudaSuccess) return -1;
-    return v;
+    return v ? v : linear_error_word();
 }
 
 extern "C" int gact_pipeline_error_reset(void) {
     const int zero = 0;
-    return cudaMemcpyToSymbol(g_pipeline_error, &zero, sizeof(int)) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+    if (cudaMemcpyToSymbol(g_pipeline_error, &zero, sizeof(int)) != cudaSuccess) return GACT_ERR_LAUNCH;
+    return linear_error_clear();
 }

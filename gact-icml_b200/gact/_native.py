@@ -16,6 +16,8 @@ LIB_PATH = _HERE / "libgact_b200.so"
 F32, F16, BF16 = 0, 1, 2
 DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 RNG_CURAND, RNG_FAST, RNG_RTN, RNG_EXTERNAL = 0, 1, 2, 3
+ACT_CODE = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+BLOCK8 = 32
 RNG_CODE = {"curand": RNG_CURAND, "fast": RNG_FAST, "rtn": RNG_RTN, "external": RNG_EXTERNAL}
 GROUP = 256
 
@@ -47,6 +49,19 @@ _SIGNATURES = {
     "gact_sensitivity": ([_vp, _d, _vp, _i, _vp], _i),
     "gact_calc_precision": ([_vp, _vp, _vp, _i, _d, _vp, _vp], _i),
     "gact_calc_precision_host": ([_vp, _vp, _vp, _i, _d], _i),
+    "gact_checkpoint8_pitch": ([_i64], _i64),
+    "gact_checkpoint8": ([_vp, _i, _i64, _i64, _i64, _i, _u64, _vp, _vp, _vp], _i),
+    "gact_restore8": ([_vp, _vp, _i64, _i64, _i, _vp, _i64, _vp], _i),
+    "gact_repitch16": ([_vp, _i64, _i64, _i64, _vp, _i64, _vp], _i),
+    "gact_layer_norm": ([_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _d, _vp, _vp, _vp, _vp, _vp, _i, _u64, _vp], _i),
+    "gact_layer_norm_backward_scratch_bytes": ([_i64, _i64], _i64),
+    "gact_layer_norm_backward": ([_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
+    "gact_linear_scratch_bytes": ([_i64, _i64, _i64, _i], _i64),
+    "gact_linear": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _i, _u64, _vp, _vp], _i),
+    "gact_linear_dgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp], _i),
+    "gact_linear_wgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp], _i),
+    "gact_act_backward_scratch_bytes": ([_i64, _i64], _i64),
+    "gact_act_backward": ([_vp, _i, _i64, _i64, _i64, _i, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp], _i),
 }
 for _name, (_args, _res) in _SIGNATURES.items():
     _fn = getattr(lib, _name)
@@ -88,8 +103,8 @@ def check_pipeline(where: str) -> None:
     err = lib.gact_pipeline_error()
     if err > 0:
         lib.gact_pipeline_error_reset()
-        raise GactError(f"{where}: a bulk copy of gact_quantize did not arrive within its wait limit "
-                        f"(pipeline error {err}); compressed activations of this step are incomplete")
+        raise GactError(f"{where}: a copy of the quantize or linear pipeline did not arrive within its wait limit "
+                        f"(pipeline error {err}); compressed activations or products of this step are incomplete")
 
 
 def require_cuda(t: torch.Tensor, name: str) -> None:

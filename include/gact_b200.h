@@ -89,6 +89,8 @@ int gact_quantize(const void* x, int dtype, int64_t n, int bits, uint64_t seed, 
  * The fp16 / bf16 kernel of gact_quantize stages its input through shared memory with bulk copies and waits for
  * them on mbarriers.  Every such wait is bounded; a wait that runs out makes the warp record an error and leave
  * (the tiles it had not written keep whatever the output buffers held), so a launch can never spin forever.
+ * The products of gact_linear, gact_linear_dgrad and gact_linear_wgrad wait for their tiles in the same bounded way and
+ * report through the same two functions.
  * gact_pipeline_error: 0 while no wait has ever run out on the current device, non-zero afterwards (sticky);
  * -1 if the word could not be read.  gact_pipeline_error_reset: clears it.  Both synchronise with the device,
  * so call them where the host waits anyway (the Python layer does so once per adaptation and when the hooks
@@ -225,6 +227,84 @@ int gact_calc_precision(int32_t* b, const float* C, const int64_t* w, int L, dou
  * GACT_ERR_BUDGET.
  */
 int gact_calc_precision_host(int32_t* b, const float* C, const int64_t* w, int L, double target);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Training operators that keep their own activations as 8-bit checkpoints (no counterpart in the reference, which
+ * restores every saved tensor before a library kernel reads it).
+ *
+ * Checkpoint format.  A row-major tensor of `rows` x `cols` is cut along its rows into blocks of 32 elements (the last
+ * block of a row may be short).  A block stores a scale byte b, the biased exponent of a power of two, and 32 signed
+ * codes: code = rint(x * 2^(127-b)), restored value = code * 2^(b-127).  b is the smallest exponent (at least 1) for which
+ * the largest |x| stays below 127 steps; b = 255 marks a block that held a NaN or an infinity, all of it restores to NaN.
+ * codes: int8[rows][pitch], pitch = gact_checkpoint8_pitch(cols) = cols rounded up to 32, codes past `cols` are 0;
+ * scales: uint8[rows][pitch / 32].  In the highest binade of the type codes stop at +-63 (64 would restore out of range).
+ * stochastic != 0: code = floor(x * 2^(127-b) + u) with u in (0,1) from Philox4x32-7 keyed by `seed`, counter = index of
+ * the element's group of 8 in the padded layout, 16 bits each; the restored value is then unbiased.
+ *
+ * Sizes: cols (and the features of a linear layer) at most GACT_MAX_COLS, rows * pitch at most GACT_MAX_ELEMENTS, layer
+ * norm rows of at most GACT_LAYER_NORM_MAX_COLS.  `ld` arguments are row pitches in elements (>= the row length).
+ * codes must be 32-byte aligned, scratch 32-byte aligned, everything else aligned to its element size unless noted.
+ * Scratch belongs to the caller; calls that overlap on the GPU must not share it.
+ * ------------------------------------------------------------------------------------------------------------------ */
+#define GACT_BLOCK8 32
+#define GACT_MAX_COLS (1LL << 24)
+#define GACT_MAX_ELEMENTS (1LL << 38)
+#define GACT_LAYER_NORM_MAX_COLS 16384
+
+/* activations of gact_linear; GELU is the erf form, GELU_TANH its tanh approximation */
+enum { GACT_ACT_NONE = 0, GACT_ACT_RELU = 1, GACT_ACT_GELU = 2, GACT_ACT_GELU_TANH = 3, GACT_ACT_SILU = 4 };
+
+int64_t gact_checkpoint8_pitch(int64_t cols);
+int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int stochastic, uint64_t seed,
+                     void* codes, void* scales, void* stream);
+int gact_restore8(const void* codes, const void* scales, int64_t rows, int64_t cols, int dtype, void* out, int64_t ld,
+                  void* stream);
+
+/* Copies rows of 16-bit elements to another row pitch (columns past `cols` of dst are left as they are). */
+int gact_repitch16(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ld_dst, void* stream);
+
+/*
+ * Layer norm over rows of `cols`: y = (x - mean) / sqrt(var + eps) * weight + bias; weight / bias may be null, their type
+ * is `param_dtype` (that of x, or GACT_F32).  y is contiguous.  mean / rstd (both or neither): fp32 per row, for the
+ * backward pass.  codes / scales (optional): checkpoint of x, made in the same pass.
+ */
+int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight, const void* bias,
+                    int param_dtype, double eps, void* y, float* mean, float* rstd, void* codes, void* scales, int stochastic,
+                    uint64_t seed, void* stream);
+/*
+ * Its backward pass from x, or (x null) from the checkpoint of x.  dx (contiguous), dweight, dbias: each may be null.
+ * Sums over rows are added in a fixed order (no atomics).  scratch: only with dweight or dbias.
+ */
+int64_t gact_layer_norm_backward_scratch_bytes(int64_t rows, int64_t cols);
+int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, const void* x, int64_t ld_x,
+                             const void* codes, const void* scales, const float* mean, const float* rstd, const void* weight,
+                             int param_dtype, void* dx, void* dweight, void* dbias, void* scratch, void* stream);
+
+/*
+ * y = act(x W^T + bias) + residual for fp16 / bf16, fp32 accumulation; weight is [cout][cin].  x and weight: base and row
+ * pitch multiples of 16 bytes (gact_repitch16 makes such a copy).  bias, residual: may be null.  y: contiguous.
+ * Kept for the backward pass, each optional: z (pre-activation rounded to `dtype`, contiguous), or zcodes / zscales (its
+ * checkpoint, made from the fp32 value; with GACT_ACT_RELU a positive pre-activation keeps a positive code).
+ * scratch: gact_linear_scratch_bytes(rows, cin, cout, direction) bytes (0: none needed), direction 0 = forward,
+ * 1 = data gradient, 2 = weight gradient.
+ */
+int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t cout, int direction);
+int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
+                int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* z, void* zcodes, void* zscales,
+                int stochastic, uint64_t seed, void* scratch, void* stream);
+/* dx = dz W (contiguous).  dz and weight: base and row pitch multiples of 16 bytes. */
+int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weight, int64_t ld_w, int dtype, int64_t rows, int64_t cin,
+                      int64_t cout, void* dx, void* scratch, void* stream);
+/* dW = dz^T x (contiguous [cout][cin]).  dz and x: base and row pitch multiples of 16 bytes. */
+int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cin,
+                      int64_t cout, void* dweight, void* scratch, void* stream);
+/*
+ * dz = dy act'(z) with z given as a tensor or (z null) as a checkpoint, and dbias = sum of dz over the rows, summed from
+ * the unrounded products.  GACT_ACT_NONE: only the sum (dz is dy).  dbias may be null (then no scratch).
+ */
+int64_t gact_act_backward_scratch_bytes(int64_t rows, int64_t cols);
+int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, int act, const void* z, int64_t ld_z,
+                      const void* zcodes, const void* zscales, void* dz, int64_t ld_dz, void* dbias, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }
