@@ -13,6 +13,8 @@
 // of range: there magnitudes stop at 63 steps.
 #pragma once
 
+#include <type_traits>
+
 #include "gact_common.cuh"
 
 namespace gact {
@@ -65,74 +67,7 @@ static __device__ __noinline__ uint32_t clamp_codes63(uint32_t w) {
     return out;
 }
 
-// Four codes -> four floats: the byte with its sign bit flipped goes into the mantissa of 2^23 (offset binary), one
-// subtraction takes the offset off again, one multiplication applies the power of two; all exact.
-__device__ __forceinline__ void restore4(uint32_t w, float down, float (&v)[4]) {
-    w ^= 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        v[i] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | i)), 8388736.0f), down);
-}
-__device__ __forceinline__ void restore8(uint2 w, float down, float (&v)[8]) {
-    float a[4], b[4];
-    restore4(w.x, down, a);
-    restore4(w.y, down, b);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
-}
-
-// The codes of 8 consecutive elements (chunk `c` of a row), computed by 4 neighbouring lanes per block; every lane of
-// the warp must call.  Returns the scale byte too.  Chunks past the row's end hold zeros.
-template <int DT, bool STOCH>
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], const PhiloxKeys& rk, uint64_t chunk, uint32_t& byte) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(kFull, m, 1));
-    m = max(m, __shfl_xor_sync(kFull, m, 2));
-    byte = scale_byte8(m);
-    const float up = scale_up8(byte);
-    uint32_t c[8];
-    if constexpr (STOCH) {
-        const uint4 r = noise8(rk, chunk);
-#pragma unroll
-        for (int j = 0; j < 8; j++) c[j] = code8_noise(v[j], up, noise8_at(r, j));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) c[j] = code8(v[j], up);
-    }
-    uint2 w = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-    if (byte >= top_byte8<DT>()) {
-        if (byte == 255u) w = make_uint2(0u, 0u);
-        else w = make_uint2(clamp_codes63(w.x), clamp_codes63(w.y));
-    }
-    return w;
-}
-
-// ---- eight consecutive elements of a row --------------------------------------------------------------------------
-// VEC: rows start on 16-byte boundaries and hold a multiple of 8 elements; otherwise element by element.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_row8(const typename Elem<DT>::T* row, int col, int cols, float (&v)[8]) {
-    if constexpr (VEC) {
-        uint32_t raw[RawRegs<DT>::N];
-        if (col < cols) {
-            const uint4 a = ld_stream_u4(row + col);
-            raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
-            if constexpr (DT == GACT_F32) {
-                const uint4 b = ld_stream_u4(row + col + 4);
-                raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < RawRegs<DT>::N; i++) raw[i] = 0;
-        }
-        raw_to_float<DT>(raw, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = (col + j < cols) ? Elem<DT>::to_float(row[col + j]) : 0.0f;
-    }
-}
-
+// ---- eight consecutive elements of a row, as four pairs (two fp32 operations per instruction) -----------------------
 template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (DT == GACT_F16) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -142,23 +77,182 @@ template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return *(const uint32_t*)&h;
     }
 }
+template <int DT> __device__ __forceinline__ void raw_to_pairs(const uint32_t (&raw)[RawRegs<DT>::N], float2 (&v)[4]) {
+    float f[8];
+    raw_to_float<DT>(raw, f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
+}
+template <int DT> __device__ __forceinline__ void pairs_to_raw(const float2 (&v)[4], uint32_t (&raw)[RawRegs<DT>::N]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (DT == GACT_F32) { raw[2 * i] = __float_as_uint(v[i].x); raw[2 * i + 1] = __float_as_uint(v[i].y); }
+        else raw[i] = pack2<DT>(v[i].x, v[i].y);
+    }
+}
+// the largest magnitude of the eight, as an fp32 bit pattern
+template <int DT> __device__ __forceinline__ uint32_t absmax8(const uint32_t (&raw)[RawRegs<DT>::N]) {
+    uint32_t m;
+    if constexpr (DT == GACT_F32) {
+        m = raw[0] & 0x7fffffffu;
+#pragma unroll
+        for (int i = 1; i < 8; i++) m = max(m, raw[i] & 0x7fffffffu);
+    } else if constexpr (DT == GACT_BF16) {
+        // |.| of two at a time, NaN kept; the sign of the result is the xor of both and is dropped at the end
+        asm("{ .reg .b32 a, b; max.NaN.xorsign.abs.bf16x2 a, %1, %2; max.NaN.xorsign.abs.bf16x2 b, %3, %4; max.NaN.xorsign.abs.bf16x2 %0, a, b; }"
+            : "=r"(m) : "r"(raw[0]), "r"(raw[1]), "r"(raw[2]), "r"(raw[3]));
+        m = max((m << 16) & 0x7fffffffu, m & 0x7fff0000u);
+    } else {
+        asm("{ .reg .b32 a, b; max.NaN.xorsign.abs.f16x2 a, %1, %2; max.NaN.xorsign.abs.f16x2 b, %3, %4; max.NaN.xorsign.abs.f16x2 %0, a, b; }"
+            : "=r"(m) : "r"(raw[0]), "r"(raw[1]), "r"(raw[2]), "r"(raw[3]));
+        const float2 f = __half22float2(*(const __half2*)&m);
+        m = max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu);
+    }
+    return m;
+}
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void store_row8(typename Elem<DT>::T* row, int col, int cols, const float (&v)[8]) {
-    if constexpr (VEC) {
-        if (col < cols) {
-            if constexpr (DT == GACT_F32) {
-                st_stream_u4(row + col, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
-                st_stream_u4(row + col + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
-            } else {
-                st_stream_u4(row + col, make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])));
-            }
+// The codes of 8 consecutive elements (chunk number `chunk` of the padded rows); a block of 32 lies in 4 neighbouring
+// lanes and every lane of the warp must call.  `m`: the lane's largest magnitude.  Returns the scale byte too.
+template <int DT, bool STOCH>
+__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const PhiloxKeys& rk, uint64_t chunk, uint32_t& byte) {
+    m = max(m, __shfl_xor_sync(kFull, m, 1));
+    m = max(m, __shfl_xor_sync(kFull, m, 2));
+    byte = scale_byte8(m);
+    const float up = scale_up8(byte);
+    uint32_t c[8];
+    if constexpr (STOCH) {
+        const uint4 r = noise8(rk, chunk);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[2 * i] = code8_noise(v[i].x, up, noise8_at(r, 2 * i));
+            c[2 * i + 1] = code8_noise(v[i].y, up, noise8_at(r, 2 * i + 1));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (col + j < cols) row[col + j] = Elem<DT>::from_float(v[j]);
+        for (int i = 0; i < 4; i++) {
+            const float2 t = fma2(v[i], splat2(up), splat2(12582912.0f));
+            c[2 * i] = __float_as_uint(t.x);
+            c[2 * i + 1] = __float_as_uint(t.y);
+        }
     }
+    uint2 w = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+    if (byte >= top_byte8<DT>()) {
+        if (byte == 255u) w = make_uint2(0u, 0u);
+        else w = make_uint2(clamp_codes63(w.x), clamp_codes63(w.y));
+    }
+    return w;
+}
+// eight codes as integers in fp32 (exact): the byte with its sign bit flipped goes into the mantissa of 2^23 (offset
+// binary), one subtraction takes the offset off again
+__device__ __forceinline__ void code_pairs(uint2 w, float2 (&v)[4]) {
+    const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t q = i < 2 ? a : b;
+        v[i] = add2(make_float2(__uint_as_float(__byte_perm(q, 0x4b000000u, 0x7540 | (2 * (i & 1)))),
+                                __uint_as_float(__byte_perm(q, 0x4b000000u, 0x7540 | (2 * (i & 1) + 1)))),
+                    splat2(-8388736.0f));
+    }
+}
+__device__ __forceinline__ void restore_pairs(uint2 w, float down, float2 (&v)[4]) {
+    code_pairs(w, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = mul2(v[i], splat2(down));
+}
+
+// A lane's 8 elements of a row, from memory.  VEC: rows start on 16-byte boundaries and hold a multiple of 8 elements,
+// one or two 16-byte accesses.  Otherwise a warp reads its 32 x 8 elements one lane-contiguous 32 at a time and turns
+// them around in shared memory (8 elements per lane straight from memory would touch every sector eight times).
+// SUB lanes of the warp share a row (32: the whole warp); rows of the lane groups follow one another.
+template <int DT, bool VEC, int SUB> struct Row8 {
+    using T = typename Elem<DT>::T;
+    using U = typename std::conditional<DT == GACT_F32, uint32_t, uint16_t>::type;
+    static constexpr int N = VEC ? RawRegs<DT>::N : 8;
+    uint32_t r[N];
+
+    // base + row * ld: the row of this lane's group; col: the lane's first column; nothing is read at or past `cols`
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row, int64_t rows, int col, int cols) {
+        if constexpr (VEC) {
+            if (row < rows && col < cols) {
+                const T* p = base + row * ld + col;
+                const uint4 a = ld_stream_u4(p);
+                r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+                if constexpr (DT == GACT_F32) {
+                    const uint4 b = ld_stream_u4(p + 4);
+                    r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) r[i] = 0;
+            }
+        } else {
+            const int lane = threadIdx.x & 31;
+            const int64_t row0 = row - lane / SUB;
+            const int col0 = col - (lane % SUB) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int e = i * 32 + lane, g = e / (SUB * 8), c = col0 + e % (SUB * 8);
+                r[i] = (row0 + g < rows && c < cols) ? (uint32_t)__ldg((const U*)base + (row0 + g) * ld + c) : 0u;
+            }
+        }
+    }
+    // the elements in storage format; `stage`: 256 elements of the warp (not used with VEC)
+    __device__ __forceinline__ void get(void* stage, uint32_t (&raw)[RawRegs<DT>::N]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < N; i++) raw[i] = r[i];
+        } else {
+            const int lane = threadIdx.x & 31;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; i++) ((U*)stage)[i * 32 + lane] = (U)r[i];
+            __syncwarp();
+            const uint4 a = ((const uint4*)stage)[DT == GACT_F32 ? 2 * lane : lane];
+            raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+            if constexpr (DT == GACT_F32) {
+                const uint4 b = ((const uint4*)stage)[2 * lane + 1];
+                raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T* base, int64_t ld, int64_t row, int64_t rows, int col, int cols, void* stage, const float2 (&v)[4]) {
+        uint32_t raw[RawRegs<DT>::N];
+        pairs_to_raw<DT>(v, raw);
+        if constexpr (VEC) {
+            if (row < rows && col < cols) {
+                T* p = base + row * ld + col;
+                st_stream_u4(p, make_uint4(raw[0], raw[1], raw[2], raw[3]));
+                if constexpr (DT == GACT_F32) st_stream_u4(p + 4, make_uint4(raw[4], raw[5], raw[6], raw[7]));
+            }
+        } else {
+            const int lane = threadIdx.x & 31;
+            const int64_t row0 = row - lane / SUB;
+            const int col0 = col - (lane % SUB) * 8;
+            __syncwarp();
+            ((uint4*)stage)[DT == GACT_F32 ? 2 * lane : lane] = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+            if constexpr (DT == GACT_F32) ((uint4*)stage)[2 * lane + 1] = make_uint4(raw[4], raw[5], raw[6], raw[7]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int e = i * 32 + lane, g = e / (SUB * 8), c = col0 + e % (SUB * 8);
+                if (row0 + g < rows && c < cols) ((U*)base)[(row0 + g) * ld + c] = ((const U*)stage)[e];
+            }
+        }
+    }
+};
+// bytes of shared memory per warp that Row8 needs
+template <int DT, bool VEC> struct Stage8 { static constexpr int kBytes = VEC ? 0 : 256 * Elem<DT>::kBytes; };
+
+// Blocks of a kernel that one SM holds, asked of the runtime once per device.
+template <class K> static inline int resident_blocks(K kernel, int threads, size_t smem, std::atomic<int> (&cache)[kMaxDevices]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 1;
+    int n = cache[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
+        cache[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 static inline bool rows_aligned(const void* p, int64_t ld, int64_t cols, int elem_bytes) {

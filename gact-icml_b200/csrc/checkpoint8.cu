@@ -5,74 +5,130 @@ namespace gact {
 
 constexpr int kCThreads = 256;
 
+// Division by a number known at launch: for i < 2^31 one multiplication, i / d = i * mul >> (31 + s) with s = ceil(log2 d)
+// and mul = floor(2^(31+s) / d) + 1 < 2^32 (the excess mul * d - 2^(31+s) is at most d <= 2^s, so the error stays below 1 / d).
+// Larger indices take the 64-bit division (a hundred instructions, which would bound the kernel).
+struct Divisor {
+    uint32_t mul, shift; int64_t d;
+    static Divisor of(int64_t d) {
+        Divisor v;
+        int s = 0;
+        while ((1LL << s) < d) s++;
+        v.mul = (uint32_t)((1ULL << (31 + s)) / (uint64_t)d + 1);
+        v.shift = 31 + s;
+        v.d = d;
+        return v;
+    }
+    __device__ __forceinline__ int64_t div(int64_t i) const {
+        return i < (1LL << 31) ? (int64_t)(((uint64_t)(uint32_t)i * mul) >> shift) : i / d;
+    }
+};
+
 struct Ckpt8Args {
     const void* x; int64_t ld; int64_t rows; int cols;
     int8_t* codes; uint8_t* scales;
     int chunks;               // chunks of 8 elements per padded row
+    int tiles;                // tiles of 256 columns per row
+    Divisor by;               // chunks or tiles of a row, by the way the kernel walks
     PhiloxKeys rk;
 };
+struct Restore8Args {
+    const int8_t* codes; const uint8_t* scales;
+    int64_t rows; int cols; int chunks; int tiles; Divisor by;
+    void* out; int64_t ld;
+};
 
-// A thread takes 8 consecutive elements, 4 neighbouring lanes a block.  U chunks per thread are loaded before the first
-// is worked on.  Chunks are numbered through all padded rows, so a warp's accesses are contiguous whatever the row length.
-template <int DT, bool VEC, bool STOCH, int U>
+// A thread takes 8 consecutive elements, 4 neighbouring lanes a block of 32.
+//   FLAT: chunks are numbered through all padded rows, so a warp's accesses are contiguous whatever the row length.
+//   else: a warp takes 256 columns of a row (rows that do not start on 16-byte boundaries: one division per warp, and the
+//         element-wise accesses of Row8 run along the row).
+// U chunks per thread are loaded before the first is worked on.
+template <bool FLAT, int U> struct Walk {
+    int64_t chunk[U], row[U];
+    int col[U];
+    __device__ __forceinline__ Walk(int64_t rows, int chunks, int tiles, const Divisor& by) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (FLAT) {
+                const int64_t i = (int64_t)blockIdx.x * (kCThreads * U) + u * kCThreads + threadIdx.x;
+                row[u] = by.div(i);
+                col[u] = (int)(i - row[u] * chunks) * 8;
+                chunk[u] = row[u] < rows ? i : -1;
+            } else {
+                const int64_t w = (int64_t)blockIdx.x * (kCThreads / 32 * U) + u * (kCThreads / 32) + (threadIdx.x >> 5);
+                row[u] = by.div(w);
+                const int c = (int)(w - row[u] * tiles) * 32 + (threadIdx.x & 31);
+                col[u] = c * 8;
+                chunk[u] = (row[u] < rows && c < chunks) ? row[u] * chunks + c : -1;
+            }
+        }
+    }
+};
+
+template <int DT, bool VEC, bool FLAT, bool STOCH, int U>
 __global__ void __launch_bounds__(kCThreads) checkpoint8_kernel(const __grid_constant__ Ckpt8Args a) {
     using T = typename Elem<DT>::T;
-    const int64_t total = a.rows * a.chunks;
-    const int64_t first = (int64_t)blockIdx.x * (kCThreads * U) + threadIdx.x;
-    float v[U][8];
+    __shared__ __align__(16) uint8_t stage[VEC || FLAT ? 16 : kCThreads * 8 * Elem<DT>::kBytes];
+    void* mine = stage + (VEC || FLAT ? 0 : (threadIdx.x >> 5) * Stage8<DT, false>::kBytes);
+    const Walk<FLAT, U> w(a.rows, a.chunks, a.tiles, a.by);
+    Row8<DT, VEC, 32> x[U];
+    uint32_t raw[U][RawRegs<DT>::N];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int64_t i = first + u * kCThreads;
-        const int64_t r = i / a.chunks;
-        if (i < total) load_row8<DT, VEC>((const T*)a.x + r * a.ld, (int)(i - r * a.chunks) * 8, a.cols, v[u]);
-        else {
+        if constexpr (VEC || !FLAT) {
+            x[u].load((const T*)a.x, a.ld, w.row[u], a.rows, w.col[u], a.cols);
+        } else {
+            float f[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[u][j] = 0.0f;
+            for (int j = 0; j < 8; j++)
+                f[j] = (w.chunk[u] >= 0 && w.col[u] + j < a.cols) ? Elem<DT>::to_float(((const T*)a.x)[w.row[u] * a.ld + w.col[u] + j]) : 0.0f;
+            const float2 p[4] = {make_float2(f[0], f[1]), make_float2(f[2], f[3]), make_float2(f[4], f[5]), make_float2(f[6], f[7])};
+            pairs_to_raw<DT>(p, raw[u]);
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int64_t i = first + u * kCThreads;
+        if constexpr (VEC || !FLAT) x[u].get(mine, raw[u]);
+        float2 v[4];
+        raw_to_pairs<DT>(raw[u], v);
         uint32_t byte;
-        const uint2 w = codes8<DT, STOCH>(v[u], a.rk, (uint64_t)i, byte);
-        if (i < total) {
-            st_stream_u2(a.codes + i * 8, w);
-            if ((threadIdx.x & 3) == 0) a.scales[i >> 2] = (uint8_t)byte;
+        const uint2 c = codes8<DT, STOCH>(v, absmax8<DT>(raw[u]), a.rk, (uint64_t)w.chunk[u], byte);
+        if (w.chunk[u] >= 0) {
+            st_stream_u2(a.codes + w.chunk[u] * 8, c);
+            if ((threadIdx.x & 3) == 0) a.scales[w.chunk[u] >> 2] = (uint8_t)byte;
         }
     }
 }
 
-struct Restore8Args {
-    const int8_t* codes; const uint8_t* scales;
-    int64_t rows; int cols; int chunks;
-    void* out; int64_t ld;
-};
-
-template <int DT, bool VEC, int U>
+template <int DT, bool VEC, bool FLAT, int U>
 __global__ void __launch_bounds__(kCThreads) restore8_kernel(const __grid_constant__ Restore8Args a) {
     using T = typename Elem<DT>::T;
-    const int64_t total = a.rows * a.chunks;
-    const int64_t first = (int64_t)blockIdx.x * (kCThreads * U) + threadIdx.x;
-    uint2 w[U];
+    __shared__ __align__(16) uint8_t stage[VEC || FLAT ? 16 : kCThreads * 8 * Elem<DT>::kBytes];
+    void* mine = stage + (VEC || FLAT ? 0 : (threadIdx.x >> 5) * Stage8<DT, false>::kBytes);
+    const Walk<FLAT, U> w(a.rows, a.chunks, a.tiles, a.by);
+    uint2 c[U];
     uint32_t b[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int64_t i = first + u * kCThreads;
-        w[u] = make_uint2(0u, 0u);
+        c[u] = make_uint2(0u, 0u);
         b[u] = 1;
-        if (i < total) {
-            w[u] = ld_stream_u2(a.codes + i * 8);
-            b[u] = a.scales[i >> 2];
+        if (w.chunk[u] >= 0) {
+            c[u] = ld_stream_u2(a.codes + w.chunk[u] * 8);
+            b[u] = a.scales[w.chunk[u] >> 2];
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int64_t i = first + u * kCThreads;
-        if (i >= total) continue;
-        const int64_t r = i / a.chunks;
-        float v[8];
-        restore8(w[u], scale_down8(b[u]), v);
-        store_row8<DT, VEC>((T*)a.out + r * a.ld, (int)(i - r * a.chunks) * 8, a.cols, v);
+        float2 v[4];
+        restore_pairs(c[u], scale_down8(b[u]), v);
+        if constexpr (VEC || !FLAT) {
+            Row8<DT, VEC, 32>::store((T*)a.out, a.ld, w.row[u], a.rows, w.col[u], a.cols, mine, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (w.chunk[u] >= 0 && w.col[u] + j < a.cols)
+                    ((T*)a.out)[w.row[u] * a.ld + w.col[u] + j] = Elem<DT>::from_float(j & 1 ? v[j / 2].y : v[j / 2].x);
+        }
     }
 }
 
@@ -88,37 +144,40 @@ __global__ void __launch_bounds__(kCThreads) repitch16_kernel(const uint16_t* __
     }
 }
 
-// Four chunks a thread once that still fills the GPU, else one (a small tensor is bound by latency).
-template <int DT, bool VEC, bool STOCH> static int launch_ckpt(const Ckpt8Args& a, cudaStream_t s) {
-    const int64_t total = a.rows * a.chunks;
-    if (total >= (int64_t)sm_count() * 2048 * 4) {
-        const int64_t blocks = (total + kCThreads * 4 - 1) / (kCThreads * 4);
-        checkpoint8_kernel<DT, VEC, STOCH, 4><<<(unsigned)blocks, kCThreads, 0, s>>>(a);
-    } else {
-        const int64_t blocks = (total + kCThreads - 1) / kCThreads;
-        checkpoint8_kernel<DT, VEC, STOCH, 1><<<(unsigned)blocks, kCThreads, 0, s>>>(a);
-    }
-    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+// Four chunks a thread once that still fills the GPU, else one (a small tensor is bound by latency).  Rows that do not
+// start on 16-byte boundaries are walked along the row once a warp's 256 columns are at least half full.
+template <bool FLAT> static int64_t walk_blocks(int64_t rows, int chunks, int tiles, int u) {
+    const int64_t per = (int64_t)(FLAT ? kCThreads : kCThreads / 32) * u;
+    return (rows * (FLAT ? chunks : tiles) + per - 1) / per;
 }
-template <int DT> static int dispatch_ckpt(const Ckpt8Args& a, bool stoch, cudaStream_t s) {
-    const bool vec = rows_aligned(a.x, a.ld, a.cols, Elem<DT>::kBytes);
-    if (vec) return stoch ? launch_ckpt<DT, true, true>(a, s) : launch_ckpt<DT, true, false>(a, s);
-    return stoch ? launch_ckpt<DT, false, true>(a, s) : launch_ckpt<DT, false, false>(a, s);
+static bool walk_big(int64_t rows, int chunks) { return rows * chunks >= (int64_t)sm_count() * 2048 * 4; }
+
+template <int DT, bool VEC, bool FLAT, bool STOCH> static void launch_ckpt(Ckpt8Args a, cudaStream_t s) {
+    a.by = Divisor::of(FLAT ? a.chunks : a.tiles);
+    if (walk_big(a.rows, a.chunks))
+        checkpoint8_kernel<DT, VEC, FLAT, STOCH, 4><<<(unsigned)walk_blocks<FLAT>(a.rows, a.chunks, a.tiles, 4), kCThreads, 0, s>>>(a);
+    else
+        checkpoint8_kernel<DT, VEC, FLAT, STOCH, 1><<<(unsigned)walk_blocks<FLAT>(a.rows, a.chunks, a.tiles, 1), kCThreads, 0, s>>>(a);
+}
+template <int DT, bool STOCH> static int dispatch_ckpt(const Ckpt8Args& a, cudaStream_t s) {
+    if (rows_aligned(a.x, a.ld, a.cols, Elem<DT>::kBytes)) launch_ckpt<DT, true, true, STOCH>(a, s);
+    else if (a.cols >= 128) launch_ckpt<DT, false, false, STOCH>(a, s);
+    else launch_ckpt<DT, false, true, STOCH>(a, s);
+    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 
-template <int DT, bool VEC> static int launch_restore(const Restore8Args& a, cudaStream_t s) {
-    const int64_t total = a.rows * a.chunks;
-    if (total >= (int64_t)sm_count() * 2048 * 4) {
-        const int64_t blocks = (total + kCThreads * 4 - 1) / (kCThreads * 4);
-        restore8_kernel<DT, VEC, 4><<<(unsigned)blocks, kCThreads, 0, s>>>(a);
-    } else {
-        const int64_t blocks = (total + kCThreads - 1) / kCThreads;
-        restore8_kernel<DT, VEC, 1><<<(unsigned)blocks, kCThreads, 0, s>>>(a);
-    }
-    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+template <int DT, bool VEC, bool FLAT> static void launch_restore(Restore8Args a, cudaStream_t s) {
+    a.by = Divisor::of(FLAT ? a.chunks : a.tiles);
+    if (walk_big(a.rows, a.chunks))
+        restore8_kernel<DT, VEC, FLAT, 4><<<(unsigned)walk_blocks<FLAT>(a.rows, a.chunks, a.tiles, 4), kCThreads, 0, s>>>(a);
+    else
+        restore8_kernel<DT, VEC, FLAT, 1><<<(unsigned)walk_blocks<FLAT>(a.rows, a.chunks, a.tiles, 1), kCThreads, 0, s>>>(a);
 }
 template <int DT> static int dispatch_restore(const Restore8Args& a, cudaStream_t s) {
-    return rows_aligned(a.out, a.ld, a.cols, Elem<DT>::kBytes) ? launch_restore<DT, true>(a, s) : launch_restore<DT, false>(a, s);
+    if (rows_aligned(a.out, a.ld, a.cols, Elem<DT>::kBytes)) launch_restore<DT, true, true>(a, s);
+    else if (a.cols >= 128) launch_restore<DT, false, false>(a, s);
+    else launch_restore<DT, false, true>(a, s);
+    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 
 }  // namespace gact
@@ -137,12 +196,13 @@ extern "C" int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t 
     Ckpt8Args a;
     a.x = x; a.ld = ld; a.rows = rows; a.cols = (int)cols;
     a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales; a.chunks = (int)(pitch8(cols) / 8);
+    a.tiles = (int)((cols + 255) / 256);
     a.rk = philox_round_keys(seed);
     cudaStream_t s = (cudaStream_t)stream;
     switch (dtype) {
-    case GACT_F32: return dispatch_ckpt<GACT_F32>(a, stochastic != 0, s);
-    case GACT_F16: return dispatch_ckpt<GACT_F16>(a, stochastic != 0, s);
-    default: return dispatch_ckpt<GACT_BF16>(a, stochastic != 0, s);
+    case GACT_F32: return stochastic ? dispatch_ckpt<GACT_F32, true>(a, s) : dispatch_ckpt<GACT_F32, false>(a, s);
+    case GACT_F16: return stochastic ? dispatch_ckpt<GACT_F16, true>(a, s) : dispatch_ckpt<GACT_F16, false>(a, s);
+    default: return stochastic ? dispatch_ckpt<GACT_BF16, true>(a, s) : dispatch_ckpt<GACT_BF16, false>(a, s);
     }
 }
 
@@ -155,7 +215,7 @@ extern "C" int gact_restore8(const void* codes, const void* scales, int64_t rows
     if (((uintptr_t)out & (uintptr_t)(elem_bytes_of(dtype) - 1)) || ((uintptr_t)codes & 31)) return GACT_ERR_ALIGN;
     Restore8Args a;
     a.codes = (const int8_t*)codes; a.scales = (const uint8_t*)scales; a.rows = rows; a.cols = (int)cols;
-    a.chunks = (int)(pitch8(cols) / 8); a.out = out; a.ld = ld;
+    a.chunks = (int)(pitch8(cols) / 8); a.tiles = (int)((cols + 255) / 256); a.out = out; a.ld = ld;
     cudaStream_t s = (cudaStream_t)stream;
     switch (dtype) {
     case GACT_F32: return dispatch_restore<GACT_F32>(a, s);

@@ -20,115 +20,141 @@ struct LnArgs {
     int8_t* codes; uint8_t* scales; int chunks; int stochastic; PhiloxKeys rk;
 };
 
-// 8 weights starting at column `col` (fp32 or the type of x), `fill` past the end or without a weight
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_param8(const void* p, int f32, int col, int cols, float fill, float (&v)[8]) {
-    if (p == nullptr) {
+// 8 weights starting at column `col` (fp32 or the type of x), 1 without a weight, 0 past the end
+template <int DT>
+__device__ __forceinline__ void load_param8(const void* p, int f32, int col, int cols, float (&v)[8]) {
+    using T = typename Elem<DT>::T;
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = fill;
-    } else if (f32 || DT == GACT_F32) {
-        if (VEC && col < cols) {
-            const float4 a = __ldg((const float4*)((const float*)p + col)), b = __ldg((const float4*)((const float*)p + col) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = (col + j < cols) ? __ldg((const float*)p + col + j) : 0.0f;
-        }
-    } else {
-        using T = typename Elem<DT>::T;
-        if (VEC && col < cols) {
-            const uint4 a = __ldg((const uint4*)((const T*)p + col));
-            const uint32_t raw[4] = {a.x, a.y, a.z, a.w};
-            if constexpr (DT != GACT_F32) raw_to_float<DT>(raw, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = (col + j < cols) ? Elem<DT>::to_float(((const T*)p)[col + j]) : 0.0f;
-        }
-    }
+    for (int j = 0; j < 8; j++)
+        v[j] = !p ? 1.0f : col + j >= cols ? 0.0f : f32 ? __ldg((const float*)p + col + j) : Elem<DT>::to_float(((const T*)p)[col + j]);
 }
 
 // Sum over the TPR threads of a row.  Up to 32 threads: shuffles inside an aligned part of a warp.  More: the block is one
-// row; `buf` holds one value per warp and is used by alternating halves, so one barrier per sum is enough.
+// row; `buf` holds one value per warp, and consecutive sums use different buffers, so one barrier per sum is enough.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
-        const int lane = threadIdx.x & 31;
-        if (lane == 0) buf[threadIdx.x >> 5] = v;
+        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = lane < W ? buf[lane] : 0.0f;
+        v = buf[0];
 #pragma unroll
-        for (int o = W / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-        v = __shfl_sync(kFull, v, 0);
+        for (int i = 1; i < W; i++) v += buf[i];
     }
     return v;
 }
 
-// A row is held by TPR threads, CH chunks of 8 elements each (chunk c of thread t: columns (t + c TPR) 8 ..).
+// A row is held by TPR threads, CH chunks of 8 elements each (chunk c of thread t: columns (t + c TPR) 8 ..).  Blocks are
+// resident and walk the rows; the next row's loads are issued before the current row is worked on, and weight and bias wait
+// in shared memory as fp32 (re-reading and widening them for every row cost as much as the norm itself).
 template <int DT, int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const __grid_constant__ LnArgs a) {
     using T = typename Elem<DT>::T;
-    __shared__ float buf[2][32];
-    const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / TPR) + threadIdx.x / TPR;
-    const bool live = row < a.rows;
-    const T* xr = (const T*)a.x + row * a.ldx;
-    float v[CH][8];
-    float sum = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CH; c++) load_row8<DT, VEC>(xr, (t + c * TPR) * 8, live ? a.cols : 0, v[c]);
-#pragma unroll
-    for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) sum += v[c][j];
-    const float mean = row_sum<TPR>(sum, buf[0]) * a.inv_cols;
-    float sq = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float d = v[c][j] - mean;
-            if (VEC ? (t + c * TPR) * 8 < a.cols : (t + c * TPR) * 8 + j < a.cols) sq = fmaf(d, d, sq);
-        }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, buf[1]) * a.inv_cols + a.eps);
-    if (live && t == 0 && a.mean) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+    constexpr int SUB = TPR < 32 ? TPR : 32, W = TPR * CH * 8;
+    using Row = Row8<DT, VEC, SUB>;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    float* pw = (float*)dyn;
+    float* pb = pw + W;
+    void* stage = dyn + 2 * W * sizeof(float) + (threadIdx.x >> 5) * Stage8<DT, VEC>::kBytes;
+    __shared__ float buf[2][2][TPR > 32 ? TPR / 32 : 1];
+    const int t = threadIdx.x % TPR, groups = blockDim.x / TPR, grp = threadIdx.x / TPR;
+    for (int c = threadIdx.x; c < W; c += blockDim.x) {
+        const bool in = c < a.cols;
+        pw[c] = !a.w ? 1.0f : !in ? 0.0f : (a.wf32 ? ((const float*)a.w)[c] : Elem<DT>::to_float(((const T*)a.w)[c]));
+        pb[c] = !a.b || !in ? 0.0f : (a.wf32 ? ((const float*)a.b)[c] : Elem<DT>::to_float(((const T*)a.b)[c]));
     }
+    __syncthreads();
+    const int64_t step = (int64_t)gridDim.x * groups;
+    int64_t base = (int64_t)blockIdx.x * groups;
+    Row x[CH];
 #pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int col = (t + c * TPR) * 8;
-        if (a.codes) {
-            uint32_t byte;
-            const uint64_t chunk = (uint64_t)row * a.chunks + (t + c * TPR);
-            const uint2 w = a.stochastic ? codes8<DT, true>(v[c], a.rk, chunk, byte) : codes8<DT, false>(v[c], a.rk, chunk, byte);
-            if (live && t + c * TPR < a.chunks) {
-                st_stream_u2(a.codes + chunk * 8, w);
-                if ((t & 3) == 0) a.scales[chunk >> 2] = (uint8_t)byte;
+    for (int c = 0; c < CH; c++) x[c].load((const T*)a.x, a.ldx, base + grp, a.rows, (t + c * TPR) * 8, a.cols);
+    for (int phase = 0; base < a.rows; base += step, phase ^= 1) {
+        const int64_t row = base + grp;
+        uint32_t raw[CH][RawRegs<DT>::N];
+#pragma unroll
+        for (int c = 0; c < CH; c++) x[c].get(stage, raw[c]);
+#pragma unroll
+        for (int c = 0; c < CH; c++) x[c].load((const T*)a.x, a.ldx, row + step, a.rows, (t + c * TPR) * 8, a.cols);
+        float2 s2 = splat2(0.0f);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            float2 v[4];
+            raw_to_pairs<DT>(raw[c], v);
+            s2 = add2(s2, add2(add2(v[0], v[1]), add2(v[2], v[3])));
+        }
+        const float mean = row_sum<TPR>(s2.x + s2.y, buf[phase][0]) * a.inv_cols;
+        float2 q2 = splat2(0.0f);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            float2 v[4];
+            raw_to_pairs<DT>(raw[c], v);
+            const int col = (t + c * TPR) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float2 d = add2(v[i], splat2(-mean));
+                if (VEC) { if (col >= a.cols) d = splat2(0.0f); }
+                else {
+                    if (col + 2 * i >= a.cols) d.x = 0.0f;
+                    if (col + 2 * i + 1 >= a.cols) d.y = 0.0f;
+                }
+                q2 = fma2(d, d, q2);
             }
         }
-        float w[8], b[8], o[8];
-        load_param8<DT, VEC>(a.w, a.wf32, col, a.cols, 1.0f, w);
-        load_param8<DT, VEC>(a.b, a.wf32, col, a.cols, 0.0f, b);
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q2.x + q2.y, buf[phase][1]) * a.inv_cols + a.eps);
+        const bool live = row < a.rows;
+        if (live && t == 0 && a.mean) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = fmaf((v[c][j] - mean) * rstd, w[j], b[j]);
-        store_row8<DT, VEC>((T*)a.y + row * a.cols, col, live ? a.cols : 0, o);
+        for (int c = 0; c < CH; c++) {
+            const int col = (t + c * TPR) * 8;
+            float2 v[4], o[4];
+            raw_to_pairs<DT>(raw[c], v);
+            if (a.codes) {
+                uint32_t byte;
+                const uint64_t chunk = (uint64_t)row * a.chunks + (t + c * TPR);
+                const uint32_t m = absmax8<DT>(raw[c]);
+                const uint2 q = a.stochastic ? codes8<DT, true>(v, m, a.rk, chunk, byte) : codes8<DT, false>(v, m, a.rk, chunk, byte);
+                if (live && t + c * TPR < a.chunks) {
+                    st_stream_u2(a.codes + chunk * 8, q);
+                    if ((t & 3) == 0) a.scales[chunk >> 2] = (uint8_t)byte;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float4 w = *(const float4*)(pw + col + 2 * i), b = *(const float4*)(pb + col + 2 * i);
+                o[i] = fma2(mul2(add2(v[i], splat2(-mean)), splat2(rstd)), make_float2(w.x, w.y), make_float2(b.x, b.y));
+                o[i + 1] = fma2(mul2(add2(v[i + 1], splat2(-mean)), splat2(rstd)), make_float2(w.z, w.w), make_float2(b.z, b.w));
+            }
+            Row::store((T*)a.y, a.cols, row, a.rows, col, a.cols, stage, o);
+        }
     }
 }
 
-template <int DT, int TPR, int CH> static int launch_ln(const LnArgs& a, bool vec, cudaStream_t s) {
-    // several rows per block while a row is at most a warp, fewer when there are few rows
-    int block = TPR > 128 ? TPR : 128;
-    if (TPR <= 32)
+template <int DT, int TPR, int CH, bool VEC> static int launch_ln_vec(const LnArgs& a, cudaStream_t s) {
+    auto* k = layer_norm_kernel<DT, TPR, CH, VEC>;
+    // rows of up to a warp share a block, fewer of them when there are few rows
+    int block = TPR;
+    if (TPR <= 32) {
+        block = 128;
         while (block > 32 && a.rows * TPR < (int64_t)sm_count() * block) block /= 2;
-    else block = TPR;
-    const int64_t per = block / TPR;
-    const int64_t blocks = (a.rows + per - 1) / per;
-    if (vec) layer_norm_kernel<DT, TPR, CH, true><<<(unsigned)blocks, block, 0, s>>>(a);
-    else layer_norm_kernel<DT, TPR, CH, false><<<(unsigned)blocks, block, 0, s>>>(a);
+    }
+    const int smem = 2 * TPR * CH * 8 * (int)sizeof(float) + block / 32 * Stage8<DT, VEC>::kBytes;
+    constexpr int kMost = 2 * TPR * CH * 8 * (int)sizeof(float) + (TPR > 128 ? TPR : 128) / 32 * Stage8<DT, VEC>::kBytes;
+    if (kMost > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return GACT_ERR_LAUNCH;
+    static std::atomic<int> cache[kMaxDevices];
+    const int64_t want = (a.rows + block / TPR - 1) / (block / TPR);
+    // (the count is that of full blocks; smaller blocks only run when there are too few rows for it to matter)
+    const int64_t most = (int64_t)sm_count() * resident_blocks(k, TPR > 128 ? TPR : TPR > 32 ? TPR : 128, kMost, cache);
+    k<<<(unsigned)(want < most ? want : most), block, smem, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+template <int DT, int TPR, int CH> static int launch_ln(const LnArgs& a, bool vec, cudaStream_t s) {
+    return vec ? launch_ln_vec<DT, TPR, CH, true>(a, s) : launch_ln_vec<DT, TPR, CH, false>(a, s);
 }
 template <int DT> static int dispatch_ln(const LnArgs& a, bool vec, cudaStream_t s) {
     const int h = a.cols;
@@ -141,8 +167,10 @@ template <int DT> static int dispatch_ln(const LnArgs& a, bool vec, cudaStream_t
     if (h <= 2048) return launch_ln<DT, 128, 2>(a, vec, s);
     if (h <= 4096) return launch_ln<DT, 256, 2>(a, vec, s);
     if (h <= 8192) return launch_ln<DT, 512, 2>(a, vec, s);
-    return launch_ln<DT, 1024, 2>(a, vec, s);
+    return launch_ln<DT, 512, 4>(a, vec, s);
 }
+
+constexpr int kLnBwdRows = 2;                       // rows a block (or row group) works on side by side
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 struct LnBwdArgs {
@@ -158,84 +186,118 @@ struct LnBwdArgs {
 };
 
 // A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
-// walks rows blockIdx, blockIdx + grid, ..., R of them (per row group) side by side so that R rows' loads are in flight
-// and one barrier serves 2 R sums.  Block sums go to `partial`, added up in a fixed order afterwards: no atomics.
+// walks the rows, R of them (per row group) side by side: one barrier serves 2 R sums, and the next R rows' loads are issued
+// before the current ones are worked on.  Block sums go to `partial`, added up in a fixed order afterwards: no atomics.
 template <int DT, int TPR, int CH, int R, bool VEC, bool COMP>
-__global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_backward_kernel(const __grid_constant__ LnBwdArgs a) {
+__global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR : 128)) layer_norm_backward_kernel(const __grid_constant__ LnBwdArgs a) {
     using T = typename Elem<DT>::T;
-    constexpr int BLOCK = TPR > 128 ? TPR : (TPR > 32 ? TPR : 128);
-    constexpr int GROUPS = BLOCK / TPR;
-    __shared__ float2 buf[2][R][32];
+    constexpr int BLOCK = TPR > 32 ? TPR : 128, GROUPS = BLOCK / TPR, SUB = TPR < 32 ? TPR : 32;
+    using Row = Row8<DT, VEC, SUB>;
+    __shared__ float2 buf[2][R][TPR > 32 ? TPR / 32 : 1];
+    __shared__ __align__(16) uint8_t staging[VEC ? 16 : BLOCK / 32 * Stage8<DT, VEC>::kBytes];
     __shared__ float fold[GROUPS > 1 ? BLOCK * 16 : 1];
-    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    float w[CH][8], dw[CH][8], db[CH][8];
+    void* stage = staging + (threadIdx.x >> 5) * Stage8<DT, VEC>::kBytes;
+    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, lane = threadIdx.x & 31;
+    float2 w[CH][4], dw[CH][4], db[CH][4];
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-        load_param8<DT, VEC>(a.w, a.wf32, (t + c * TPR) * 8, a.cols, 1.0f, w[c]);
+        float f[8];
+        load_param8<DT>(a.w, a.wf32, (t + c * TPR) * 8, a.cols, f);
 #pragma unroll
-        for (int j = 0; j < 8; j++) dw[c][j] = db[c][j] = 0.0f;
+        for (int i = 0; i < 4; i++) {
+            w[c][i] = make_float2(f[2 * i], f[2 * i + 1]);
+            dw[c][i] = db[c][i] = splat2(0.0f);
+        }
     }
-    int phase = 0;
+    Row py[R][CH], px[COMP ? 1 : R][COMP ? 1 : CH];
+    uint2 pq[R][CH];
+    uint32_t pe[R][CH];
+    float pm[R], pr[R];
+    auto fetch = [&](int64_t base) {
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const int64_t row = base + k * GROUPS + grp;
+            const bool live = row < a.rows;
+            pm[k] = live ? __ldg(a.mean + row) : 0.0f;
+            pr[k] = live ? __ldg(a.rstd + row) : 0.0f;
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                py[k][c].load((const T*)a.dy, a.ldy, row, a.rows, (t + c * TPR) * 8, a.cols);
+                if constexpr (COMP) {
+                    pq[k][c] = make_uint2(0u, 0u);
+                    pe[k][c] = 1;
+                    if (live && t + c * TPR < a.chunks) {
+                        const int64_t chunk = row * a.chunks + (t + c * TPR);
+                        pq[k][c] = ld_stream_u2(a.codes + chunk * 8);
+                        pe[k][c] = a.scales[chunk >> 2];
+                    }
+                } else {
+                    px[k][c].load((const T*)a.x, a.ldx, row, a.rows, (t + c * TPR) * 8, a.cols);
+                }
+            }
+        }
+    };
     const int64_t step = (int64_t)gridDim.x * GROUPS * R;
-    for (int64_t r0 = ((int64_t)blockIdx.x * GROUPS) * R; r0 < a.rows; r0 += step, phase ^= 1) {
-        float g[R][CH][8], xh[R][CH][8];
+    int64_t r0 = (int64_t)blockIdx.x * GROUPS * R;
+    fetch(r0);
+    for (int phase = 0; r0 < a.rows; r0 += step, phase ^= 1) {
+        float2 g[R][CH][4], xh[R][CH][4];
         float2 s[R];
         float rs[R];
 #pragma unroll
         for (int k = 0; k < R; k++) {
-            const int64_t row = r0 + k * GROUPS + grp;
-            const bool live = row < a.rows;
-            const float mean = live ? a.mean[row] : 0.0f;
-            rs[k] = live ? a.rstd[row] : 0.0f;
+            rs[k] = pr[k];
+            const float2 off = splat2(-pm[k] * pr[k]);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                uint32_t raw[RawRegs<DT>::N];
+                py[k][c].get(stage, raw);
+                raw_to_pairs<DT>(raw, g[k][c]);
+                // x^ = x' r - mean r; a code is a small integer and its scale a power of two, so x' r is one product
+                float2 up;
+                if constexpr (COMP) {
+                    code_pairs(pq[k][c], xh[k][c]);
+                    up = splat2(scale_down8(pe[k][c]) * rs[k]);
+                } else {
+                    px[k][c].get(stage, raw);
+                    raw_to_pairs<DT>(raw, xh[k][c]);
+                    up = splat2(rs[k]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) xh[k][c][i] = fma2(xh[k][c][i], up, off);
+            }
+        }
+        fetch(r0 + step);
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            float2 s1 = splat2(0.0f), s2 = splat2(0.0f);
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 const int col = (t + c * TPR) * 8;
-                load_row8<DT, VEC>((const T*)a.dy + row * a.ldy, col, live ? a.cols : 0, g[k][c]);
-                if constexpr (COMP) {
-                    uint2 q = make_uint2(0u, 0u);
-                    uint32_t byte = 1;
-                    if (live && t + c * TPR < a.chunks) {
-                        const int64_t chunk = row * a.chunks + (t + c * TPR);
-                        q = ld_stream_u2(a.codes + chunk * 8);
-                        byte = a.scales[chunk >> 2];
-                    }
-                    restore8(q, scale_down8(byte), xh[k][c]);
-                } else {
-                    load_row8<DT, VEC>((const T*)a.x + row * a.ldx, col, live ? a.cols : 0, xh[k][c]);
-                }
 #pragma unroll
-                for (int j = 0; j < 8; j++) xh[k][c][j] = (xh[k][c][j] - mean) * rs[k];
+                for (int i = 0; i < 4; i++) {
+                    // a column past the end has dy = 0, but a NaN scale of the row's last block must not leak out of it
+                    if (VEC) { if (col >= a.cols) xh[k][c][i] = splat2(0.0f); }
+                    else {
+                        if (col + 2 * i >= a.cols) xh[k][c][i].x = 0.0f;
+                        if (col + 2 * i + 1 >= a.cols) xh[k][c][i].y = 0.0f;
+                    }
+                    dw[c][i] = fma2(g[k][c][i], xh[k][c][i], dw[c][i]);
+                    db[c][i] = add2(db[c][i], g[k][c][i]);
+                    g[k][c][i] = mul2(g[k][c][i], w[c][i]);
+                    s1 = add2(s1, g[k][c][i]);
+                    s2 = fma2(g[k][c][i], xh[k][c][i], s2);
+                }
             }
-        }
+            s[k] = make_float2(s1.x + s1.y, s2.x + s2.y);
 #pragma unroll
-        for (int k = 0; k < R; k++) {
-            s[k] = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < CH; c++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    // a column past the end has g = 0 (its dy reads as 0) but a NaN scale or an infinite mean must not leak
-                    // out of it: only real columns take part
-                    if (VEC ? (t + c * TPR) * 8 < a.cols : (t + c * TPR) * 8 + j < a.cols) {
-                        dw[c][j] = fmaf(g[k][c][j], xh[k][c][j], dw[c][j]);
-                        db[c][j] += g[k][c][j];
-                        g[k][c][j] *= w[c][j];
-                        s[k].x += g[k][c][j];
-                        s[k].y = fmaf(g[k][c][j], xh[k][c][j], s[k].y);
-                    }
-                }
-        }
-#pragma unroll
-        for (int k = 0; k < R; k++) {
-#pragma unroll
-            for (int o = (TPR < 32 ? TPR : 32) / 2; o >= 1; o >>= 1) {
+            for (int o = SUB / 2; o >= 1; o >>= 1) {
                 s[k].x += __shfl_xor_sync(kFull, s[k].x, o);
                 s[k].y += __shfl_xor_sync(kFull, s[k].y, o);
             }
         }
         if constexpr (TPR > 32) {
             constexpr int W = TPR / 32;
-            const int lane = threadIdx.x & 31;
             if (lane == 0) {
 #pragma unroll
                 for (int k = 0; k < R; k++) buf[phase][k][threadIdx.x >> 5] = s[k];
@@ -243,27 +305,24 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_backward_ker
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < R; k++) {
-                s[k] = lane < W ? buf[phase][k][lane] : make_float2(0.0f, 0.0f);
+                // every lane adds the warps' sums itself (a broadcast read each), in warp order
+                s[k] = buf[phase][k][0];
 #pragma unroll
-                for (int o = W / 2; o >= 1; o >>= 1) {
-                    s[k].x += __shfl_xor_sync(kFull, s[k].x, o);
-                    s[k].y += __shfl_xor_sync(kFull, s[k].y, o);
-                }
-                s[k].x = __shfl_sync(kFull, s[k].x, 0);
-                s[k].y = __shfl_sync(kFull, s[k].y, 0);
+                for (int i = 1; i < W; i++) s[k] = add2(s[k], buf[phase][k][i]);
             }
         }
         if (a.dx) {
 #pragma unroll
             for (int k = 0; k < R; k++) {
                 const int64_t row = r0 + k * GROUPS + grp;
-                const float c1 = s[k].x * a.inv_cols, c2 = s[k].y * a.inv_cols;
+                // r (g - c1 - x^ c2)
+                const float2 c1 = splat2(-s[k].x * a.inv_cols), c2 = splat2(-s[k].y * a.inv_cols);
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
-                    float o[8];
+                    float2 o[4];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = rs[k] * (g[k][c][j] - c1 - xh[k][c][j] * c2);
-                    store_row8<DT, VEC>((T*)a.dx + row * a.cols, (t + c * TPR) * 8, row < a.rows ? a.cols : 0, o);
+                    for (int i = 0; i < 4; i++) o[i] = mul2(fma2(xh[k][c][i], c2, add2(g[k][c][i], c1)), splat2(rs[k]));
+                    Row::store((T*)a.dx, a.cols, row, a.rows, (t + c * TPR) * 8, a.cols, stage, o);
                 }
             }
         }
@@ -272,17 +331,20 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_backward_ker
     if constexpr (GROUPS > 1) {
         // fold the row groups of the block: fold[j][thread]
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            fold[j * BLOCK + threadIdx.x] = dw[0][j];
-            fold[(8 + j) * BLOCK + threadIdx.x] = db[0][j];
+        for (int i = 0; i < 4; i++) {
+            fold[(4 * i) * BLOCK + threadIdx.x] = dw[0][i].x;
+            fold[(4 * i + 1) * BLOCK + threadIdx.x] = dw[0][i].y;
+            fold[(4 * i + 2) * BLOCK + threadIdx.x] = db[0][i].x;
+            fold[(4 * i + 3) * BLOCK + threadIdx.x] = db[0][i].y;
         }
         __syncthreads();
         if (grp == 0) {
             for (int k = 1; k < GROUPS; k++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    dw[0][j] += fold[j * BLOCK + k * TPR + t];
-                    db[0][j] += fold[(8 + j) * BLOCK + k * TPR + t];
+                for (int i = 0; i < 4; i++) {
+                    const float* f = fold + k * TPR + t;
+                    dw[0][i] = add2(dw[0][i], make_float2(f[(4 * i) * BLOCK], f[(4 * i + 1) * BLOCK]));
+                    db[0][i] = add2(db[0][i], make_float2(f[(4 * i + 2) * BLOCK], f[(4 * i + 3) * BLOCK]));
                 }
         }
     }
@@ -292,23 +354,27 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_backward_ker
         for (int c = 0; c < CH; c++) {
             const int col = (t + c * TPR) * 8;
             if (col >= a.width) continue;
-            *(float4*)(p + col) = make_float4(dw[c][0], dw[c][1], dw[c][2], dw[c][3]);
-            *(float4*)(p + col + 4) = make_float4(dw[c][4], dw[c][5], dw[c][6], dw[c][7]);
-            *(float4*)(p + a.width + col) = make_float4(db[c][0], db[c][1], db[c][2], db[c][3]);
-            *(float4*)(p + a.width + col + 4) = make_float4(db[c][4], db[c][5], db[c][6], db[c][7]);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                *(float4*)(p + col + 2 * i) = make_float4(dw[c][i].x, dw[c][i].y, dw[c][i + 1].x, dw[c][i + 1].y);
+                *(float4*)(p + a.width + col + 2 * i) = make_float4(db[c][i].x, db[c][i].y, db[c][i + 1].x, db[c][i + 1].y);
+            }
         }
     }
 }
 
-// Blocks of the backward pass: about 2 x 512 threads per SM keep enough rows in flight, more only lengthens the sum of
-// the partials (each block writes 2 x cols floats).
+// Threads per row, chunks per thread and rows per step of the backward pass, by the row length.
+struct LnBwdShape { int tpr, block, r; };
+static LnBwdShape ln_bwd_shape(int64_t cols) {
+    const int tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
+    return {tpr, tpr > 32 ? tpr : 128, cols <= 4096 ? kLnBwdRows : 1};
+}
+// Resident blocks: 512 threads per SM (more only lengthens the sum of the partials, 2 x cols floats per block).
 static int64_t ln_bwd_blocks(int64_t rows, int64_t cols) {
-    const int tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256
-                  : 512;
-    const int block = tpr > 32 ? tpr : 128;
-    const int64_t groups = block / tpr;
-    const int64_t most = (int64_t)sm_count() * (1024 / block);
-    const int64_t want = (rows + groups - 1) / groups;
+    const LnBwdShape p = ln_bwd_shape(cols);
+    const int64_t per = (int64_t)(p.block / p.tpr) * p.r;
+    const int64_t most = (int64_t)sm_count() * (512 / p.block);
+    const int64_t want = (rows + per - 1) / per;
     return want < most ? want : most;
 }
 
@@ -325,14 +391,14 @@ template <int DT, int TPR, int CH, int R> static int launch_ln_bwd(const LnBwdAr
 }
 template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, int64_t blocks, cudaStream_t s) {
     const int h = a.cols;
-    if (h <= 32) return launch_ln_bwd<DT, 4, 1, 2>(a, vec, blocks, s);
-    if (h <= 64) return launch_ln_bwd<DT, 8, 1, 2>(a, vec, blocks, s);
-    if (h <= 128) return launch_ln_bwd<DT, 16, 1, 2>(a, vec, blocks, s);
-    if (h <= 256) return launch_ln_bwd<DT, 32, 1, 2>(a, vec, blocks, s);
-    if (h <= 512) return launch_ln_bwd<DT, 64, 1, 2>(a, vec, blocks, s);
-    if (h <= 1024) return launch_ln_bwd<DT, 128, 1, 2>(a, vec, blocks, s);
-    if (h <= 2048) return launch_ln_bwd<DT, 256, 1, 2>(a, vec, blocks, s);
-    if (h <= 4096) return launch_ln_bwd<DT, 512, 1, 2>(a, vec, blocks, s);
+    if (h <= 32) return launch_ln_bwd<DT, 4, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 64) return launch_ln_bwd<DT, 8, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 128) return launch_ln_bwd<DT, 16, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 256) return launch_ln_bwd<DT, 32, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 512) return launch_ln_bwd<DT, 64, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 1024) return launch_ln_bwd<DT, 128, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 2048) return launch_ln_bwd<DT, 256, 1, kLnBwdRows>(a, vec, blocks, s);
+    if (h <= 4096) return launch_ln_bwd<DT, 512, 1, kLnBwdRows>(a, vec, blocks, s);
     if (h <= 8192) return launch_ln_bwd<DT, 512, 2, 1>(a, vec, blocks, s);
     return launch_ln_bwd<DT, 512, 4, 1>(a, vec, blocks, s);
 }

@@ -26,7 +26,7 @@ struct GemmArgs {
     int tiles_m, tiles_n, splits, per_split;  // stages per split
     // epilogue
     void* out; int64_t ldo; int ovec;         // bytes per store: 32, 16 or 2
-    const void* bias; int bvec;
+    const void* bias;
     const void* res; int64_t ldr; int rvec;
     int act;
     void* z; int zvec;                        // pre-activation in the operand type (row pitch N), or
@@ -41,62 +41,81 @@ __device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
                  "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
-// ---- activations ----------------------------------------------------------------------------------------------------
+// ---- activations, two values at a time -------------------------------------------------------------------------------
+__device__ __forceinline__ float fast_rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(fast_rcp(x.x), fast_rcp(x.y)); }
+__device__ __forceinline__ float2 exp2_2(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+constexpr float kLog2e = 1.4426950408889634f;
+
 // Phi(z) = (1 + erf(z / sqrt 2)) / 2 through Abramowitz & Stegun 7.1.26 (|error| of erf <= 1.5e-7): with
 // t = 1 / (1 + 0.3275911 |z| / sqrt 2), erfc(|z| / sqrt 2) = t (a1 + t (a2 + ...)) exp(-z^2 / 2).  One exponential serves
-// Phi and the density.  The tail keeps its relative precision (no cancellation against 1 for negative z).
-__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& gauss) {
-    const float az = fabsf(z);
-    gauss = __expf(-0.5f * z * z);
-    const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678118654752f, az, 1.0f));
-    float p = fmaf(t, 1.061405429f, -1.453152027f);
-    p = fmaf(t, p, 1.421413741f);
-    p = fmaf(t, p, -0.284496736f);
-    p = fmaf(t, p, 0.254829592f);
-    const float half_tail = 0.5f * p * t * gauss;
-    cdf = z < 0.0f ? half_tail : 1.0f - half_tail;
+// Phi and the density.  The tail keeps its relative precision (no cancellation against 1 for negative z).  The
+// coefficients are halved here, so that the polynomial gives the tail of Phi directly.
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2& gauss) {
+    const float2 az = make_float2(fabsf(z.x), fabsf(z.y));
+    gauss = exp2_2(mul2(mul2(z, splat2(-0.5f * kLog2e)), z));
+    const float2 t = rcp2(fma2(az, splat2(0.3275911f * 0.70710678118654752f), splat2(1.0f)));
+    float2 p = fma2(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
+    p = fma2(t, p, splat2(0.5f * 1.421413741f));
+    p = fma2(t, p, splat2(0.5f * -0.284496736f));
+    p = fma2(t, p, splat2(0.5f * 0.254829592f));
+    const float2 tail = mul2(mul2(p, t), gauss), rest = fma2(tail, splat2(-1.0f), splat2(1.0f));
+    return make_float2(z.x < 0.0f ? tail.x : rest.x, z.y < 0.0f ? tail.y : rest.y);
 }
-__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+// 1 / (1 + exp(-u)); an exponential that overflows gives 0
+__device__ __forceinline__ float2 sigmoid2(float2 u) { return rcp2(add2(exp2_2(mul2(u, splat2(-kLog2e))), splat2(1.0f))); }
 constexpr float kTanhA = 1.5957691216057308f;       // 2 sqrt(2 / pi): (1 + tanh u) / 2 = sigmoid(2 u)
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    if (act == GACT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (act == GACT_ACT_GELU) {
-        float c, g;
-        normal_cdf(z, c, g);
-        return z * c;
+template <int ACT> __device__ __forceinline__ float2 act_value2(float2 z) {
+    if constexpr (ACT == GACT_ACT_RELU) {
+        return make_float2(z.x > 0.0f ? z.x : (z.x != z.x ? z.x : 0.0f), z.y > 0.0f ? z.y : (z.y != z.y ? z.y : 0.0f));
+    } else if constexpr (ACT == GACT_ACT_GELU) {
+        float2 g;
+        return mul2(z, normal_cdf2(z, g));
+    } else if constexpr (ACT == GACT_ACT_GELU_TANH) {
+        return mul2(z, sigmoid2(mul2(mul2(z, splat2(kTanhA)), fma2(mul2(z, z), splat2(0.044715f), splat2(1.0f)))));
+    } else if constexpr (ACT == GACT_ACT_SILU) {
+        return mul2(z, sigmoid2(z));
     }
-    if (act == GACT_ACT_GELU_TANH) return z * sigmoid(kTanhA * fmaf(0.044715f * z * z, z, z));
-    if (act == GACT_ACT_SILU) return z * sigmoid(z);
     return z;
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == GACT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act == GACT_ACT_GELU) {
-        float c, g;
-        normal_cdf(z, c, g);
-        return fmaf(z * 0.39894228040143268f, g, c);
+template <int ACT> __device__ __forceinline__ float2 act_slope2(float2 z) {
+    if constexpr (ACT == GACT_ACT_RELU) {
+        return make_float2(z.x > 0.0f ? 1.0f : (z.x != z.x ? z.x : 0.0f), z.y > 0.0f ? 1.0f : (z.y != z.y ? z.y : 0.0f));
+    } else if constexpr (ACT == GACT_ACT_GELU) {
+        float2 g;
+        const float2 c = normal_cdf2(z, g);
+        return fma2(mul2(z, splat2(0.39894228040143268f)), g, c);
+    } else if constexpr (ACT == GACT_ACT_GELU_TANH) {
+        const float2 q = mul2(z, z);
+        const float2 p = sigmoid2(mul2(mul2(z, splat2(kTanhA)), fma2(q, splat2(0.044715f), splat2(1.0f))));
+        const float2 r = mul2(mul2(z, p), fma2(p, splat2(-1.0f), splat2(1.0f)));
+        return fma2(r, fma2(q, splat2(3.0f * 0.044715f * kTanhA), splat2(kTanhA)), p);
+    } else if constexpr (ACT == GACT_ACT_SILU) {
+        const float2 p = sigmoid2(z);
+        return fma2(mul2(z, p), fma2(p, splat2(-1.0f), splat2(1.0f)), p);
     }
-    if (act == GACT_ACT_GELU_TANH) {
-        const float p = sigmoid(kTanhA * fmaf(0.044715f * z * z, z, z));
-        return fmaf(z * p * (1.0f - p), kTanhA * fmaf(3.0f * 0.044715f, z * z, 1.0f), p);
-    }
-    if (act == GACT_ACT_SILU) {
-        const float p = sigmoid(z);
-        return fmaf(z * p, 1.0f - p, p);
-    }
-    return 1.0f;
+    return splat2(1.0f);
 }
 
 // ---- epilogue of 32 consecutive columns of one row -------------------------------------------------------------------
 template <int DT>
-__device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, const float (&v)[32]) {
+__device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, const float2 (&v)[16]) {
     using T = typename Elem<DT>::T;
     T* p = (T*)base + row * ld + n;
-    if (n + 32 <= N && vec >= 16) {
-        uint32_t w[16];
+    uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < 16; i++) w[i] = pack2<DT>(v[i].x, v[i].y);
+    if (n + 32 <= N && vec >= 16) {
         if (vec == 32) {
             const uint32_t a[8] = {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, b[8] = {w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]};
             st_v8(p, a);
@@ -108,11 +127,11 @@ __device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t
     } else {
 #pragma unroll
         for (int j = 0; j < 32; j++)
-            if (n + j < N) p[j] = Elem<DT>::from_float(v[j]);
+            if (n + j < N) ((uint16_t*)p)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
     }
 }
 template <int DT>
-__device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, float (&v)[32]) {
+__device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, float2 (&v)[16]) {
     using T = typename Elem<DT>::T;
     const T* p = (const T*)base + row * ld + n;
     if (n + 32 <= N && vec >= 16) {
@@ -120,46 +139,64 @@ __device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int
         for (int i = 0; i < 4; i++) {
             const uint4 u = __ldg((const uint4*)(p + 8 * i));
             const uint32_t raw[4] = {u.x, u.y, u.z, u.w};
-            float f[8];
-            raw_to_float<DT>(raw, f);
+            float2 f[4];
+            raw_to_pairs<DT>(raw, f);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[8 * i + j] += f[j];
+            for (int j = 0; j < 4; j++) v[4 * i + j] = add2(v[4 * i + j], f[j]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (n + j < N) v[j] += Elem<DT>::to_float(p[j]);
+        for (int i = 0; i < 16; i++) {
+            if (n + 2 * i < N) v[i].x += Elem<DT>::to_float(p[2 * i]);
+            if (n + 2 * i + 1 < N) v[i].y += Elem<DT>::to_float(p[2 * i + 1]);
+        }
     }
 }
-
-// z = v + bias -> checkpoint of z, y = act(z) + residual -> out.  Called by threads that own (row, n .. n+31).
-template <int DT>
-__device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row, int64_t n, float (&v)[32]) {
-    if (a.bias) add32<DT>(a.bias, 0, a.bvec, 0, n, a.N, v);
-    if (a.zcodes) {
-        uint32_t m = 0;
+template <int ACT> __device__ __forceinline__ void activate32(float2 (&v)[16]) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            if (n + j >= a.N) v[j] = 0.0f;
-            m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-        }
-        const uint32_t byte = scale_byte8(m);
+    for (int i = 0; i < 16; i++) v[i] = act_value2<ACT>(v[i]);
+}
+
+// z = v + bias -> checkpoint of z, y = act(z) + residual -> out.  Called by threads that own (row, n .. n+31);
+// `bias`: the 32 biases as fp32 in shared memory (zeros past N or without one).
+template <int DT>
+__device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row, int64_t n, const float* bias, float2 (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const float4 b = *(const float4*)(bias + 2 * i);
+        v[i] = add2(v[i], make_float2(b.x, b.y));
+        v[i + 1] = add2(v[i + 1], make_float2(b.z, b.w));
+    }
+    if (a.zcodes) {
+        // columns past N are zero: their weights and biases are
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i].x), "f"(v[i].y));
+        const uint32_t byte = scale_byte8(__float_as_uint(m) & 0x7fffffffu);
         const float up = scale_up8(byte);
         const uint64_t at = (uint64_t)row * a.zpitch + n;
         uint32_t w[8];
+        if (!a.stochastic && a.act != GACT_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            uint32_t c[4];
-            uint4 r;
-            if (a.stochastic) r = noise8(a.rk, at / 8 + i / 2);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float z = v[4 * i + j];
-                c[j] = a.stochastic ? code8_noise(z, up, noise8_at(r, (i & 1) * 4 + j)) : code8(z, up);
-                // ReLU's slope is decided by the sign of z: a positive z keeps a positive code
-                if (a.act == GACT_ACT_RELU && z > 0.0f && (c[j] & 0xffu) == 0u) c[j] = 1u;
+            for (int i = 0; i < 8; i++) {
+                const float2 p = fma2(v[2 * i], splat2(up), splat2(12582912.0f)), q = fma2(v[2 * i + 1], splat2(up), splat2(12582912.0f));
+                w[i] = pack4(__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y));
             }
-            w[i] = pack4(c[0], c[1], c[2], c[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                uint32_t c[4];
+                uint4 r = make_uint4(0u, 0u, 0u, 0u);
+                if (a.stochastic) r = noise8(a.rk, at / 8 + i / 2);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float z = (j & 1) ? v[2 * i + j / 2].y : v[2 * i + j / 2].x;
+                    c[j] = a.stochastic ? code8_noise(z, up, noise8_at(r, (i & 1) * 4 + j)) : code8(z, up);
+                    // ReLU's slope is decided by the sign of z: a positive z keeps a positive code
+                    if (a.act == GACT_ACT_RELU && z > 0.0f && (c[j] & 0xffu) == 0u) c[j] = 1u;
+                }
+                w[i] = pack4(c[0], c[1], c[2], c[3]);
+            }
         }
         if (byte >= top_byte8<GACT_F32>()) {
 #pragma unroll
@@ -169,12 +206,18 @@ __device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row
         a.zscales[at >> 5] = (uint8_t)byte;
     }
     if (a.z) store32<DT>(a.z, a.N, a.zvec, row, n, a.N, v);
-    if (a.act != GACT_ACT_NONE) {
-#pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = act_value(v[j], a.act);
+    switch (a.act) {
+    case GACT_ACT_RELU: activate32<GACT_ACT_RELU>(v); break;
+    case GACT_ACT_GELU: activate32<GACT_ACT_GELU>(v); break;
+    case GACT_ACT_GELU_TANH: activate32<GACT_ACT_GELU_TANH>(v); break;
+    case GACT_ACT_SILU: activate32<GACT_ACT_SILU>(v); break;
+    default: break;
     }
     if (a.res) add32<DT>(a.res, a.ldr, a.rvec, row, n, a.N, v);
     store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
+}
+template <int DT> __device__ __forceinline__ float bias_at(const GemmArgs& a, int64_t n) {
+    return a.bias && n < a.N ? Elem<DT>::to_float(((const typename Elem<DT>::T*)a.bias)[n]) : 0.0f;
 }
 
 // ---- the matrix product ----------------------------------------------------------------------------------------------
@@ -216,6 +259,7 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
     uint64_t* bars = (uint64_t*)(base + S * R::kStage);
     const uint32_t full = smem_addr(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16, drain = acc_empty + 16;
     __shared__ uint32_t tmem_slot;
+    __shared__ __align__(16) float bias[2][EPI == kEpiLinear ? BN : 4];
     __shared__ volatile int dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -301,11 +345,18 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
         for (int64_t u = blockIdx.x; u < units; u += gridDim.x, n++) {
             const Unit x = unit_at<BN>(a, u);
             const uint32_t acc = n & 1;
+            constexpr int kSpan = BN / 2;             // columns per warp
+            if constexpr (EPI == kEpiLinear) {
+                // this tile's biases as fp32; the buffers alternate, so one barrier of the epilogue warps per tile is enough
+                const int e = threadIdx.x - 128;
+                if (e < BN) bias[acc][e] = bias_at<DT>(a, x.n0 + e);
+                asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+            }
+            // (a warp that gave up goes on through the tiles without storing: every warp meets every barrier)
             const bool ok = mbar_wait(acc_full + 8 * acc, (n >> 1) & 1, &dead);
-            if (!__all_sync(kFull, ok)) break;
+            if (!__all_sync(kFull, ok)) continue;
             tc_fence_after();
             const int64_t row = x.m0 + q * 32 + lane;
-            constexpr int kSpan = BN / 2;             // columns per warp
 #pragma unroll 1
             for (int c = 0; c < kSpan; c += 32) {
                 const int64_t col = x.n0 + half * kSpan + c;
@@ -313,20 +364,19 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
                 uint32_t r[32];
                 tmem_load32(tmem + ((uint32_t)(q * 32) << 16) + acc * BN + half * kSpan + c, r);
                 if (row < a.M) {
-                    float v[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
-                    if constexpr (EPI == kEpiLinear) {
-                        linear_epilogue32<DT>(a, row, col, v);
-                    } else if constexpr (EPI == kEpiStore) {
-                        store32<DT>(a.out, a.ldo, a.ovec, row, col, a.N, v);
-                    } else {
+                    if constexpr (EPI == kEpiPartial) {
                         float* p = a.partial + ((int64_t)x.split * a.M + row) * a.ldp + col;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint32_t w[8] = {r[8 * i], r[8 * i + 1], r[8 * i + 2], r[8 * i + 3], r[8 * i + 4], r[8 * i + 5], r[8 * i + 6], r[8 * i + 7]};
                             st_v8(p + 8 * i, w);
                         }
+                    } else {
+                        float2 v[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                        if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, col, bias[acc] + half * kSpan + c, v);
+                        else store32<DT>(a.out, a.ldo, a.ovec, row, col, a.N, v);
                     }
                 }
                 __syncwarp();
@@ -342,25 +392,31 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
     if (warp == 2) tmem_free(tmem, kTmem);
 }
 
-// Adds the partial sums of the splits in order and runs the epilogue: one thread per 32 columns of a row.
+// Adds the partial sums of the splits in order and runs the epilogue: one thread per 32 columns of a row, 128 rows and the
+// same 32 columns per block.
 template <int DT, int EPI>
 __global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ GemmArgs a) {
-    const int64_t per_row = a.ldp / 32;
-    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (i >= a.M * per_row) return;
-    const int64_t row = i / per_row, n = (i - row * per_row) * 32;
-    float v[32];
+    __shared__ __align__(16) float bias[32];
+    const int64_t n = (int64_t)blockIdx.y * 32;
+    if constexpr (EPI == kEpiLinear) {
+        if (threadIdx.x < 32) bias[threadIdx.x] = bias_at<DT>(a, n + threadIdx.x);
+        __syncthreads();
+    }
+    const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (row >= a.M) return;
+    float2 v[16];
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = 0.0f;
+    for (int i = 0; i < 16; i++) v[i] = splat2(0.0f);
     for (int s = 0; s < a.splits; s++) {
         const float4* p = (const float4*)(a.partial + ((int64_t)s * a.M + row) * a.ldp + n);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float4 f = p[j];
-            v[4 * j] += f.x; v[4 * j + 1] += f.y; v[4 * j + 2] += f.z; v[4 * j + 3] += f.w;
+            v[2 * j] = add2(v[2 * j], make_float2(f.x, f.y));
+            v[2 * j + 1] = add2(v[2 * j + 1], make_float2(f.z, f.w));
         }
     }
-    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, v);
+    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, bias, v);
     else store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
 }
 
@@ -451,8 +507,7 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
     a.ldp = pitch8(a.N);
     const int st = launch_gemm_kernel<DT, A_MN, B_MN, 256, kEpiPartial>(ma, mb, a, s);
     if (st != GACT_OK) return st;
-    const int64_t threads = a.M * (a.ldp / 32);
-    gemm_join_kernel<DT, kEpi><<<(unsigned)((threads + 127) / 128), 128, 0, s>>>(a);
+    gemm_join_kernel<DT, kEpi><<<dim3((unsigned)((a.M + 127) / 128), (unsigned)(a.ldp / 32)), 128, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 
@@ -466,59 +521,83 @@ struct ActBwdArgs {
 };
 constexpr int kAWarps = 8;
 
-// A warp owns 256 columns (8 per lane) and walks rows; eight warps of a block take eight rows at a time.
-template <int DT, bool VEC, bool COMP, bool ACT>
+// A warp owns 256 columns (8 per lane) and walks rows; eight warps of a block take eight rows at a time, and the next rows'
+// loads are issued before the current ones are worked on.
+template <int DT, bool VEC, bool COMP, int ACT>
 __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid_constant__ ActBwdArgs a) {
     using T = typename Elem<DT>::T;
-    __shared__ float fold[kAWarps][8][33];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = (blockIdx.x * 32 + lane) * 8;
-    float db[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) db[j] = 0.0f;
-    const int64_t step = (int64_t)gridDim.y * kAWarps;
+    using Row = Row8<DT, VEC, 32>;
+    constexpr bool kAct = ACT != GACT_ACT_NONE;
     constexpr int U = 2;
-    for (int64_t r = (int64_t)blockIdx.y * kAWarps + warp; r < a.rows; r += U * step) {
-        float g[U][8], z[U][8];
+    __shared__ float fold[kAWarps][8][33];
+    __shared__ __align__(16) uint8_t staging[VEC ? 16 : kAWarps * Stage8<DT, VEC>::kBytes];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    void* stage = staging + warp * Stage8<DT, VEC>::kBytes;
+    const int col = (blockIdx.x * 32 + lane) * 8;
+    float2 db[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) db[i] = splat2(0.0f);
+    const int64_t step = (int64_t)gridDim.y * kAWarps;
+    Row py[U], pz[kAct && !COMP ? U : 1];
+    uint2 pq[U];
+    uint32_t pe[U];
+    auto fetch = [&](int64_t r) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t row = r + u * step;
-            const int cols = row < a.rows ? a.cols : 0;
-            load_row8<DT, VEC>((const T*)a.dy + row * a.ldy, col, cols, g[u]);
-            if constexpr (ACT) {
-                if constexpr (COMP) {
-                    uint2 q = make_uint2(0u, 0u);
-                    uint32_t byte = 1;
-                    if (col < cols) {
-                        const int64_t chunk = row * a.chunks + (col >> 3);
-                        q = ld_stream_u2(a.codes + chunk * 8);
-                        byte = a.scales[chunk >> 2];
-                    }
-                    restore8(q, scale_down8(byte), z[u]);
-                } else {
-                    load_row8<DT, VEC>((const T*)a.z + row * a.ldz, col, cols, z[u]);
+            py[u].load((const T*)a.dy, a.ldy, row, a.rows, col, a.cols);
+            if constexpr (kAct && COMP) {
+                pq[u] = make_uint2(0u, 0u);
+                pe[u] = 1;
+                if (row < a.rows && col < a.cols) {
+                    const int64_t chunk = row * a.chunks + (col >> 3);
+                    pq[u] = ld_stream_u2(a.codes + chunk * 8);
+                    pe[u] = a.scales[chunk >> 2];
                 }
+            } else if constexpr (kAct) {
+                pz[u].load((const T*)a.z, a.ldz, row, a.rows, col, a.cols);
             }
         }
+    };
+    int64_t r = (int64_t)blockIdx.y * kAWarps + warp;
+    fetch(r);
+    for (; r < a.rows; r += U * step) {
+        float2 g[U][4], z[U][4];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t row = r + u * step;
-            if constexpr (ACT) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) g[u][j] *= act_slope(z[u][j], a.act);
-                store_row8<DT, VEC>((T*)a.dz + row * a.ldo, col, row < a.rows ? a.cols : 0, g[u]);
+            uint32_t raw[RawRegs<DT>::N];
+            py[u].get(stage, raw);
+            raw_to_pairs<DT>(raw, g[u]);
+            if constexpr (kAct && COMP) {
+                restore_pairs(pq[u], scale_down8(pe[u]), z[u]);
+            } else if constexpr (kAct) {
+                pz[u].get(stage, raw);
+                raw_to_pairs<DT>(raw, z[u]);
             }
-            if (row < a.rows) {
+        }
+        fetch(r + U * step);
 #pragma unroll
-                for (int j = 0; j < 8; j++) db[j] += g[u][j];
+        for (int u = 0; u < U; u++) {
+            if constexpr (kAct) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) g[u][i] = mul2(g[u][i], act_slope2<ACT>(z[u][i]));
+                Row::store((T*)a.dz, a.ldo, r + u * step, a.rows, col, a.cols, stage, g[u]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // rows past the end: dy = 0 and z = 0, the slope is finite, nothing is added
+                db[i] = add2(db[i], g[u][i]);
             }
         }
     }
     if (!a.partial) return;
 #pragma unroll
-    for (int j = 0; j < 8; j++) fold[warp][j][lane] = db[j];
+    for (int i = 0; i < 4; i++) {
+        fold[warp][2 * i][lane] = db[i].x;
+        fold[warp][2 * i + 1][lane] = db[i].y;
+    }
     __syncthreads();
-    // thread (j, lane): column blockIdx.x * 256 + lane * 8 + j
+    // thread (l, j): column blockIdx.x * 256 + l * 8 + j
     const int j = threadIdx.x & 7, l = threadIdx.x >> 3;
     float sum = 0.0f;
 #pragma unroll
@@ -535,17 +614,26 @@ static int64_t act_bwd_parts(int64_t rows, int64_t cols) {
     return parts < 1 ? 1 : parts > 65535 ? 65535 : parts;
 }
 
-template <int DT> static void dispatch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
+template <int DT, int ACT> static void launch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
     const int block = kAWarps * 32;
-    if (a.act == GACT_ACT_NONE) {
-        if (vec) act_backward_kernel<DT, true, false, false><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, false, false><<<grid, block, 0, s>>>(a);
+    if constexpr (ACT == GACT_ACT_NONE) {
+        if (vec) act_backward_kernel<DT, true, false, ACT><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, ACT><<<grid, block, 0, s>>>(a);
     } else if (a.codes) {
-        if (vec) act_backward_kernel<DT, true, true, true><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, true, true><<<grid, block, 0, s>>>(a);
+        if (vec) act_backward_kernel<DT, true, true, ACT><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, true, ACT><<<grid, block, 0, s>>>(a);
     } else {
-        if (vec) act_backward_kernel<DT, true, false, true><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, false, true><<<grid, block, 0, s>>>(a);
+        if (vec) act_backward_kernel<DT, true, false, ACT><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, ACT><<<grid, block, 0, s>>>(a);
+    }
+}
+template <int DT> static void dispatch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
+    switch (a.act) {
+    case GACT_ACT_RELU: return launch_act_bwd<DT, GACT_ACT_RELU>(a, vec, grid, s);
+    case GACT_ACT_GELU: return launch_act_bwd<DT, GACT_ACT_GELU>(a, vec, grid, s);
+    case GACT_ACT_GELU_TANH: return launch_act_bwd<DT, GACT_ACT_GELU_TANH>(a, vec, grid, s);
+    case GACT_ACT_SILU: return launch_act_bwd<DT, GACT_ACT_SILU>(a, vec, grid, s);
+    default: return launch_act_bwd<DT, GACT_ACT_NONE>(a, vec, grid, s);
     }
 }
 
@@ -589,7 +677,7 @@ extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int6
     if (gemm_scratch(rows, cout, cin) && !scratch) return GACT_ERR_NULL;
     GemmArgs a = {};
     a.M = rows; a.N = cout; a.out = y; a.ldo = cout; a.ovec = vec_bytes(y, cout);
-    a.bias = bias; a.bvec = vec_bytes(bias, 0);
+    a.bias = bias;
     a.res = residual; a.ldr = ld_res; a.rvec = vec_bytes(residual, ld_res);
     a.act = act; a.z = z; a.zvec = vec_bytes(z, cout);
     a.zcodes = (int8_t*)zcodes; a.zscales = (uint8_t*)zscales; a.zpitch = pitch8(cout);
