@@ -56,7 +56,9 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         cmd = ["nvcc", "-shared", "-o", str(OUT)] + [str(o) for o in objs] + ["-gencode", "arch=compute_100a,code=sm_100a"]
         subprocess.check_call(cmd)
     build_fastcall(force)
-    build_hooks(force)
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        for f in [ex.submit(build_hooks, force), ex.submit(build_fused, force)]:
+            f.result()
     return OUT
 
 
@@ -80,15 +82,27 @@ def build_fastcall(force: bool = False):
 
 
 HOOKS = HERE / "gact" / "_hooks.so"
+FUSED = HERE / "gact" / "_fused.so"
 
 
 def build_hooks(force: bool = False):
-    """The native fast path of the saved-tensor hooks (csrc/hooks.cpp): host C++ against libtorch, calling
-    libgact_b200.so beside it through the C ABI.  Optional: without it the hooks run their Python implementation.
-    Returns the path, or None when the compile failed."""
-    src = CSRC / "hooks.cpp"
-    if not (force or _stale(HOOKS, [src, OUT] + sorted(INCLUDE.glob("*.h")))):
-        return HOOKS
+    """The native fast path of the saved-tensor hooks (csrc/hooks.cpp).  Optional: without it the hooks run their Python
+    implementation.  Returns the path, or None when the compile failed."""
+    return build_torch_module(CSRC / "hooks.cpp", HOOKS, force)
+
+
+def build_fused(force: bool = False):
+    """The host side of gact.fused (csrc/fused.cpp).  Required by gact.fused and gact.layers."""
+    if build_torch_module(CSRC / "fused.cpp", FUSED, force) is None:
+        raise RuntimeError("gact/_fused.so was not built")
+    return FUSED
+
+
+def build_torch_module(src: Path, target: Path, force: bool):
+    """Host C++ against libtorch, calling libgact_b200.so beside it through the C ABI."""
+    # the shared library is linked by name: only a changed interface (the headers) makes a module stale
+    if not (force or _stale(target, [src] + sorted(INCLUDE.glob("*.h")))):
+        return target
     import sysconfig
 
     import torch
@@ -96,13 +110,13 @@ def build_hooks(force: bool = False):
     incs = [f"-I{p}" for p in ce.include_paths("cuda")] + [f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}"]
     libs = [f"-L{p}" for p in ce.library_paths("cuda")] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"] + incs + [str(src), "-o", str(HOOKS)] + libs + \
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"] + incs + [str(src), "-o", str(target)] + libs + \
           [f"-L{OUT.parent}", "-l:" + OUT.name, "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
-        print("hooks module not built:", r.stderr.strip().splitlines()[-1] if r.stderr.strip() else r.returncode)
+        print(target.name, "not built:", r.stderr.strip()[-2000:] if r.stderr.strip() else r.returncode)
         return None
-    return HOOKS
+    return target
 
 
 if __name__ == "__main__":

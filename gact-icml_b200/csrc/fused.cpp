@@ -1,0 +1,479 @@
+/*
+ * gact._fused: the host side of gact.fused (argument checks, allocation, library calls) as native code.
+ *
+ * The operators are called once or twice per layer and step, several of them in front of kernels of a few microseconds;
+ * written in Python their checks, allocations and ctypes calls cost 20 us per call, here about 5.  Like gact._hooks this
+ * module belongs to the Python layer (it links against libtorch) and reaches the kernels through the C ABI of
+ * libgact_b200.so.  Errors are raised as Python exceptions: RuntimeError for tensors the operators cannot take (device,
+ * type), ValueError for shapes, TypeError for wrong kinds of arguments.
+ */
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "gact_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+long long g_launches = 0;          // library kernels enqueued from here
+
+int type_code(at::ScalarType t) {
+    switch (t) {
+    case at::kFloat: return GACT_F32;
+    case at::kHalf: return GACT_F16;
+    case at::kBFloat16: return GACT_BF16;
+    default: return -1;
+    }
+}
+
+void check(int status, const char* what) {
+    if (status == GACT_OK) return;
+    const std::string msg = std::string(what) + ": " + gact_error_string(status) + " (status " + std::to_string(status) + ")";
+    if (status == GACT_ERR_SIZE || status == GACT_ERR_DTYPE || status == GACT_ERR_MODE) C10_THROW_ERROR(ValueError, msg);
+    C10_THROW_ERROR(Error, msg);
+}
+
+void check_tensor(const Tensor& t, const char* name, bool half_only, const Tensor* like) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+    TORCH_CHECK(t.layout() == at::kStrided, name, " must be a dense tensor");
+    const int c = type_code(t.scalar_type());
+    TORCH_CHECK(c >= 0 && !(half_only && c == GACT_F32), "The type of ", name, " is not correct!");
+    if (like) TORCH_CHECK(t.device() == like->device(), name, " is on ", t.device().str(), ", the input on ", like->device().str());
+}
+
+int64_t rows_of(const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); i++) n *= t.size(i);
+    return n;
+}
+
+// t as rows of its last dimension with unit stride inside a row; copies only what cannot be described that way
+struct Rows { Tensor t; int64_t rows, ld; };
+Rows as_rows(const Tensor& t) {
+    const int64_t cols = t.size(-1), rows = rows_of(t);
+    if (t.is_contiguous()) return {t, rows, cols};
+    Tensor u = t.dim() == 2 ? t : t.reshape({rows, cols});
+    if (cols > 1 && u.stride(1) != 1) u = u.contiguous();
+    int64_t ld = rows > 1 ? u.stride(0) : cols;
+    if (ld < cols) {                                 // expanded rows
+        u = u.contiguous();
+        ld = cols;
+    }
+    return {u, rows, ld};
+}
+
+// an operand that a tensor map can describe: base and pitch multiples of 16 bytes; anything else is copied to such a pitch
+Rows as_operand(Rows r, int64_t cols, void* stream) {
+    if (r.ld % 8 == 0 && ((uintptr_t)r.t.data_ptr() & 15) == 0) return r;
+    const int64_t pitch = (cols + 7) / 8 * 8;
+    Tensor out = at::empty({r.rows, pitch}, r.t.options());
+    check(gact_repitch16(r.t.data_ptr(), r.ld, r.rows, cols, out.data_ptr(), pitch, stream), "gact_repitch16");
+    g_launches++;
+    return {out, r.rows, pitch};
+}
+
+struct Seed { int stochastic = 0; uint64_t value = 0; };
+
+struct Codes { Tensor codes, scales; };
+Codes empty_codes(int64_t rows, int64_t cols, const Tensor& like) {
+    const int64_t pitch = gact_checkpoint8_pitch(cols);
+    const auto opt = like.options().dtype(at::kChar);
+    return {at::empty({rows, pitch}, opt), at::empty({rows, pitch / GACT_BLOCK8}, opt)};
+}
+void check_codes(const Codes& c, int64_t rows, int64_t cols, const Tensor* like) {
+    const int64_t pitch = gact_checkpoint8_pitch(cols);
+    const Tensor* ts[2] = {&c.codes, &c.scales};
+    const int64_t want[2] = {pitch, pitch / GACT_BLOCK8};
+    for (int i = 0; i < 2; i++) {
+        const Tensor& t = *ts[i];
+        const char* name = i ? "checkpoint scales" : "checkpoint codes";
+        TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+        TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == want[i] && t.is_contiguous() && t.element_size() == 1, name,
+                          " must be contiguous bytes of shape (", rows, ", ", want[i], ")");
+        const Tensor& l = like ? *like : c.codes;
+        TORCH_CHECK(t.device() == l.device(), name, " is on ", t.device().str(), ", the input on ", l.device().str());
+    }
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* stream_of(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+Tensor scratch(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
+std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
+    std::vector<int64_t> s = t.sizes().vec();
+    s.back() = last;
+    return s;
+}
+
+Codes checkpoint8(const Tensor& x, const Seed& seed) {
+    const Rows r = as_rows(x);
+    const int64_t cols = x.size(-1);
+    Codes c = empty_codes(r.rows, cols, x);
+    if (x.numel() == 0) return c;
+    check(gact_checkpoint8(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, seed.stochastic, seed.value, c.codes.data_ptr(),
+                           c.scales.data_ptr(), stream_of(x)), "gact_checkpoint8");
+    g_launches++;
+    return c;
+}
+
+// ---- argument conversion ----------------------------------------------------------------------------------------------
+Tensor tensor_arg(PyObject* o, const char* name) {
+    TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor");
+    return THPVariable_Unpack(o);
+}
+Tensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor_arg(o, name); }
+Seed seed_arg(PyObject* o) {
+    Seed s;
+    if (o != Py_None) {
+        s.stochastic = 1;
+        s.value = PyLong_AsUnsignedLongLongMask(o);
+        if (PyErr_Occurred()) throw python_error();
+    }
+    return s;
+}
+bool bool_arg(PyObject* o) {
+    const int t = PyObject_IsTrue(o);
+    if (t < 0) throw python_error();
+    return t != 0;
+}
+PyObject* wrap(const Tensor& t) {
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(t);
+}
+PyObject* tuple_of(std::initializer_list<Tensor> ts) {
+    PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+    if (!out) throw python_error();
+    Py_ssize_t i = 0;
+    for (const Tensor& t : ts) PyTuple_SET_ITEM(out, i++, wrap(t));
+    return out;
+}
+void count_args(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, "takes ", want, " arguments, got ", n); }
+
+// ---- entry points -----------------------------------------------------------------------------------------------------
+// checkpoint8(input, seed) -> (codes, scales)
+PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 2);
+    const Tensor x = tensor_arg(args[0], "input");
+    check_tensor(x, "input", false, nullptr);
+    TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(x.device());
+    const Codes c = checkpoint8(x, seed_arg(args[1]));
+    return tuple_of({c.codes, c.scales});
+    END_HANDLE_TH_ERRORS
+}
+
+// restore8(codes, scales, shape, dtype) -> tensor
+PyObject* py_restore8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 4);
+    const Codes c{tensor_arg(args[0], "codes"), tensor_arg(args[1], "scales")};
+    TORCH_CHECK_TYPE(PyTuple_Check(args[2]), "shape must be a tuple");
+    TORCH_CHECK_TYPE(THPDtype_Check(args[3]), "dtype must be a torch.dtype");
+    std::vector<int64_t> shape;
+    int64_t rows = 1;
+    const Py_ssize_t nd = PyTuple_GET_SIZE(args[2]);
+    for (Py_ssize_t i = 0; i < nd; i++) {
+        shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[2], i)));
+        if (PyErr_Occurred()) throw python_error();
+        if (i + 1 < nd) rows *= shape.back();
+    }
+    const at::ScalarType st = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+    TORCH_CHECK(type_code(st) >= 0, "The type of the result is not correct!");
+    TORCH_CHECK_VALUE(nd > 0, "a checkpoint has at least one dimension");
+    check_codes(c, rows, shape.back(), nullptr);
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(c.codes.device());
+    const Tensor out = at::empty(shape, c.codes.options().dtype(st));
+    if (out.numel() > 0) {
+        check(gact_restore8(c.codes.data_ptr(), c.scales.data_ptr(), rows, shape.back(), type_code(st), out.data_ptr(), shape.back(), stream_of(out)),
+              "gact_restore8");
+        g_launches++;
+    }
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// type of weight and bias (that of the input, or fp32; both alike)
+at::ScalarType param_type(const Tensor& w, const Tensor& b, int64_t cols, const Tensor& x) {
+    at::ScalarType t = x.scalar_type();
+    bool seen = false;
+    const Tensor* ps[2] = {&w, &b};
+    for (int i = 0; i < 2; i++) {
+        const Tensor& p = *ps[i];
+        const char* name = i ? "bias" : "weight";
+        if (!p.defined()) continue;
+        check_tensor(p, name, false, &x);
+        TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == cols, name, " must have shape (", cols, ",)");
+        TORCH_CHECK((p.scalar_type() == x.scalar_type() || p.scalar_type() == at::kFloat) && (!seen || p.scalar_type() == t), "The type of ", name,
+                    " is not correct!");
+        t = p.scalar_type();
+        seen = true;
+    }
+    return t;
+}
+
+// layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, codes or input, scales, statistics, weight)
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 7);
+    const Tensor x = tensor_arg(args[0], "input");
+    Tensor w = optional_arg(args[1], "weight"), b = optional_arg(args[2], "bias");
+    const double eps = PyFloat_AsDouble(args[3]);
+    if (PyErr_Occurred()) throw python_error();
+    const bool compress = bool_arg(args[4]), save = bool_arg(args[6]);
+    const Seed seed = seed_arg(args[5]);
+    check_tensor(x, "input", false, nullptr);
+    TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
+    const int64_t cols = x.size(-1);
+    TORCH_CHECK_VALUE(cols >= 1 && cols <= GACT_LAYER_NORM_MAX_COLS, "layer norm takes rows of 1 to ", GACT_LAYER_NORM_MAX_COLS, " elements, got ", cols);
+    const at::ScalarType pt = param_type(w, b, cols, x);
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(x.device());
+    if (w.defined()) w = w.contiguous();
+    if (b.defined()) b = b.contiguous();
+    const Rows r = as_rows(x);
+    const Tensor y = at::empty(x.sizes(), x.options());
+    Codes c;
+    Tensor stats;
+    if (save) {
+        stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+        if (compress) c = empty_codes(r.rows, cols, x);
+    }
+    if (r.rows > 0) {
+        float* mean = save ? (float*)stats.data_ptr() : nullptr;
+        check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(), mean,
+                              save ? mean + r.rows : nullptr, ptr(c.codes), ptr(c.scales), seed.stochastic, seed.value, stream_of(x)),
+              "gact_layer_norm");
+        g_launches++;
+    }
+    return tuple_of({y, !save ? Tensor() : compress ? c.codes : x, c.scales, stats, w});
+    END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_backward(grad_output, codes or input, scales or None, statistics, weight, fp32 parameters, need_input,
+//                     need_weight, need_bias) -> (grad of the input, of weight, of bias)
+PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 9);
+    const Tensor dy = tensor_arg(args[0], "grad_output"), kept = tensor_arg(args[1], "saved input"), scales = optional_arg(args[2], "saved scales"),
+                 stats = tensor_arg(args[3], "saved statistics"), w = optional_arg(args[4], "weight");
+    const bool f32 = bool_arg(args[5]), nx = bool_arg(args[6]), nw = bool_arg(args[7]), nb = bool_arg(args[8]);
+    check_tensor(dy, "grad_output", false, &stats);
+    TORCH_CHECK_VALUE(dy.dim() > 0, "grad_output needs at least one dimension");
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(dy.device());
+    const int64_t cols = dy.size(-1);
+    const Rows r = as_rows(dy);
+    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == r.rows && stats.is_contiguous() && stats.scalar_type() == at::kFloat,
+                      "saved statistics do not fit grad_output");
+    Rows x{Tensor(), 0, 0};
+    Codes c;
+    if (scales.defined()) {
+        c = {kept, scales};
+        check_codes(c, r.rows, cols, &dy);
+    } else {
+        check_tensor(kept, "saved input", false, &dy);
+        TORCH_CHECK_VALUE(kept.sizes() == dy.sizes() && kept.scalar_type() == dy.scalar_type(), "saved input does not fit grad_output");
+        x = as_rows(kept);
+    }
+    const at::ScalarType pt = f32 ? at::kFloat : dy.scalar_type();
+    if (w.defined()) {
+        check_tensor(w, "weight", false, &dy);
+        TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == cols && w.is_contiguous() && w.scalar_type() == pt, "weight does not fit grad_output");
+    }
+    Tensor dx, dw, db, scr;
+    if (nx) dx = at::empty(dy.sizes(), dy.options());
+    if (nw) dw = at::empty({cols}, dy.options().dtype(pt));
+    if (nb) db = at::empty({cols}, dy.options().dtype(pt));
+    if (nw || nb) scr = scratch(gact_layer_norm_backward_scratch_bytes(r.rows, cols), dy);
+    if (nx || nw || nb) {
+        const float* mean = (const float*)stats.data_ptr();
+        check(gact_layer_norm_backward(r.t.data_ptr(), type_code(dy.scalar_type()), r.rows, cols, r.ld, ptr(x.t), x.ld, ptr(c.codes), ptr(c.scales),
+                                       mean, mean + r.rows, ptr(w), type_code(pt), ptr(dx), ptr(dw), ptr(db), ptr(scr), stream_of(dy)),
+              "gact_layer_norm_backward");
+        g_launches += 1 + (nw || nb);
+    }
+    return tuple_of({dx, dw, db});
+    END_HANDLE_TH_ERRORS
+}
+
+// linear(input, weight, bias, activation code, residual, compress, seed, save, codes, scales)
+//   -> (y, codes or input, scales, codes of z or z, scales of z)
+PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 10);
+    const Tensor x = tensor_arg(args[0], "input"), w = tensor_arg(args[1], "weight");
+    Tensor b = optional_arg(args[2], "bias");
+    const int act = (int)PyLong_AsLong(args[3]);
+    if (PyErr_Occurred()) throw python_error();
+    const Tensor res = optional_arg(args[4], "residual");
+    const bool compress = bool_arg(args[5]), save = bool_arg(args[7]);
+    const Seed seed = seed_arg(args[6]);
+    Codes c{optional_arg(args[8], "checkpoint codes"), optional_arg(args[9], "checkpoint scales")};
+    check_tensor(x, "input", true, nullptr);
+    check_tensor(w, "weight", true, &x);
+    TORCH_CHECK(w.scalar_type() == x.scalar_type(), "The type of weight is not correct!");
+    TORCH_CHECK_VALUE(x.dim() > 0 && w.dim() == 2 && x.size(-1) == w.size(1), "input ", x.sizes(), " does not fit weight ", w.sizes());
+    const int64_t cout = w.size(0), cin = w.size(1);
+    TORCH_CHECK_VALUE(cin > 0 && cout > 0, "a linear layer needs at least one input and one output feature");
+    const std::vector<int64_t> out_shape = with_last(x, cout);
+    if (b.defined()) {
+        check_tensor(b, "bias", true, &x);
+        TORCH_CHECK(b.scalar_type() == x.scalar_type(), "The type of bias is not correct!");
+        TORCH_CHECK_VALUE(b.dim() == 1 && b.size(0) == cout, "bias must have shape (", cout, ",)");
+    }
+    if (res.defined()) {
+        check_tensor(res, "residual", true, &x);
+        TORCH_CHECK(res.scalar_type() == x.scalar_type(), "The type of residual is not correct!");
+        TORCH_CHECK_VALUE(res.sizes() == at::IntArrayRef(out_shape), "residual must have shape ", at::IntArrayRef(out_shape), ", got ", res.sizes());
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(x.device());
+    if (b.defined()) b = b.contiguous();
+    Rows xr = as_rows(x), wr = as_rows(w);
+    Rows rr{Tensor(), 0, 0};
+    if (res.defined()) rr = as_rows(res);
+    if (c.codes.defined()) check_codes(c, xr.rows, cin, &x);
+    const Tensor y = at::empty(out_shape, x.options());
+    Codes zc;
+    Tensor z;
+    if (save) {
+        if (act && compress) zc = empty_codes(xr.rows, cout, x);
+        else if (act) z = at::empty({xr.rows, cout}, x.options());
+        if (compress && !c.codes.defined()) c = checkpoint8(x, seed);
+    }
+    if (xr.rows > 0) {
+        void* s = stream_of(x);
+        xr = as_operand(xr, cin, s);
+        wr = as_operand(wr, cin, s);
+        const int64_t bytes = gact_linear_scratch_bytes(xr.rows, cin, cout, 0);
+        const Tensor scr = scratch(bytes, x);
+        // the codes of the pre-activation draw their noise from another key than those of the input
+        check(gact_linear(xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, ptr(b), ptr(rr.t), rr.ld, type_code(x.scalar_type()), xr.rows, cin, cout, act,
+                          y.data_ptr(), ptr(z), ptr(zc.codes), ptr(zc.scales), seed.stochastic, seed.value + 0x9E3779B97F4A7C15ull, ptr(scr), s),
+              "gact_linear");
+        g_launches += 1 + (bytes > 0);
+    }
+    if (!save) return tuple_of({y, Tensor(), Tensor(), Tensor(), Tensor()});
+    return tuple_of({y, compress ? c.codes : x, compress ? c.scales : Tensor(), zc.codes.defined() ? zc.codes : z, zc.scales});
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_backward(grad_output, weight, activation code, codes or input, scales or None, codes of z or z or None, scales of z
+//                 or None, need_input, need_weight, need_bias) -> (grad of the input, of weight, of bias)
+PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    count_args(nargs, 10);
+    const Tensor dy = tensor_arg(args[0], "grad_output"), w = tensor_arg(args[1], "weight");
+    const int act = (int)PyLong_AsLong(args[2]);
+    if (PyErr_Occurred()) throw python_error();
+    const Tensor xk = optional_arg(args[3], "saved input"), xs = optional_arg(args[4], "saved scales"), zk = optional_arg(args[5], "saved pre-activation"),
+                 zs = optional_arg(args[6], "saved scales");
+    const bool nx = bool_arg(args[7]), nw = bool_arg(args[8]), nb = bool_arg(args[9]);
+    check_tensor(w, "weight", true, nullptr);
+    check_tensor(dy, "grad_output", true, &w);
+    TORCH_CHECK(dy.scalar_type() == w.scalar_type(), "The type of grad_output is not correct!");
+    TORCH_CHECK_VALUE(w.dim() == 2 && dy.dim() > 0 && dy.size(-1) == w.size(0), "grad_output ", dy.sizes(), " does not fit weight ", w.sizes());
+    const int64_t cout = w.size(0), cin = w.size(1);
+    const int code = type_code(dy.scalar_type());
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(dy.device());
+    Rows dz = as_rows(dy);
+    const int64_t rows = dz.rows;
+    Tensor dx, dw, db;
+    if (nx) dx = at::empty(with_last(dy, cin), dy.options());
+    if (nw) dw = at::empty({cout, cin}, dy.options());
+    if (nb) db = at::empty({cout}, dy.options());
+    if (rows == 0) {
+        if (nw) dw.zero_();
+        if (nb) db.zero_();
+        return tuple_of({dx, dw, db});
+    }
+    void* s = stream_of(dy);
+    // one scratch buffer serves the three steps, which run one after the other on this stream
+    const int64_t ab = nb ? gact_act_backward_scratch_bytes(rows, cout) : 0, xb = nx ? gact_linear_scratch_bytes(rows, cin, cout, 1) : 0,
+                  wb = nw ? gact_linear_scratch_bytes(rows, cin, cout, 2) : 0;
+    const Tensor scr = scratch(std::max(ab, std::max(xb, wb)), dy);
+    if (nb || (act && (nx || nw))) {
+        Rows z{Tensor(), 0, 0};
+        Codes zc;
+        Tensor out;
+        const int64_t pitch = (cout + 7) / 8 * 8;
+        if (act) {
+            TORCH_CHECK_VALUE(zk.defined(), "the pre-activation was not saved");
+            if (zs.defined()) {
+                zc = {zk, zs};
+                check_codes(zc, rows, cout, &dy);
+            } else {
+                check_tensor(zk, "saved pre-activation", true, &dy);
+                TORCH_CHECK_VALUE(zk.dim() == 2 && zk.size(0) == rows && zk.size(1) == cout && zk.scalar_type() == dy.scalar_type(),
+                                  "saved pre-activation does not fit grad_output");
+                z = as_rows(zk);
+            }
+            out = at::empty({rows, pitch}, dy.options());
+        }
+        check(gact_act_backward(dz.t.data_ptr(), code, rows, cout, dz.ld, act, ptr(z.t), z.ld, ptr(zc.codes), ptr(zc.scales), ptr(out), pitch, ptr(db),
+                                ptr(scr), s), "gact_act_backward");
+        g_launches += 1 + nb;
+        if (act) dz = {out, rows, pitch};
+    }
+    if (nx || nw) dz = as_operand(dz, cout, s);
+    if (nx) {
+        const Rows wr = as_operand(as_rows(w), cin, s);
+        check(gact_linear_dgrad(dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, code, rows, cin, cout, dx.data_ptr(), ptr(scr), s), "gact_linear_dgrad");
+        g_launches += 1 + (xb > 0);
+    }
+    if (nw) {
+        TORCH_CHECK_VALUE(xk.defined(), "the input was not saved");
+        Rows x{Tensor(), 0, 0};
+        if (xs.defined()) {
+            const Codes c{xk, xs};
+            check_codes(c, rows, cin, &dy);
+            const int64_t pitch = xk.size(1);
+            x = {at::empty({rows, pitch}, dy.options()), rows, pitch};
+            check(gact_restore8(xk.data_ptr(), xs.data_ptr(), rows, cin, code, x.t.data_ptr(), pitch, s), "gact_restore8");
+            g_launches++;
+        } else {
+            check_tensor(xk, "saved input", true, &dy);
+            TORCH_CHECK_VALUE(xk.dim() > 0 && xk.size(-1) == cin && rows_of(xk) == rows && xk.scalar_type() == dy.scalar_type(),
+                              "saved input does not fit grad_output");
+            x = as_operand(as_rows(xk), cin, s);
+        }
+        check(gact_linear_wgrad(dz.t.data_ptr(), dz.ld, x.t.data_ptr(), x.ld, code, rows, cin, cout, dw.data_ptr(), ptr(scr), s), "gact_linear_wgrad");
+        g_launches += 1 + (wb > 0);
+    }
+    return tuple_of({dx, dw, db});
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launches); }
+
+#define FAST(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL
+PyMethodDef kMethods[] = {
+    {"checkpoint8", FAST(py_checkpoint8), "checkpoint8(input, seed) -> (codes, scales)"},
+    {"restore8", FAST(py_restore8), "restore8(codes, scales, shape, dtype) -> tensor"},
+    {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, kept, scales, statistics, weight)"},
+    {"layer_norm_backward", FAST(py_layer_norm_backward),
+     "layer_norm_backward(grad_output, kept, scales, statistics, weight, fp32 parameters, need_input, need_weight, need_bias) -> three gradients"},
+    {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, codes, scales) -> (y, kept, scales, z, z scales)"},
+    {"linear_backward", FAST(py_linear_backward),
+     "linear_backward(grad_output, weight, activation, kept, scales, z, z scales, need_input, need_weight, need_bias) -> three gradients"},
+    {"launches", py_launches, METH_NOARGS, "library kernels enqueued by this module"},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fused", "Host side of gact.fused.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__fused(void) { return PyModule_Create(&kModule); }

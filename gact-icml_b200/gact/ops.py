@@ -226,9 +226,16 @@ except ImportError:
     _hooks = None
 
 
+# The host side of gact.fused counts its own launches (gact.fused itself requires it).
+try:
+    from gact import _fused
+except ImportError:
+    _fused = None
+
+
 def launches():
-    """Library kernels enqueued so far by this module and by the native hooks."""
-    return launch_count + (_hooks.launches() if _hooks is not None else 0)
+    """Library kernels enqueued so far by this module, by the native hooks and by the fused operators."""
+    return launch_count + (_hooks.launches() if _hooks is not None else 0) + (_fused.launches() if _fused is not None else 0)
 
 
 _dense_cache = {}
