@@ -221,18 +221,22 @@ template <int DT> __device__ __forceinline__ float bias_at(const GemmArgs& a, in
 }
 
 // ---- the matrix product ----------------------------------------------------------------------------------------------
-template <int BN> struct Ring {
-    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+// CG blocks (a cluster) work on one tile of CG * 128 rows and BN columns: each holds its own 128 rows of A, BN / CG columns
+// of B and the accumulators of its rows.  A pair reads every B tile once for 256 rows, which halves the shared-memory
+// traffic that bounds a single block's products.
+template <int CG, int BN> struct Ring {
+    static constexpr int kCols = BN / CG;                     // columns of B per block
+    static constexpr int kA = kBM * kBK * 2, kB = kCols * kBK * 2, kStage = kA + kB;
+    static constexpr int kStages = 196608 / kStage < 8 ? 196608 / kStage : 8;
     static constexpr int kBytes = kStages * kStage + 1024 /* alignment */ + 256 /* barriers */;
 };
 
 struct Unit { int64_t m0, n0; int k0, k1, split; };
 
-// Units (tile x split of the reduction) in an order that keeps concurrently running tiles close together: bands of 16 tile
+// Units (tile x split of the reduction) in an order that keeps concurrently running tiles close together: bands of tile
 // rows, inside a band row by row of columns.
-template <int BN> __device__ __forceinline__ Unit unit_at(const GemmArgs& a, int64_t u) {
-    constexpr int kBand = 16;
+template <int CG, int BN> __device__ __forceinline__ Unit unit_at(const GemmArgs& a, int64_t u) {
+    constexpr int kBand = 16 / CG;
     const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
     Unit x;
     x.split = (int)(u / tiles);
@@ -240,19 +244,19 @@ template <int BN> __device__ __forceinline__ Unit unit_at(const GemmArgs& a, int
     const int64_t band = t / ((int64_t)kBand * a.tiles_n);
     const int rows = (int)min((int64_t)kBand, (int64_t)a.tiles_m - band * kBand);
     const int64_t in = t - band * kBand * a.tiles_n;
-    x.m0 = (band * kBand + in % rows) * kBM;
+    x.m0 = (band * kBand + in % rows) * (kBM * CG);
     x.n0 = (in / rows) * BN;
     x.k0 = x.split * a.per_split;
     x.k1 = min(a.ktiles, x.k0 + a.per_split);
     return x;
 }
 
-template <int DT, bool A_MN, bool B_MN, int BN, int EPI>
-__global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                            const __grid_constant__ GemmArgs a) {
-    using R = Ring<BN>;
+template <int DT, bool A_MN, bool B_MN, int CG, int BN, int EPI>
+__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GemmArgs a) {
+    using R = Ring<CG, BN>;
     constexpr int S = R::kStages;
-    constexpr uint32_t kTmem = 2 * BN < 32 ? 32 : 2 * BN;
+    constexpr uint32_t kTmem = 2 * BN;
     extern __shared__ uint8_t raw[];
     uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t ring = smem_addr(base);
@@ -262,60 +266,71 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
     __shared__ __align__(16) float bias[2][EPI == kEpiLinear ? BN : 4];
     __shared__ volatile int dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 1 ? 0u : cluster_rank();
 
     if (threadIdx.x == 0) {
         dead = 0;
+        // full, acc_empty: those of block 0 are used; empty, acc_full: each block has its own
         for (int i = 0; i < S; i++) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, kEpiWarps); }
+        for (int i = 0; i < 2; i++) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, CG * kEpiWarps); }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_map(&map_a);
         prefetch_map(&map_b);
     }
-    if (warp == 2) tmem_alloc(smem_addr(&tmem_slot), kTmem);
+    __syncwarp();
+    if (warp == 2) tmem_alloc<CG>(smem_addr(&tmem_slot), kTmem);
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CG == 1) __syncthreads();
+    else cluster_sync();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+    const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
-            for (int64_t u = blockIdx.x; u < units && !dead; u += gridDim.x) {
-                const Unit x = unit_at<BN>(a, u);
+            const uint32_t full0 = CG == 1 ? full : peer_addr(full, 0);
+            for (int64_t u = first; u < units && !dead; u += stride) {
+                const Unit x = unit_at<CG, BN>(a, u);
+                const int m0 = (int)(x.m0 + rank * kBM), n0 = (int)(x.n0 + rank * R::kCols);
                 for (int k = x.k0; k < x.k1; k++, it++) {
                     const uint32_t s = it % S, ph = (it / S) & 1;
                     if (!mbar_wait(empty + 8 * s, ph ^ 1, &dead)) break;
-                    const uint32_t bar = full + 8 * s, da = ring + s * R::kStage, db = da + R::kA;
-                    mbar_expect_tx(bar, R::kStage);
+                    const uint32_t bar = full0 + 8 * s, da = ring + s * R::kStage, db = da + R::kA;
+                    // block 0 announces the bytes of both (the other's may land first: the phase still waits for this arrival)
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, CG * R::kStage);
                     if (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; i++) tma_load_2d(da + i * 8192, &map_a, (int)x.m0 + 64 * i, k * kBK, bar);
+                        for (int i = 0; i < kBM / 64; i++) tma_load_2d<CG>(da + i * 8192, &map_a, m0 + 64 * i, k * kBK, bar);
                     } else {
-                        tma_load_2d(da, &map_a, k * kBK, (int)x.m0, bar);
+                        tma_load_2d<CG>(da, &map_a, k * kBK, m0, bar);
                     }
                     if (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; i++) tma_load_2d(db + i * 8192, &map_b, (int)x.n0 + 64 * i, k * kBK, bar);
+                        for (int i = 0; i < R::kCols / 64; i++) tma_load_2d<CG>(db + i * 8192, &map_b, n0 + 64 * i, k * kBK, bar);
                     } else {
-                        tma_load_2d(db, &map_b, k * kBK, (int)x.n0, bar);
+                        tma_load_2d<CG>(db, &map_b, k * kBK, n0, bar);
                     }
                 }
             }
             if (dead) {
-                // give up in order: the copies that were issued (at most one per stage) land before the block ends
+                // give up in order: the copies that were issued (at most one per stage; block 0's barriers count both blocks')
+                // land before the blocks end
                 atomicExch(&g_linear_error, 1);
-                for (uint32_t j = it > (uint32_t)S ? it - S : 0; j < it; j++)
-                    for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full + 8 * (j % S), (j / S) & 1); i++) {}
+                if (rank == 0)
+                    for (uint32_t j = it > (uint32_t)S ? it - S : 0; j < it; j++)
+                        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full + 8 * (j % S), (j / S) & 1); i++) {}
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = mma_idesc(kBM, BN, DT == GACT_BF16, A_MN, B_MN);
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = mma_idesc(CG * kBM, BN, DT == GACT_BF16, A_MN, B_MN);
             uint32_t it = 0, n = 0;
-            for (int64_t u = blockIdx.x; u < units && !dead; u += gridDim.x, n++) {
-                const Unit x = unit_at<BN>(a, u);
+            for (int64_t u = first; u < units && !dead; u += stride, n++) {
+                const Unit x = unit_at<CG, BN>(a, u);
                 const uint32_t acc = n & 1;
                 if (!mbar_wait(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, &dead)) break;
                 tc_fence_after();
@@ -329,21 +344,23 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
                     for (int j = 0; j < kBK / 16; j++) {
                         const uint64_t da = smem_desc(sa + j * (A_MN ? 2048 : 32), A_MN ? 8192 : 16);
                         const uint64_t db = smem_desc(sb + j * (B_MN ? 2048 : 32), B_MN ? 8192 : 16);
-                        mma_f16(d, da, db, idesc, (k > x.k0 || j > 0) ? 1u : 0u);
+                        mma_f16<CG>(d, da, db, idesc, (k > x.k0 || j > 0) ? 1u : 0u);
                     }
-                    mma_commit(empty + 8 * s);
+                    mma_commit<CG>(empty + 8 * s);
                 }
-                mma_commit(acc_full + 8 * acc);
+                mma_commit<CG>(acc_full + 8 * acc);
             }
             // every product has finished before TMEM is given back
-            mma_commit(drain);
+            mma_commit<CG>(drain);
             for (uint32_t i = 0; i < kWaitLimit && !mbar_try(drain, 0); i++) {}
         }
+        __syncwarp();
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t acc_empty0 = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
         uint32_t n = 0;
-        for (int64_t u = blockIdx.x; u < units; u += gridDim.x, n++) {
-            const Unit x = unit_at<BN>(a, u);
+        for (int64_t u = first; u < units; u += stride, n++) {
+            const Unit x = unit_at<CG, BN>(a, u);
             const uint32_t acc = n & 1;
             constexpr int kSpan = BN / 2;             // columns per warp
             if constexpr (EPI == kEpiLinear) {
@@ -356,7 +373,7 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
             const bool ok = mbar_wait(acc_full + 8 * acc, (n >> 1) & 1, &dead);
             if (!__all_sync(kFull, ok)) continue;
             tc_fence_after();
-            const int64_t row = x.m0 + q * 32 + lane;
+            const int64_t row = x.m0 + rank * kBM + q * 32 + lane;
 #pragma unroll 1
             for (int c = 0; c < kSpan; c += 32) {
                 const int64_t col = x.n0 + half * kSpan + c;
@@ -382,14 +399,18 @@ __global__ void __launch_bounds__(kGThreads, 1) gemm_kernel(const __grid_constan
                 __syncwarp();
             }
             tc_fence_before();
-            if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            if (lane == 0) {
+                if constexpr (CG == 1) mbar_arrive(acc_empty + 8 * acc);
+                else mbar_arrive_cluster(acc_empty0 + 8 * acc);
+            }
         }
     }
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CG == 1) __syncthreads();
+    else cluster_sync();
     tc_fence_after();
-    if (warp == 2) tmem_free(tmem, kTmem);
+    if (warp == 2) tmem_free<CG>(tmem, kTmem);
 }
 
 // Adds the partial sums of the splits in order and runs the epilogue: one thread per 32 columns of a row, 128 rows and the
@@ -446,29 +467,35 @@ static bool make_map(CUtensorMap* m, int dtype, const void* p, int64_t rows, int
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Plan { int bn, splits, per_split; int64_t tiles_m, tiles_n; };
+struct Plan { int cg, bn, splits, per_split; int64_t tiles_m, tiles_n; };
 
-// Tile width and splits of the reduction.  (First version: the widest tile, reduction split until the SMs are busy.)
+// Tile shape (two blocks on 256 x 256, one on 128 x 128 or 128 x 64) and splits of the reduction.  For each shape: rounds
+// of tiles over the SMs times the time of a tile, in nanoseconds as measured (a stage of 64 K-elements and the fixed part of
+// a tile), and the join of splits (a launch, and the partial sums written and read).  The cheapest wins.
 static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
-    Plan p;
+    struct Shape { int cg, bn; double stage, tile; };
+    static const Shape shapes[3] = {{2, 256, 300.0, 2500.0}, {1, 128, 190.0, 2200.0}, {1, 64, 130.0, 2000.0}};
     const int sms = sm_count();
     const int64_t kt = (K + kBK - 1) / kBK;
-    p.bn = 256;
-    p.tiles_m = (M + kBM - 1) / kBM;
-    p.tiles_n = (N + p.bn - 1) / p.bn;
-    const int64_t tiles = p.tiles_m * p.tiles_n;
-    int64_t splits = 1;
-    if (tiles * 2 <= sms) {
-        splits = sms / tiles;
-        if (splits > kt / 4) splits = kt / 4;
-        if (splits < 1) splits = 1;
-        if (splits > 16) splits = 16;
+    Plan best = {};
+    double best_t = 1e300;
+    for (const Shape& h : shapes) {
+        Plan p;
+        p.cg = h.cg; p.bn = h.bn;
+        p.tiles_m = (M + kBM * h.cg - 1) / (kBM * h.cg);
+        p.tiles_n = (N + h.bn - 1) / h.bn;
+        const int64_t tiles = p.tiles_m * p.tiles_n, slots = sms / h.cg;
+        for (int64_t splits = 1; splits <= 16; splits *= 2) {
+            p.per_split = (int)((kt + splits - 1) / splits);
+            p.splits = (int)((kt + p.per_split - 1) / p.per_split);
+            if (p.splits != splits || (splits > 1 && p.per_split < 4)) break;
+            const int64_t rounds = (tiles * splits + slots - 1) / slots;
+            double t = 2000.0 + (double)rounds * (p.per_split * h.stage) + h.tile;
+            if (splits > 1) t += 2500.0 + (double)(splits + 1) * (double)M * (double)N * 4.0 / 4000.0;
+            if (t < best_t) { best_t = t; best = p; }
+        }
     }
-    p.per_split = (int)((kt + splits - 1) / splits);
-    if (p.per_split < 1) p.per_split = 1;
-    p.splits = (int)((kt + p.per_split - 1) / p.per_split);
-    if (p.splits < 1) p.splits = 1;
-    return p;
+    return best;
 }
 
 static int64_t gemm_scratch(int64_t M, int64_t N, int64_t K) {
@@ -481,14 +508,20 @@ static int vec_bytes(const void* p, int64_t ld) {
     return (v & 31) == 0 ? 32 : (v & 15) == 0 ? 16 : 2;
 }
 
-template <int DT, bool A_MN, bool B_MN, int BN, int EPI>
+template <int DT, bool A_MN, bool B_MN, int CG, int BN, int EPI>
 static int launch_gemm_kernel(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& a, cudaStream_t s) {
-    auto* k = gemm_kernel<DT, A_MN, B_MN, BN, EPI>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<BN>::kBytes) != cudaSuccess) return GACT_ERR_LAUNCH;
-    const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits;
-    const int64_t grid = units < sm_count() ? units : sm_count();
-    k<<<(unsigned)grid, kGThreads, Ring<BN>::kBytes, s>>>(ma, mb, a);
+    auto* k = gemm_kernel<DT, A_MN, B_MN, CG, BN, EPI>;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<CG, BN>::kBytes) != cudaSuccess) return GACT_ERR_LAUNCH;
+    const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits, slots = sm_count() / CG;
+    const int64_t grid = (units < slots ? units : slots) * CG;
+    k<<<(unsigned)grid, kGThreads, Ring<CG, BN>::kBytes, s>>>(ma, mb, a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+template <int DT, bool A_MN, bool B_MN, int EPI>
+static int launch_gemm_shape(const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& a, cudaStream_t s) {
+    if (p.cg == 2) return launch_gemm_kernel<DT, A_MN, B_MN, 2, 256, EPI>(ma, mb, a, s);
+    if (p.bn == 128) return launch_gemm_kernel<DT, A_MN, B_MN, 1, 128, EPI>(ma, mb, a, s);
+    return launch_gemm_kernel<DT, A_MN, B_MN, 1, 64, EPI>(ma, mb, a, s);
 }
 
 // C (M x N) = A B with the reduction over K.  A: K-major (M rows of K) or MN-major (K rows of M); B likewise with N.
@@ -497,15 +530,15 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
     const Plan p = plan_gemm(a.M, a.N, K);
     CUtensorMap ma, mb;
     const bool ok = make_map(&ma, DT, A, A_MN ? K : a.M, A_MN ? a.M : K, lda, A_MN ? 64 : kBM) &&
-                    make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn);
+                    make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn / p.cg);
     if (!ok) return GACT_ERR_LAUNCH;
     a.ktiles = (int)((K + kBK - 1) / kBK);
     a.tiles_m = (int)p.tiles_m; a.tiles_n = (int)p.tiles_n; a.splits = p.splits; a.per_split = p.per_split;
     constexpr int kEpi = LINEAR ? kEpiLinear : kEpiStore;
-    if (p.splits == 1) return launch_gemm_kernel<DT, A_MN, B_MN, 256, kEpi>(ma, mb, a, s);
+    if (p.splits == 1) return launch_gemm_shape<DT, A_MN, B_MN, kEpi>(p, ma, mb, a, s);
     a.partial = (float*)scratch;
     a.ldp = pitch8(a.N);
-    const int st = launch_gemm_kernel<DT, A_MN, B_MN, 256, kEpiPartial>(ma, mb, a, s);
+    const int st = launch_gemm_shape<DT, A_MN, B_MN, kEpiPartial>(p, ma, mb, a, s);
     if (st != GACT_OK) return st;
     gemm_join_kernel<DT, kEpi><<<dim3((unsigned)((a.M + 127) / 128), (unsigned)(a.ldp / 32)), 128, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
