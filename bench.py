@@ -607,6 +607,8 @@ def train_once(args, workload, level, dev, rank, world, steps, warmup, reference
         kw["batch"] = args.batch
     if workload == "bert_large" and args.layers:
         kw["layers"] = args.layers
+    if workload == "bert_large" and args.fused_layers:
+        kw["fused"] = True
     if workload != "gcn" and args.autocast is not None:
         kw["autocast"] = AUTOCAST[args.autocast]
     wl = workloads.BUILDERS[workload](dev, **kw)
@@ -725,6 +727,8 @@ def memory_ladder(args, dev, reference):
     from gact.controller import Controller
     total = torch.cuda.get_device_properties(dev).total_memory
     kw = {}
+    if args.workload == "bert_large" and args.fused_layers:
+        kw["fused"] = True
     if args.autocast is not None:
         kw["autocast"] = AUTOCAST[args.autocast]
 
@@ -828,6 +832,7 @@ def main():
     ap.add_argument("--level", default="L2", help="optimisation level of the training workloads (L0 = uncompressed)")
     ap.add_argument("--batch", type=int, default=0, help="per-GPU batch of the training workloads (0 = the workload's own)")
     ap.add_argument("--layers", type=int, default=0, help="bert_large only: fewer encoder layers for quick runs")
+    ap.add_argument("--fused-layers", action="store_true", help="bert_large only: linear, GELU and layer norm on gact.layers (8-bit checkpoints)")
     ap.add_argument("--autocast", default=None, choices=["bf16", "fp16", "off"], help="autocast type of the training workloads (default: the workload's own)")
     ap.add_argument("--dp-probe", default="allreduce", choices=["allreduce", "local", "shard"])
     ap.add_argument("--bucket-mb", type=int, default=100, help="DDP gradient bucket size of the training workloads")
@@ -851,6 +856,8 @@ def main():
     args.warmup = max(args.warmup, 3) if args.impl == "ours" else args.warmup
     if args.steps is None:
         args.steps = 5 if (args.impl == "reference" and args.workload == "sweep") else 20
+    if args.fused_layers and (args.workload != "bert_large" or args.impl == "reference"):
+        raise SystemExit("--fused-layers goes with --workload bert_large of this implementation")
     if args.workload != "sweep":
         if not torch.cuda.is_available():
             raise SystemExit("training workloads need a CUDA device")

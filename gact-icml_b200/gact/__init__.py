@@ -2,7 +2,8 @@
 
 Same Python surface as the GACT reference package (``gact/gact/__init__.py``): ``gact.config``,
 ``gact.set_optimization_level``, ``gact.set_adapt_interval``, ``gact.controller.Controller`` and
-``gact.ops``.  All device work goes through ``libgact_b200.so`` (hand-written sm_100a kernels behind a C
+``gact.ops``; ``gact.fused`` and ``gact.layers`` (imported on demand) are training operators and layers that keep their
+own activations as 8-bit checkpoints.  All device work goes through ``libgact_b200.so`` (hand-written sm_100a kernels behind a C
 ABI, bound with ctypes in ``gact._native``); there is no CPU fallback.
 """
 from . import ops

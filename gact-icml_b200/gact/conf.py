@@ -54,6 +54,8 @@ class QuantizationConfig:
         # run the per-tensor part of the hooks in the native module gact/_hooks.so when it was built (same
         # decisions, same dictionaries, about half the host time per saved tensor); False = the Python code
         self.native_hooks = True
+        # the 8-bit checkpoints of gact.layers: False = round to nearest, True = stochastically (unbiased)
+        self.stochastic_checkpoints = False
 
 
 def set_optimization_level(level):

@@ -1,0 +1,226 @@
+"""Autograd functions and modules on the operators of ``gact.fused``.
+
+    layers.convert(model)                      nn.LayerNorm / nn.Linear (and the activation behind a Linear in nn.Sequential)
+    y = layers.linear(x, w, b, activation="gelu", residual=r)
+    y = layers.layer_norm(x, w, b, eps)
+
+What such a layer keeps for its backward pass is its own 8-bit checkpoint (or, at level L0 / with
+``config.compress_activation`` off, the tensors themselves); a ``Controller``'s hooks see int8 codes and parameters, leave
+both alone and go on compressing everything else the model saves.  Converted layers therefore have a fixed width of 8 bits:
+auto precision adapts the other tensors.  ``config.stochastic_checkpoints`` rounds the codes stochastically instead of to
+nearest.
+
+Linear layers compute in float16 / bfloat16 (under autocast the inputs are cast to its type, as torch does); layer norm keeps
+the type of its input.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from gact import fused
+from gact.conf import config
+from gact.fused import Checkpoint8, LayerNormSaved, LinearSaved
+
+_calls = 0
+
+
+def _next_seed():
+    """None (round to nearest), or a seed of its own for every call: from torch's seed, the rank and a running number."""
+    if not config.stochastic_checkpoints:
+        return None
+    global _calls
+    _calls += 1
+    rank = torch.distributed.get_rank() if torch.distributed.is_available() and torch.distributed.is_initialized() else 0
+    return (torch.initial_seed() * 0x9E3779B97F4A7C15 + (rank << 40) + 2 * _calls) & 0xFFFFFFFFFFFFFFFF
+
+
+def _keeps_graph(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _flat(kept):
+    """(tensors, shape, dtype) of a Checkpoint8 or a tensor, for save_for_backward."""
+    if isinstance(kept, Checkpoint8):
+        return (kept.codes, kept.scales), kept.shape, kept.dtype
+    return (kept, None), None, None
+
+
+def _unflat(a, b, shape, dtype):
+    return a if b is None else Checkpoint8(a, b, shape, dtype)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, compress, seed):
+        y, s = fused.op_layer_norm(x, weight, bias, eps, compress=compress, seed=seed)
+        (a, b), shape, dtype = _flat(s.x)
+        ctx.save_for_backward(a, b, s.stats, s.weight)
+        ctx.kept, ctx.meta = (shape, dtype), (s.shape, s.dtype, s.param_dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        a, b, stats, weight = ctx.saved_tensors
+        saved = LayerNormSaved(_unflat(a, b, *ctx.kept), stats, weight, *ctx.meta)
+        n = ctx.needs_input_grad
+        return (*fused.op_layer_norm_backward(dy, saved, (n[0], n[1], n[2])), None, None, None)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, compress, seed, codes, scales):
+        ck = None if codes is None else Checkpoint8(codes, scales, x.shape, x.dtype)
+        y, s = fused.op_linear(x, weight, bias, activation, residual, compress=compress, seed=seed, checkpoint=ck)
+        (xa, xb), xshape, xdtype = _flat(s.x)
+        (za, zb), zshape, zdtype = _flat(s.z)
+        ctx.save_for_backward(xa, xb, za, zb, weight)
+        ctx.kept, ctx.meta = (xshape, xdtype, zshape, zdtype), (activation, s.out_shape, s.has_bias)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xa, xb, za, zb, weight = ctx.saved_tensors
+        xshape, xdtype, zshape, zdtype = ctx.kept
+        saved = LinearSaved(_unflat(xa, xb, xshape, xdtype), _unflat(za, zb, zshape, zdtype), weight, *ctx.meta)
+        n = ctx.needs_input_grad
+        dx, dw, db = fused.op_linear_backward(dy, saved, (n[0], n[1], n[2]))
+        return dx, dw, db, (dy if n[3] else None), None, None, None, None, None
+
+
+def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
+    """Layer norm over the last dimension, differentiable; what it keeps is decided by ``compress`` (None: by the level,
+    ``config.compress_activation``)."""
+    if not _keeps_graph(input, weight, bias):
+        return fused.op_layer_norm(input, weight, bias, eps, save=False)[0]
+    compress = config.compress_activation if compress is None else compress
+    return _LayerNorm.apply(input, weight, bias, eps, compress, _next_seed() if compress else None)
+
+
+def _autocast(*tensors):
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    dt = torch.get_autocast_dtype("cuda")
+    return tuple(t if t is None or not t.is_floating_point() else t.to(dt) for t in tensors)
+
+
+def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None):
+    """activation(input W^T + bias) + residual, differentiable; see ``gact.fused.op_linear``.  ``compress`` as in
+    ``layer_norm``; ``checkpoint``: a Checkpoint8 of the input (in the type it is computed in) to share."""
+    input, weight, bias, residual = _autocast(input, weight, bias, residual)
+    if input.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("gact.layers.linear computes in float16 or bfloat16: cast the model or use torch.autocast "
+                           "(got an input of %s)" % input.dtype)
+    if not _keeps_graph(input, weight, bias, residual):
+        return fused.op_linear(input, weight, bias, activation, residual, save=False)[0]
+    compress = config.compress_activation if compress is None else compress
+    codes = scales = None
+    if compress and checkpoint is not None:
+        if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
+            raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
+        codes, scales = checkpoint.codes, checkpoint.scales
+    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, codes, scales)
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm that keeps its input in 8 bits."""
+
+    def forward(self, input):
+        shape = self.normalized_shape
+        if len(shape) == 1:
+            return layer_norm(input, self.weight, self.bias, self.eps)
+        x = input.flatten(-len(shape))
+        w = None if self.weight is None else self.weight.flatten()
+        b = None if self.bias is None else self.bias.flatten()
+        return layer_norm(x, w, b, self.eps).view(input.shape)
+
+
+class Linear(nn.Linear):
+    """nn.Linear with the activation behind it in its epilogue; keeps its input and pre-activation in 8 bits."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        self.activation = activation
+        self._shared = None
+
+    def forward(self, input, residual=None):
+        checkpoint, self._shared = self._shared, None
+        return linear(input, self.weight, self.bias, self.activation, residual, checkpoint=checkpoint)
+
+    def extra_repr(self):
+        return super().extra_repr() + ("" if self.activation is None else ", activation=%s" % self.activation)
+
+
+def share_input(parent, children):
+    """Lets linear layers that ``parent`` calls with its own first argument share one checkpoint of it (the query, key and
+    value layers of an attention block): made when ``parent`` is called, used by the next call of each child."""
+    children = list(children)
+
+    def before(module, args):
+        x = args[0] if args else None
+        if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(x, *(c.weight for c in children)):
+            x = _autocast(x)[0]
+            if x.dtype in (torch.float16, torch.bfloat16):
+                ck = fused.op_checkpoint8(x.detach(), _next_seed())
+                for c in children:
+                    c._shared = ck
+
+    def after(module, args, output):
+        for c in children:
+            c._shared = None
+
+    parent.register_forward_pre_hook(before)
+    parent.register_forward_hook(after, always_call=True)
+
+
+def activation_name(module):
+    """The name ``linear`` knows an activation module by, or None."""
+    if type(module) is nn.GELU:
+        return "gelu_tanh" if module.approximate == "tanh" else "gelu"
+    return {nn.ReLU: "relu", nn.SiLU: "silu"}.get(type(module))
+
+
+def _as_linear(m, activation=None):
+    out = Linear.__new__(Linear)
+    nn.Module.__init__(out)
+    out.in_features, out.out_features, out.weight, out.bias = m.in_features, m.out_features, m.weight, m.bias
+    out.activation, out._shared = activation, None
+    out.train(m.training)
+    return out
+
+
+def _as_layer_norm(m):
+    out = LayerNorm.__new__(LayerNorm)
+    nn.Module.__init__(out)
+    out.normalized_shape, out.eps, out.elementwise_affine = m.normalized_shape, m.eps, m.elementwise_affine
+    out.weight, out.bias = m.weight, m.bias
+    out.train(m.training)
+    return out
+
+
+def convert(module):
+    """Replaces, in place, every nn.LayerNorm and nn.Linear under ``module`` by the layers above, which take over the very
+    parameters; a GELU / ReLU / SiLU that follows a Linear inside an nn.Sequential moves into its epilogue.  Subclasses of
+    nn.Linear / nn.LayerNorm, and layers that carry hooks, stay as they are.  Returns ``module`` (or its replacement)."""
+    if type(module) is nn.Linear and not _hooked(module):
+        return _as_linear(module)
+    if type(module) is nn.LayerNorm and not _hooked(module):
+        return _as_layer_norm(module)
+    names = list(module._modules)
+    for i, name in enumerate(names):
+        child = module._modules[name]
+        if child is None:
+            continue
+        new = convert(child)
+        if type(module) is nn.Sequential and type(new) is Linear and new.activation is None and i + 1 < len(names):
+            act = activation_name(module._modules[names[i + 1]])
+            if act is not None and not _hooked(module._modules[names[i + 1]]):
+                new.activation = act
+                module._modules[names[i + 1]] = nn.Identity()
+        module._modules[name] = new
+    return module
+
+
+def _hooked(m):
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)

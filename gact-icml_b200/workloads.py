@@ -45,14 +45,32 @@ def _wrap_ddp(model, device, world):
     return model
 
 
-def bert_large(device, batch=64, seq_len=128, world=1, seed=0, layers=24, autocast=torch.bfloat16) -> Workload:
+def fuse_bert(model):
+    """Moves a Hugging Face BERT onto ``gact.layers``: every linear and layer norm, GELU in the epilogue of the layer in
+    front of it, one 8-bit checkpoint of the hidden states for query, key and value."""
+    from gact import layers
+    layers.convert(model)
+    for block in model.bert.encoder.layer:
+        inter = block.intermediate
+        if model.config.hidden_act == "gelu":
+            inter.dense.activation, inter.intermediate_act_fn = "gelu", nn.Identity()
+        att = block.attention.self
+        layers.share_input(att, (att.query, att.key, att.value))
+    return model
+
+
+def bert_large(device, batch=64, seq_len=128, world=1, seed=0, layers=24, autocast=torch.bfloat16, fused=False) -> Workload:
     """BERT-large sequence classification: 24 layers, hidden 1024, 16 heads, FFN 4096, vocab 30522; uniform random
-    token ids, 2 uniform random labels, AdamW lr 2e-5, bf16 autocast."""
+    token ids, 2 uniform random labels, AdamW lr 2e-5, bf16 autocast.  ``fused``: on ``gact.layers`` (needs autocast)."""
     from transformers import BertConfig, BertForSequenceClassification
     torch.manual_seed(seed)
     cfg = BertConfig(vocab_size=30522, hidden_size=1024, num_hidden_layers=layers, num_attention_heads=16,
                      intermediate_size=4096, max_position_embeddings=512, num_labels=2)
     model = BertForSequenceClassification(cfg).to(device)
+    if fused:
+        if autocast is None:
+            raise ValueError("the fused layers compute in float16 or bfloat16: choose an autocast type")
+        fuse_bert(model)
     model.train()
     model = _wrap_ddp(model, device, world)
     opt = torch.optim.AdamW(model.parameters(), lr=2e-5)
@@ -85,7 +103,8 @@ def bert_large(device, batch=64, seq_len=128, world=1, seed=0, layers=24, autoca
 
     return Workload("bert_large", model, opt, step, backprop, batch,
                     {"model": "BERT-large seq-cls (random init)", "layers": layers, "seq_len": seq_len, "batch_per_gpu": batch,
-                     "optimizer": "AdamW lr 2e-5", "autocast": str(autocast).split(".")[-1] if autocast else "off"},
+                     "optimizer": "AdamW lr 2e-5", "autocast": str(autocast).split(".")[-1] if autocast else "off",
+                     **({"fused_layers": True} if fused else {})},
                     forward, finish)
 
 

@@ -91,3 +91,36 @@ def test_python_refuses_host_tensors_and_wrong_arguments():
         fused.op_restore8(c)
     with pytest.raises(RuntimeError, match="type"):
         fused.op_restore8(c, torch.float64)
+
+
+def test_convert_on_the_host():
+    import torch.nn as nn
+    from gact import layers
+
+    class Own(nn.Linear):
+        pass
+
+    m = nn.Sequential(nn.Linear(4, 8), nn.ReLU(), nn.Sequential(nn.LayerNorm(8), nn.Linear(8, 8, bias=False)), nn.GELU(), Own(8, 2))
+    hooked = nn.Linear(2, 2)
+    hooked.register_forward_hook(lambda *a: None)
+    m.append(hooked)
+    params = list(m.parameters())
+    keys = list(m.state_dict())
+    layers.convert(m)
+    assert all(a is b for a, b in zip(params, m.parameters())) and list(m.state_dict()) == keys
+    assert m[0].activation == "relu" and isinstance(m[1], nn.Identity) and type(m[2][0]) is layers.LayerNorm
+    assert m[2][1].bias is None and m[2][1].activation is None and isinstance(m[3], nn.GELU)      # not in one Sequential
+    assert type(m[4]) is Own and m[5] is hooked
+    assert type(layers.convert(nn.Linear(2, 2))) is layers.Linear
+    with pytest.raises(RuntimeError, match="autocast"):
+        m[0](torch.zeros(2, 4))
+
+
+def test_config_has_the_rounding_switch():
+    import gact
+    assert gact.config.stochastic_checkpoints is False
+    from gact import layers
+    assert layers._next_seed() is None
+    gact.config.stochastic_checkpoints = True
+    a, b = layers._next_seed(), layers._next_seed()
+    assert a != b and 0 <= a < 1 << 64
