@@ -248,13 +248,12 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Codes c;
     Tensor stats;
     if (save) {
-        stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+        stats = at::empty({r.rows, 2}, x.options().dtype(at::kFloat));
         if (compress) c = empty_codes(r.rows, cols, x);
     }
     if (r.rows > 0) {
-        float* mean = save ? (float*)stats.data_ptr() : nullptr;
-        check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(), mean,
-                              save ? mean + r.rows : nullptr, ptr(c.codes), ptr(c.scales), seed.stochastic, seed.value, stream_of(x)),
+        check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(),
+                              (float*)ptr(stats), ptr(c.codes), ptr(c.scales), seed.stochastic, seed.value, stream_of(x)),
               "gact_layer_norm");
         g_launches++;
     }
@@ -276,7 +275,7 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
     c10::cuda::CUDAGuard guard(dy.device());
     const int64_t cols = dy.size(-1);
     const Rows r = as_rows(dy);
-    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == r.rows && stats.is_contiguous() && stats.scalar_type() == at::kFloat,
+    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == r.rows && stats.size(1) == 2 && stats.is_contiguous() && stats.scalar_type() == at::kFloat,
                       "saved statistics do not fit grad_output");
     Rows x{Tensor(), 0, 0};
     Codes c;
@@ -299,9 +298,8 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
     if (nb) db = at::empty({cols}, dy.options().dtype(pt));
     if (nw || nb) scr = scratch(gact_layer_norm_backward_scratch_bytes(r.rows, cols), dy);
     if (nx || nw || nb) {
-        const float* mean = (const float*)stats.data_ptr();
         check(gact_layer_norm_backward(r.t.data_ptr(), type_code(dy.scalar_type()), r.rows, cols, r.ld, ptr(x.t), x.ld, ptr(c.codes), ptr(c.scales),
-                                       mean, mean + r.rows, ptr(w), type_code(pt), ptr(dx), ptr(dw), ptr(db), ptr(scr), stream_of(dy)),
+                                       (const float*)stats.data_ptr(), ptr(w), type_code(pt), ptr(dx), ptr(dw), ptr(db), ptr(scr), stream_of(dy)),
               "gact_layer_norm_backward");
         g_launches += 1 + (nw || nb);
     }

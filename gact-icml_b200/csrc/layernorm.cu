@@ -8,6 +8,7 @@
 // the codes and writes dx.  Statistics, sums and the weight gradients are fp32; the variance is taken around the mean
 // (x stays in registers, so the second look at it is free).
 #include "blocks8.cuh"
+#include "tcgen05.cuh"
 
 namespace gact {
 
@@ -16,85 +17,99 @@ struct LnArgs {
     const void* w; const void* b; int wf32;          // weight / bias in fp32 (else in the type of x); null: 1 and 0
     int64_t rows; int cols; float inv_cols; float eps;
     void* y;
-    float* mean; float* rstd;
+    float* stats;                                    // (mean, 1 / deviation) per row, or null
     int8_t* codes; uint8_t* scales; int chunks; int stochastic; PhiloxKeys rk;
 };
 
-// 8 weights starting at column `col` (fp32 or the type of x), 1 without a weight, 0 past the end
+// 8 weights starting at column `col` (fp32 or the type of x); `none` without a weight, 0 past the end
 template <int DT>
-__device__ __forceinline__ void load_param8(const void* p, int f32, int col, int cols, float (&v)[8]) {
+__device__ __forceinline__ void load_param8(const void* p, int f32, int col, int cols, float none, float (&f)[8]) {
     using T = typename Elem<DT>::T;
 #pragma unroll
     for (int j = 0; j < 8; j++)
-        v[j] = !p ? 1.0f : col + j >= cols ? 0.0f : f32 ? __ldg((const float*)p + col + j) : Elem<DT>::to_float(((const T*)p)[col + j]);
+        f[j] = !p ? none : col + j >= cols ? 0.0f : f32 ? __ldg((const float*)p + col + j) : Elem<DT>::to_float(((const T*)p)[col + j]);
 }
-
-// Sum over the TPR threads of a row.  Up to 32 threads: shuffles inside an aligned part of a warp.  More: the block is one
-// row; `buf` holds one value per warp, and consecutive sums use different buffers, so one barrier per sum is enough.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* buf) {
-#pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    if constexpr (TPR > 32) {
-        constexpr int W = TPR / 32;
-        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = buf[0];
-#pragma unroll
-        for (int i = 1; i < W; i++) v += buf[i];
+// all W of them into shared memory as fp32, by the whole block
+template <int DT, int W>
+__device__ __forceinline__ void stage_params(const void* p, int f32, int cols, float none, float* to) {
+    const bool wide = p && ((uintptr_t)p & 15) == 0;
+    for (int col = threadIdx.x * 8; col < W; col += blockDim.x * 8) {
+        float f[8];
+        if (wide && col + 8 <= cols && (f32 || DT == GACT_F32)) {
+            const float4 a = __ldg((const float4*)((const float*)p + col)), b = __ldg((const float4*)((const float*)p + col) + 1);
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+        } else if (wide && col + 8 <= cols) {
+            if constexpr (DT != GACT_F32) {
+                const uint4 a = __ldg((const uint4*)((const typename Elem<DT>::T*)p + col));
+                const uint32_t raw[4] = {a.x, a.y, a.z, a.w};
+                raw_to_float<DT>(raw, f);
+            }
+        } else {
+            load_param8<DT>(p, f32, col, cols, none, f);
+        }
+        *(float4*)(to + col) = make_float4(f[0], f[1], f[2], f[3]);
+        *(float4*)(to + col + 4) = make_float4(f[4], f[5], f[6], f[7]);
     }
-    return v;
 }
 
-// A row is held by TPR threads, CH chunks of 8 elements each (chunk c of thread t: columns (t + c TPR) 8 ..).  Blocks are
-// resident and walk the rows; the next row's loads are issued before the current row is worked on, and weight and bias wait
-// in shared memory as fp32 (re-reading and widening them for every row cost as much as the norm itself).
+// A row is held by TPR threads, CH chunks of 8 elements each (chunk c of thread t: columns (t + c TPR) 8 ..).  Resident blocks walk the rows; the next row's loads are
+// issued before the current row is worked on, and weight and bias wait in shared memory as fp32.
 template <int DT, int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const __grid_constant__ LnArgs a) {
     using T = typename Elem<DT>::T;
-    constexpr int SUB = TPR < 32 ? TPR : 32, W = TPR * CH * 8;
+    constexpr int SUB = TPR < 32 ? TPR : 32, W = TPR * CH * 8, WARPS = TPR > 32 ? TPR / 32 : 1;
     using Row = Row8<DT, VEC, SUB>;
     extern __shared__ __align__(16) uint8_t dyn[];
     float* pw = (float*)dyn;
     float* pb = pw + W;
     void* stage = dyn + 2 * W * sizeof(float) + (threadIdx.x >> 5) * Stage8<DT, VEC>::kBytes;
-    __shared__ float buf[2][2][TPR > 32 ? TPR / 32 : 1];
-    const int t = threadIdx.x % TPR, groups = blockDim.x / TPR, grp = threadIdx.x / TPR;
-    for (int c = threadIdx.x; c < W; c += blockDim.x) {
-        const bool in = c < a.cols;
-        pw[c] = !a.w ? 1.0f : !in ? 0.0f : (a.wf32 ? ((const float*)a.w)[c] : Elem<DT>::to_float(((const T*)a.w)[c]));
-        pb[c] = !a.b || !in ? 0.0f : (a.wf32 ? ((const float*)a.b)[c] : Elem<DT>::to_float(((const T*)a.b)[c]));
-    }
-    __syncthreads();
+    __shared__ float buf[2][2][WARPS];
+    const int t = threadIdx.x % TPR, groups = blockDim.x / TPR, grp = threadIdx.x / TPR, lane = threadIdx.x & 31;
     const int64_t step = (int64_t)gridDim.x * groups;
-    int64_t base = (int64_t)blockIdx.x * groups;
+    int64_t row = (int64_t)blockIdx.x * groups + grp;
     Row x[CH];
 #pragma unroll
-    for (int c = 0; c < CH; c++) x[c].load((const T*)a.x, a.ldx, base + grp, a.rows, (t + c * TPR) * 8, a.cols);
-    for (int phase = 0; base < a.rows; base += step, phase ^= 1) {
-        const int64_t row = base + grp;
-        uint32_t raw[CH][RawRegs<DT>::N];
+    for (int c = 0; c < CH; c++) x[c].load((const T*)a.x, a.ldx, row, a.rows, (t + c * TPR) * 8, a.cols);
+    stage_params<DT, W>(a.w, a.wf32, a.cols, 1.0f, pw);
+    stage_params<DT, W>(a.b, a.wf32, a.cols, 0.0f, pb);
+    __syncthreads();
+    // a sum over the threads of the row; the buffers alternate from sum to sum and from row to row: one barrier each
+    auto row_sum = [&](float v, float* b) {
 #pragma unroll
-        for (int c = 0; c < CH; c++) x[c].get(stage, raw[c]);
+        for (int o = SUB / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        if constexpr (TPR > 32) {
+            if (lane == 0) b[threadIdx.x >> 5] = v;
+            __syncthreads();
+            v = b[0];
+#pragma unroll
+            for (int i = 1; i < WARPS; i++) v += b[i];
+        }
+        return v;
+    };
+    // (groups of a block run the same number of steps: `row - grp` decides)
+    for (int phase = 0; row - grp < a.rows; row += step, phase ^= 1) {
+        float2 v[CH][4];
+        uint32_t top[CH];
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            uint32_t raw[RawRegs<DT>::N];
+            x[c].get(stage, raw);
+            raw_to_pairs<DT>(raw, v[c]);
+            top[c] = absmax8<DT>(raw);
+        }
 #pragma unroll
         for (int c = 0; c < CH; c++) x[c].load((const T*)a.x, a.ldx, row + step, a.rows, (t + c * TPR) * 8, a.cols);
         float2 s2 = splat2(0.0f);
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            float2 v[4];
-            raw_to_pairs<DT>(raw[c], v);
-            s2 = add2(s2, add2(add2(v[0], v[1]), add2(v[2], v[3])));
-        }
-        const float mean = row_sum<TPR>(s2.x + s2.y, buf[phase][0]) * a.inv_cols;
+        for (int c = 0; c < CH; c++) s2 = add2(s2, add2(add2(v[c][0], v[c][1]), add2(v[c][2], v[c][3])));
+        const float mean = row_sum(s2.x + s2.y, buf[phase][0]) * a.inv_cols;
         float2 q2 = splat2(0.0f);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            float2 v[4];
-            raw_to_pairs<DT>(raw[c], v);
             const int col = (t + c * TPR) * 8;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float2 d = add2(v[i], splat2(-mean));
+                float2 d = add2(v[c][i], splat2(-mean));
                 if (VEC) { if (col >= a.cols) d = splat2(0.0f); }
                 else {
                     if (col + 2 * i >= a.cols) d.x = 0.0f;
@@ -103,22 +118,18 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
                 q2 = fma2(d, d, q2);
             }
         }
-        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q2.x + q2.y, buf[phase][1]) * a.inv_cols + a.eps);
+        // rsqrtf: at most 2 steps off
+        const float rstd = rsqrtf(row_sum(q2.x + q2.y, buf[phase][1]) * a.inv_cols + a.eps);
         const bool live = row < a.rows;
-        if (live && t == 0 && a.mean) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
-        }
+        if (live && t == 0 && a.stats) ((float2*)a.stats)[row] = make_float2(mean, rstd);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int col = (t + c * TPR) * 8;
-            float2 v[4], o[4];
-            raw_to_pairs<DT>(raw[c], v);
+            float2 o[4];
             if (a.codes) {
                 uint32_t byte;
                 const uint64_t chunk = (uint64_t)row * a.chunks + (t + c * TPR);
-                const uint32_t m = absmax8<DT>(raw[c]);
-                const uint2 q = a.stochastic ? codes8<DT, true>(v, m, a.rk, chunk, byte) : codes8<DT, false>(v, m, a.rk, chunk, byte);
+                const uint2 q = a.stochastic ? codes8<DT, true>(v[c], top[c], a.rk, chunk, byte) : codes8<DT, false>(v[c], top[c], a.rk, chunk, byte);
                 if (live && t + c * TPR < a.chunks) {
                     st_stream_u2(a.codes + chunk * 8, q);
                     if ((t & 3) == 0) a.scales[chunk >> 2] = (uint8_t)byte;
@@ -127,8 +138,8 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const float4 w = *(const float4*)(pw + col + 2 * i), b = *(const float4*)(pb + col + 2 * i);
-                o[i] = fma2(mul2(add2(v[i], splat2(-mean)), splat2(rstd)), make_float2(w.x, w.y), make_float2(b.x, b.y));
-                o[i + 1] = fma2(mul2(add2(v[i + 1], splat2(-mean)), splat2(rstd)), make_float2(w.z, w.w), make_float2(b.z, b.w));
+                o[i] = fma2(mul2(add2(v[c][i], splat2(-mean)), splat2(rstd)), make_float2(w.x, w.y), make_float2(b.x, b.y));
+                o[i + 1] = fma2(mul2(add2(v[c][i + 1], splat2(-mean)), splat2(rstd)), make_float2(w.z, w.w), make_float2(b.z, b.w));
             }
             Row::store((T*)a.y, a.cols, row, a.rows, col, a.cols, stage, o);
         }
@@ -137,47 +148,52 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
 
 template <int DT, int TPR, int CH, bool VEC> static int launch_ln_vec(const LnArgs& a, cudaStream_t s) {
     auto* k = layer_norm_kernel<DT, TPR, CH, VEC>;
-    // rows of up to a warp share a block, fewer of them when there are few rows
-    int block = TPR;
-    if (TPR <= 32) {
-        block = 128;
-        while (block > 32 && a.rows * TPR < (int64_t)sm_count() * block) block /= 2;
-    }
-    const int smem = 2 * TPR * CH * 8 * (int)sizeof(float) + block / 32 * Stage8<DT, VEC>::kBytes;
-    constexpr int kMost = 2 * TPR * CH * 8 * (int)sizeof(float) + (TPR > 128 ? TPR : 128) / 32 * Stage8<DT, VEC>::kBytes;
-    if (kMost > 48 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return GACT_ERR_LAUNCH;
+    constexpr int kBlock = TPR > 32 ? TPR : 128;
+    constexpr int kSmem = 2 * TPR * CH * 8 * (int)sizeof(float) + kBlock / 32 * Stage8<DT, VEC>::kBytes;
+    if (kSmem > 40 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return GACT_ERR_LAUNCH;
     static std::atomic<int> cache[kMaxDevices];
-    const int64_t want = (a.rows + block / TPR - 1) / (block / TPR);
-    // (the count is that of full blocks; smaller blocks only run when there are too few rows for it to matter)
-    const int64_t most = (int64_t)sm_count() * resident_blocks(k, TPR > 128 ? TPR : TPR > 32 ? TPR : 128, kMost, cache);
-    k<<<(unsigned)(want < most ? want : most), block, smem, s>>>(a);
+    const int64_t per = kBlock / TPR, want = (a.rows + per - 1) / per;
+    const int64_t most = (int64_t)sm_count() * resident_blocks(k, kBlock, kSmem, cache);
+    k<<<(unsigned)(want < most ? want : most), kBlock, kSmem, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 template <int DT, int TPR, int CH> static int launch_ln(const LnArgs& a, bool vec, cudaStream_t s) {
     return vec ? launch_ln_vec<DT, TPR, CH, true>(a, s) : launch_ln_vec<DT, TPR, CH, false>(a, s);
 }
+// Many rows: 32 elements per thread, so that the reductions, the row's scalars and the addresses (about 100 instructions per
+// thread and row) do not bound the kernel.  Few rows: latency counts, and every row is spread over as many threads as it has
+// chunks.
 template <int DT> static int dispatch_ln(const LnArgs& a, bool vec, cudaStream_t s) {
     const int h = a.cols;
+    if (vec && a.rows > (int64_t)sm_count() * 8 && h > 64 && h <= 8192) {
+        if (h <= 128) return launch_ln_vec<DT, 8, 2, true>(a, s);
+        if (h <= 256) return launch_ln_vec<DT, 8, 4, true>(a, s);
+        if (h <= 512) return launch_ln_vec<DT, 16, 4, true>(a, s);
+        if (h <= 1024) return launch_ln_vec<DT, 32, 4, true>(a, s);
+        if (h <= 2048) return launch_ln_vec<DT, 64, 4, true>(a, s);
+        if (h <= 4096) return launch_ln_vec<DT, 128, 4, true>(a, s);
+        return launch_ln_vec<DT, 256, 4, true>(a, s);
+    }
     if (h <= 32) return launch_ln<DT, 4, 1>(a, vec, s);
     if (h <= 64) return launch_ln<DT, 8, 1>(a, vec, s);
     if (h <= 128) return launch_ln<DT, 16, 1>(a, vec, s);
     if (h <= 256) return launch_ln<DT, 32, 1>(a, vec, s);
-    if (h <= 512) return launch_ln<DT, 32, 2>(a, vec, s);
-    if (h <= 1024) return launch_ln<DT, 32, 4>(a, vec, s);
-    if (h <= 2048) return launch_ln<DT, 128, 2>(a, vec, s);
-    if (h <= 4096) return launch_ln<DT, 256, 2>(a, vec, s);
+    if (h <= 512) return launch_ln<DT, 64, 1>(a, vec, s);
+    if (h <= 1024) return launch_ln<DT, 128, 1>(a, vec, s);
+    if (h <= 2048) return launch_ln<DT, 256, 1>(a, vec, s);
+    if (h <= 4096) return launch_ln<DT, 512, 1>(a, vec, s);
     if (h <= 8192) return launch_ln<DT, 512, 2>(a, vec, s);
     return launch_ln<DT, 512, 4>(a, vec, s);
 }
 
-constexpr int kLnBwdRows = 2;                       // rows a block (or row group) works on side by side
+constexpr int kLnBwdRows = 2;                       // rows a block (or row group) of the plain kernel works on side by side
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 struct LnBwdArgs {
     const void* dy; int64_t ldy;
     const void* x; int64_t ldx;                       // the input itself, or null:
     const int8_t* codes; const uint8_t* scales; int chunks;
-    const float* mean; const float* rstd;
+    const float* stats;
     const void* w; int wf32;
     int64_t rows; int cols; float inv_cols;
     void* dx;                                          // null: weight gradients only
@@ -185,7 +201,7 @@ struct LnBwdArgs {
     int width;
 };
 
-// A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
+// For short rows, few rows and rows that do not start on 16-byte boundaries.  A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
 // walks the rows, R of them (per row group) side by side: one barrier serves 2 R sums, and the next R rows' loads are issued
 // before the current ones are worked on.  Block sums go to `partial`, added up in a fixed order afterwards: no atomics.
 template <int DT, int TPR, int CH, int R, bool VEC, bool COMP>
@@ -202,7 +218,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         float f[8];
-        load_param8<DT>(a.w, a.wf32, (t + c * TPR) * 8, a.cols, f);
+        load_param8<DT>(a.w, a.wf32, (t + c * TPR) * 8, a.cols, 1.0f, f);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             w[c][i] = make_float2(f[2 * i], f[2 * i + 1]);
@@ -212,14 +228,13 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
     Row py[R][CH], px[COMP ? 1 : R][COMP ? 1 : CH];
     uint2 pq[R][CH];
     uint32_t pe[R][CH];
-    float pm[R], pr[R];
+    float2 ps[R];
     auto fetch = [&](int64_t base) {
 #pragma unroll
         for (int k = 0; k < R; k++) {
             const int64_t row = base + k * GROUPS + grp;
             const bool live = row < a.rows;
-            pm[k] = live ? __ldg(a.mean + row) : 0.0f;
-            pr[k] = live ? __ldg(a.rstd + row) : 0.0f;
+            ps[k] = live ? __ldg((const float2*)a.stats + row) : make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 py[k][c].load((const T*)a.dy, a.ldy, row, a.rows, (t + c * TPR) * 8, a.cols);
@@ -246,8 +261,8 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
         float rs[R];
 #pragma unroll
         for (int k = 0; k < R; k++) {
-            rs[k] = pr[k];
-            const float2 off = splat2(-pm[k] * pr[k]);
+            rs[k] = ps[k].y;
+            const float2 off = splat2(-ps[k].x * ps[k].y);
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 uint32_t raw[RawRegs<DT>::N];
@@ -363,21 +378,230 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
     }
 }
 
-// Threads per row, chunks per thread and rows per step of the backward pass, by the row length.
-struct LnBwdShape { int tpr, block, r; };
-static LnBwdShape ln_bwd_shape(int64_t cols) {
-    const int tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
-    return {tpr, tpr > 32 ? tpr : 128, cols <= 4096 ? kLnBwdRows : 1};
+// ---- long rows: rings of bulk copies ----------------------------------------------------------------------------------
+// Rows that start on 16-byte boundaries are brought into shared memory by bulk copies (one elected thread, one instruction
+// per row and tensor), kRingStages rows deep, and worked on there: a row is read from shared memory as often as it is needed,
+// so it costs no registers while it waits and the loads in flight do not depend on the number of warps.  The block works on
+// one row.  Waits are bounded (see mbar_wait); one that runs out is recorded and the block goes on to its end without waiting.
+constexpr int kRingStages = 3;
+__device__ int g_norm_error = 0;
+
+struct RowRing {
+    uint32_t bar; volatile int* dead; uint32_t issued, taken;      // rows issued and taken so far
+    __device__ __forceinline__ uint32_t stage(uint32_t n) const { return n % kRingStages; }
+    // the next row to work on has landed; returns its stage
+    __device__ __forceinline__ uint32_t take() {
+        const uint32_t s = stage(taken);
+        mbar_wait(bar + 8 * s, (taken / kRingStages) & 1, dead);
+        taken++;
+        return s;
+    }
+    // elected thread: announces a row of `bytes`; the copies follow
+    __device__ __forceinline__ uint32_t announce(uint32_t bytes) {
+        const uint32_t s = stage(issued);
+        mbar_expect_tx(bar + 8 * s, bytes);
+        issued++;
+        return s;
+    }
+    // elected thread, at the end: a ring that gave up waits (again bounded) for the copies that may still be in flight
+    __device__ __forceinline__ void close() {
+        if (!*dead) return;
+        atomicExch(&g_norm_error, 1);
+        for (uint32_t j = issued > (uint32_t)kRingStages ? issued - kRingStages : 0; j < issued; j++)
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(bar + 8 * (j % kRingStages), (j / kRingStages) & 1); i++) {}
+    }
+};
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
-// Resident blocks: 512 threads per SM (more only lengthens the sum of the partials, 2 x cols floats per block).
-static int64_t ln_bwd_blocks(int64_t rows, int64_t cols) {
-    const LnBwdShape p = ln_bwd_shape(cols);
-    const int64_t per = (int64_t)(p.block / p.tpr) * p.r;
-    const int64_t most = (int64_t)sm_count() * (512 / p.block);
-    const int64_t want = (rows + per - 1) / per;
+template <int DT> __device__ __forceinline__ void take_raw(const uint8_t* row, int chunk, uint32_t (&raw)[RawRegs<DT>::N]) {
+    const uint4* p = (const uint4*)(row + chunk * 8 * Elem<DT>::kBytes);
+    const uint4 a = p[0];
+    raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+    if constexpr (DT == GACT_F32) {
+        const uint4 b = p[1];
+        raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+    }
+}
+
+// dy and the codes of a row (or x) are read twice, before and after the sums; the weight gradients of a thread's columns stay
+// in its registers.
+template <int DT, int TPR, int CH, bool COMP>
+__global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __grid_constant__ LnBwdArgs a) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = TPR * CH * 8, WARPS = TPR / 32, N = RawRegs<DT>::N;
+    constexpr int YROW = W * Elem<DT>::kBytes, XROW = COMP ? W : YROW, ROW = YROW + XROW;
+    extern __shared__ __align__(128) uint8_t dyn[];               // weights (fp32), rings
+    float* pw = (float*)dyn;
+    __shared__ __align__(8) uint64_t bars[kRingStages];
+    __shared__ float2 buf[2][WARPS];
+    __shared__ volatile int dead;
+    const int t = threadIdx.x, lane = threadIdx.x & 31;
+    uint8_t* ring = dyn + W * sizeof(float);
+    if (t == 0) {
+        dead = 0;
+        for (int i = 0; i < kRingStages; i++) mbar_init(smem_addr(bars + i), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    RowRing r{smem_addr(bars), &dead, 0, 0};
+    const int64_t step = gridDim.x;
+    int64_t row = blockIdx.x;
+    const uint32_t ybytes = (uint32_t)a.cols * Elem<DT>::kBytes, xbytes = COMP ? (uint32_t)a.chunks * 8 : ybytes;
+    auto issue = [&](int64_t w) {
+        if (w < a.rows) {
+            const uint32_t s = r.announce(ybytes + xbytes), to = smem_addr(ring + s * ROW), bar = r.bar + 8 * s;
+            bulk_copy(to, (const T*)a.dy + w * a.ldy, ybytes, bar);
+            if (COMP) bulk_copy(to + YROW, a.codes + w * a.chunks * 8, xbytes, bar);
+            else bulk_copy(to + YROW, (const T*)a.x + w * a.ldx, xbytes, bar);
+        }
+    };
+    if (t == 0)
+        for (int i = 0; i < kRingStages - 1; i++) issue(row + i * step);
+    // statistics and scales are a few bytes per row: plain loads, one row ahead
+    float2 ps = splat2(0.0f);
+    uint32_t pe[CH];
+    auto fetch = [&](int64_t w) {
+        if (w < a.rows) {
+            ps = __ldg((const float2*)a.stats + w);
+            if (COMP) {
+                const uint8_t* p = a.scales + ((w * a.chunks + t) >> 2);
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+                    if (t + c * TPR < a.chunks) pe[c] = __ldg(p + c * (TPR / 4));
+            }
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < CH; c++) pe[c] = 1;
+    fetch(row);
+    stage_params<DT, W>(a.w, a.wf32, a.cols, 1.0f, pw);
+    __syncthreads();
+    float2 dw[CH][4], db[CH][4];
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) dw[c][i] = db[c][i] = splat2(0.0f);
+    T* dx = (T*)a.dx + row * a.cols + t * 8;
+    for (int phase = 0; row < a.rows; row += step, phase ^= 1) {
+        const float rs = ps.y, off = -ps.x * ps.y;
+        float up[CH];
+#pragma unroll
+        for (int c = 0; c < CH; c++) up[c] = COMP ? scale_down8(pe[c]) * rs : rs;
+        fetch(row + step);
+        const uint8_t* in = ring + r.take() * ROW;
+        // dy and x^ of chunk c: x^ = x' r - mean r; a code is a small integer and its scale a power of two, so x' r is one product
+        auto expand = [&](int c, float2 (&g)[4], float2 (&xh)[4]) {
+            uint32_t raw[N];
+            take_raw<DT>(in, t + c * TPR, raw);
+            raw_to_pairs<DT>(raw, g);
+            if constexpr (COMP) {
+                code_pairs(*(const uint2*)(in + YROW + (t + c * TPR) * 8), xh);
+            } else {
+                take_raw<DT>(in + YROW, t + c * TPR, raw);
+                raw_to_pairs<DT>(raw, xh);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) xh[i] = fma2(xh[i], splat2(up[c]), splat2(off));
+        };
+        float2 s1 = splat2(0.0f), s2 = splat2(0.0f);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            if ((t + c * TPR) * 8 < a.cols) {                    // (past the row: whatever the ring holds)
+                float2 g[4], xh[4];
+                expand(c, g, xh);
+                const float* pc = pw + (t + c * TPR) * 8;
+                const float4 wa = *(const float4*)pc, wb = *(const float4*)(pc + 4);
+                const float2 w[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    dw[c][i] = fma2(g[i], xh[i], dw[c][i]);
+                    db[c][i] = add2(db[c][i], g[i]);
+                    g[i] = mul2(g[i], w[i]);
+                    s1 = add2(s1, g[i]);
+                    s2 = fma2(g[i], xh[i], s2);
+                }
+            }
+        }
+        float2 s = make_float2(s1.x + s1.y, s2.x + s2.y);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) s = add2(s, make_float2(__shfl_xor_sync(kFull, s.x, o), __shfl_xor_sync(kFull, s.y, o)));
+        // (two buffers in turn: one barrier per row is enough)
+        if (lane == 0) buf[phase][threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = buf[phase][0];
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) s = add2(s, buf[phase][i]);
+        // every thread is past the row before this one: its stage takes the row kRingStages - 1 steps on
+        if (t == 0) issue(row + (kRingStages - 1) * step);
+        if (a.dx) {
+            // r (g - c1 - x^ c2)
+            const float2 e1 = splat2(-s.x * a.inv_cols * rs), e2 = splat2(-s.y * a.inv_cols * rs);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                if ((t + c * TPR) * 8 < a.cols) {
+                    float2 g[4], xh[4];
+                    expand(c, g, xh);
+                    const float* pc = pw + (t + c * TPR) * 8;
+                    const float4 wa = *(const float4*)pc, wb = *(const float4*)(pc + 4);
+                    const float2 w[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) g[i] = fma2(xh[i], e2, fma2(mul2(g[i], w[i]), splat2(rs), e1));
+                    uint32_t raw[N];
+                    pairs_to_raw<DT>(g, raw);
+                    st_stream_u4(dx + c * TPR * 8, make_uint4(raw[0], raw[1], raw[2], raw[3]));
+                    if constexpr (DT == GACT_F32) st_stream_u4(dx + c * TPR * 8 + 4, make_uint4(raw[4], raw[5], raw[6], raw[7]));
+                }
+            }
+        }
+        dx += step * a.cols;
+    }
+    if (t == 0) r.close();
+    if (!a.partial) return;
+    float* p = a.partial + (int64_t)blockIdx.x * 2 * a.width;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int col = (t + c * TPR) * 8;
+        if (col < a.width) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                *(float4*)(p + col + 2 * i) = make_float4(dw[c][i].x, dw[c][i].y, dw[c][i + 1].x, dw[c][i + 1].y);
+                *(float4*)(p + a.width + col + 2 * i) = make_float4(db[c][i].x, db[c][i].y, db[c][i + 1].x, db[c][i + 1].y);
+            }
+        }
+    }
+}
+
+// Rings need rows long enough to be worth a copy each, and several rows per block to run ahead.
+static bool ln_ring(bool vec, int64_t rows, int64_t cols) { return vec && cols > 1024 && cols <= 8192 && rows > (int64_t)sm_count() * 8; }
+
+// Shapes and blocks of the backward pass.  The number of blocks decides how many partial sums there are (2 x cols floats per
+// block), so it must not depend on anything but the sizes: 512 threads per SM for the plain kernel, and for the rings as many
+// blocks as their registers and shared memory let an SM hold.
+struct LnBwdShape { bool ring; int tpr, block, rows_per_step, per_sm; };
+static LnBwdShape ln_bwd_shape(bool vec, int64_t rows, int64_t cols) {
+    if (ln_ring(vec, rows, cols)) return cols <= 4096 ? LnBwdShape{true, 128, 128, 1, 4} : LnBwdShape{true, 512, 512, 1, 1};
+    const int tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
+    const int block = tpr > 32 ? tpr : 128;
+    return {false, tpr, block, block / tpr * (cols <= 4096 ? kLnBwdRows : 1), 512 / block};
+}
+static int64_t ln_bwd_blocks(bool vec, int64_t rows, int64_t cols) {
+    const LnBwdShape p = ln_bwd_shape(vec, rows, cols);
+    const int64_t want = (rows + p.rows_per_step - 1) / p.rows_per_step, most = (int64_t)sm_count() * p.per_sm;
     return want < most ? want : most;
 }
 
+template <int DT, int TPR, int CH, bool COMP> static int launch_ln_bwd_ring_kernel(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
+    auto* k = layer_norm_backward_ring_kernel<DT, TPR, CH, COMP>;
+    constexpr int W = TPR * CH * 8, E = Elem<DT>::kBytes, kSmem = W * (int)sizeof(float) + kRingStages * W * (E + (COMP ? 1 : E));
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return GACT_ERR_LAUNCH;
+    k<<<(unsigned)blocks, TPR, kSmem, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+template <int DT, int TPR, int CH> static int launch_ln_bwd_ring(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
+    return a.codes ? launch_ln_bwd_ring_kernel<DT, TPR, CH, true>(a, blocks, s) : launch_ln_bwd_ring_kernel<DT, TPR, CH, false>(a, blocks, s);
+}
 template <int DT, int TPR, int CH, int R> static int launch_ln_bwd(const LnBwdArgs& a, bool vec, int64_t blocks, cudaStream_t s) {
     const int block = TPR > 32 ? TPR : 128;
     if (a.codes) {
@@ -391,6 +615,11 @@ template <int DT, int TPR, int CH, int R> static int launch_ln_bwd(const LnBwdAr
 }
 template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, int64_t blocks, cudaStream_t s) {
     const int h = a.cols;
+    if (ln_bwd_shape(vec, a.rows, h).ring) {
+        if (h <= 2048) return launch_ln_bwd_ring<DT, 128, 2>(a, blocks, s);
+        if (h <= 4096) return launch_ln_bwd_ring<DT, 128, 4>(a, blocks, s);
+        return launch_ln_bwd_ring<DT, 512, 2>(a, blocks, s);
+    }
     if (h <= 32) return launch_ln_bwd<DT, 4, 1, kLnBwdRows>(a, vec, blocks, s);
     if (h <= 64) return launch_ln_bwd<DT, 8, 1, kLnBwdRows>(a, vec, blocks, s);
     if (h <= 128) return launch_ln_bwd<DT, 16, 1, kLnBwdRows>(a, vec, blocks, s);
@@ -404,7 +633,7 @@ template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, int64
 }
 
 // ---- sums of partials over the blocks that wrote them ---------------------------------------------------------------
-constexpr int kRCols = 32, kRRows = 16;
+constexpr int kRCols = 32, kRRows = 32;
 struct ReduceArgs { const float* partial; int parts; int64_t width; void* out0; int64_t n0; void* out1; int64_t n1; };
 
 template <int DT>
@@ -413,8 +642,24 @@ __global__ void __launch_bounds__(kRCols * kRRows) reduce_columns_kernel(const R
     const int tx = threadIdx.x % kRCols, ty = threadIdx.x / kRCols;
     const int64_t c = (int64_t)blockIdx.x * kRCols + tx;
     float sum = 0.0f;
-    if (c < a.width)
-        for (int p = ty; p < a.parts; p += kRRows) sum += a.partial[(int64_t)p * a.width + c];
+    if (c < a.width) {
+        const float* q = a.partial + (int64_t)ty * a.width + c;
+        const int64_t step = (int64_t)kRRows * a.width;
+        int p = ty;
+        // eight loads in flight per thread: the partials are few and the kernel is all latency
+        for (; p + 7 * kRRows < a.parts; p += 8 * kRRows, q += 8 * step) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = q[i * step];
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += v[i];
+        }
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = p + i * kRRows < a.parts ? q[i * step] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += v[i];
+    }
     buf[ty][tx] = sum;
     __syncthreads();
     if (ty == 0 && c < a.width) {
@@ -442,6 +687,15 @@ int reduce_columns(const float* partial, int parts, int64_t width, void* out0, i
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 
+int norm_error_word() {
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_norm_error, sizeof(int)) == cudaSuccess ? v : -1;
+}
+int norm_error_clear() {
+    const int zero = 0;
+    return cudaMemcpyToSymbol(g_norm_error, &zero, sizeof(int)) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+}
+
 static bool ln_sizes_ok(int64_t rows, int64_t cols) {
     return rows >= 0 && cols >= 1 && cols <= GACT_LAYER_NORM_MAX_COLS && rows <= GACT_MAX_ELEMENTS / pitch8(cols) && rows <= (1LL << 30);
 }
@@ -452,22 +706,22 @@ static bool param_ok(const void* p, int dtype) { return !p || ((uintptr_t)p & (u
 using namespace gact;
 
 extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight, const void* bias,
-                               int param_dtype, double eps, void* y, float* mean, float* rstd, void* codes, void* scales, int stochastic,
+                               int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int stochastic,
                                uint64_t seed, void* stream) {
     if (dtype < GACT_F32 || dtype > GACT_BF16 || (param_dtype != dtype && param_dtype != GACT_F32)) return GACT_ERR_DTYPE;
     if (!ln_sizes_ok(rows, cols) || ld < cols) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
-    if (!x || !y || (codes && !scales) || (!mean != !rstd)) return GACT_ERR_NULL;
+    if (!x || !y || (codes && !scales)) return GACT_ERR_NULL;
     const uintptr_t em = (uintptr_t)(elem_bytes_of(dtype) - 1);
-    if (((uintptr_t)x & em) || ((uintptr_t)y & em) || ((uintptr_t)codes & 31) || !param_ok(weight, param_dtype) || !param_ok(bias, param_dtype))
+    if (((uintptr_t)x & em) || ((uintptr_t)y & em) || ((uintptr_t)codes & 31) || ((uintptr_t)stats & 7) || !param_ok(weight, param_dtype) ||
+        !param_ok(bias, param_dtype))
         return GACT_ERR_ALIGN;
     LnArgs a;
     a.x = x; a.ldx = ld; a.w = weight; a.b = bias; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.eps = (float)eps;
-    a.y = y; a.mean = mean; a.rstd = rstd; a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales;
+    a.y = y; a.stats = stats; a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales;
     a.chunks = (int)(pitch8(cols) / 8); a.stochastic = stochastic; a.rk = philox_round_keys(seed);
-    const bool vec = rows_aligned(x, ld, cols, elem_bytes_of(dtype)) && rows_aligned(y, cols, cols, elem_bytes_of(dtype)) &&
-                     (((uintptr_t)weight | (uintptr_t)bias) & 15) == 0;
+    const bool vec = rows_aligned(x, ld, cols, elem_bytes_of(dtype)) && rows_aligned(y, cols, cols, elem_bytes_of(dtype));
     cudaStream_t s = (cudaStream_t)stream;
     switch (dtype) {
     case GACT_F32: return dispatch_ln<GACT_F32>(a, vec, s);
@@ -478,11 +732,13 @@ extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t c
 
 extern "C" int64_t gact_layer_norm_backward_scratch_bytes(int64_t rows, int64_t cols) {
     if (!ln_sizes_ok(rows, cols)) return -1;
-    return ln_bwd_blocks(rows, cols) * 2 * ((cols + 7) / 8 * 8) * (int64_t)sizeof(float);
+    // (whichever kernel the operands' alignment picks)
+    const int64_t a = ln_bwd_blocks(true, rows, cols), b = ln_bwd_blocks(false, rows, cols);
+    return (a > b ? a : b) * 2 * ((cols + 7) / 8 * 8) * (int64_t)sizeof(float);
 }
 
 extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, const void* x, int64_t ld_x,
-                                        const void* codes, const void* scales, const float* mean, const float* rstd, const void* weight,
+                                        const void* codes, const void* scales, const float* stats, const void* weight,
                                         int param_dtype, void* dx, void* dweight, void* dbias, void* scratch, void* stream) {
     if (dtype < GACT_F32 || dtype > GACT_BF16 || (param_dtype != dtype && param_dtype != GACT_F32)) return GACT_ERR_DTYPE;
     if (!ln_sizes_ok(rows, cols) || ld_dy < cols || (x && ld_x < cols)) return GACT_ERR_SIZE;
@@ -495,21 +751,20 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
         if (dbias && cudaMemsetAsync(dbias, 0, bytes, s) != cudaSuccess) return GACT_ERR_LAUNCH;
         return GACT_OK;
     }
-    if (!dy || !mean || !rstd || (!x && (!codes || !scales)) || (params && !scratch)) return GACT_ERR_NULL;
+    if (!dy || !stats || (!x && (!codes || !scales)) || (params && !scratch)) return GACT_ERR_NULL;
     if (!dx && !params) return GACT_OK;
     const uintptr_t em = (uintptr_t)(elem_bytes_of(dtype) - 1);
-    if (((uintptr_t)dy & em) || ((uintptr_t)x & em) || ((uintptr_t)dx & em) || ((uintptr_t)codes & 31) || ((uintptr_t)scratch & 15) ||
+    if (((uintptr_t)dy & em) || ((uintptr_t)x & em) || ((uintptr_t)dx & em) || ((uintptr_t)codes & 31) || ((uintptr_t)scratch & 15) || ((uintptr_t)stats & 7) ||
         !param_ok(weight, param_dtype) || !param_ok(dweight, param_dtype) || !param_ok(dbias, param_dtype))
         return GACT_ERR_ALIGN;
     LnBwdArgs a;
     a.dy = dy; a.ldy = ld_dy; a.x = x; a.ldx = ld_x; a.codes = x ? nullptr : (const int8_t*)codes; a.scales = (const uint8_t*)scales;
-    a.chunks = (int)(pitch8(cols) / 8); a.mean = mean; a.rstd = rstd; a.w = weight; a.wf32 = param_dtype == GACT_F32;
+    a.chunks = (int)(pitch8(cols) / 8); a.stats = stats; a.w = weight; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.dx = dx;
     a.partial = params ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
     const int eb = elem_bytes_of(dtype);
-    const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb)) &&
-                     ((uintptr_t)weight & 15) == 0;
-    const int64_t blocks = ln_bwd_blocks(rows, cols);
+    const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb));
+    const int64_t blocks = ln_bwd_blocks(vec, rows, cols);
     int st;
     switch (dtype) {
     case GACT_F32: st = dispatch_ln_bwd<GACT_F32>(a, vec, blocks, s); break;

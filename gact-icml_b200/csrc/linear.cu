@@ -107,15 +107,21 @@ template <int ACT> __device__ __forceinline__ float2 act_slope2(float2 z) {
     return splat2(1.0f);
 }
 
-// ---- epilogue of 32 consecutive columns of one row -------------------------------------------------------------------
+// ---- epilogue of 32 rows x 32 columns: a lane holds one row --------------------------------------------------------------
+// Rows on 16-byte boundaries are written and read by their own lane, 32 or 16 bytes at a time.  Other rows (and the ragged
+// last columns) go through shared memory, where the tile is turned around: lane l takes column l of one row after the other,
+// so that an access covers 64 contiguous bytes instead of 2 bytes of 32 rows (`stage`: 32 x 17 words of the warp).
+constexpr int kStageWords = 32 * 17;
+
 template <int DT>
-__device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, const float2 (&v)[16]) {
+__device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t row, int64_t M, int64_t n, int64_t N, const float2 (&v)[16], uint32_t* stage) {
     using T = typename Elem<DT>::T;
-    T* p = (T*)base + row * ld + n;
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) w[i] = pack2<DT>(v[i].x, v[i].y);
     if (n + 32 <= N && vec >= 16) {
+        if (row >= M) return;
+        T* p = (T*)base + row * ld + n;
         if (vec == 32) {
             const uint32_t a[8] = {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, b[8] = {w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]};
             st_v8(p, a);
@@ -125,31 +131,49 @@ __device__ __forceinline__ void store32(void* base, int64_t ld, int vec, int64_t
             for (int i = 0; i < 4; i++) *(uint4*)(p + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
     } else {
+        const int lane = threadIdx.x & 31;
+        const int64_t row0 = row - lane;
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (n + j < N) ((uint16_t*)p)[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+        for (int i = 0; i < 16; i++) stage[lane * 17 + i] = w[i];
+        __syncwarp();
+        uint16_t* p = (uint16_t*)base + row0 * ld + n + lane;
+        const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
+        if (n + lane < N)
+            for (int r = 0; r < rows; r++, p += ld) *p = ((const uint16_t*)(stage + r * 17))[lane];
     }
 }
 template <int DT>
-__device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int64_t row, int64_t n, int64_t N, float2 (&v)[16]) {
+__device__ __forceinline__ void add32(const void* base, int64_t ld, int vec, int64_t row, int64_t M, int64_t n, int64_t N, float2 (&v)[16], uint32_t* stage) {
     using T = typename Elem<DT>::T;
-    const T* p = (const T*)base + row * ld + n;
+    uint32_t w[16];
     if (n + 32 <= N && vec >= 16) {
+        if (row >= M) return;
+        const T* p = (const T*)base + row * ld + n;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint4 u = __ldg((const uint4*)(p + 8 * i));
-            const uint32_t raw[4] = {u.x, u.y, u.z, u.w};
-            float2 f[4];
-            raw_to_pairs<DT>(raw, f);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[4 * i + j] = add2(v[4 * i + j], f[j]);
+            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
         }
     } else {
+        const int lane = threadIdx.x & 31;
+        const int64_t row0 = row - lane;
+        const uint16_t* p = (const uint16_t*)base + row0 * ld + n + lane;
+        const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
+        __syncwarp();
+#pragma unroll 8
+        for (int r = 0; r < 32; r++, p += ld) ((uint16_t*)(stage + r * 17))[lane] = (n + lane < N && r < rows) ? __ldg(p) : (uint16_t)0;
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            if (n + 2 * i < N) v[i].x += Elem<DT>::to_float(p[2 * i]);
-            if (n + 2 * i + 1 < N) v[i].y += Elem<DT>::to_float(p[2 * i + 1]);
-        }
+        for (int i = 0; i < 16; i++) w[i] = stage[lane * 17 + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t raw[4] = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        float2 f[4];
+        raw_to_pairs<DT>(raw, f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[4 * i + j] = add2(v[4 * i + j], f[j]);
     }
 }
 template <int ACT> __device__ __forceinline__ void activate32(float2 (&v)[16]) {
@@ -157,10 +181,10 @@ template <int ACT> __device__ __forceinline__ void activate32(float2 (&v)[16]) {
     for (int i = 0; i < 16; i++) v[i] = act_value2<ACT>(v[i]);
 }
 
-// z = v + bias -> checkpoint of z, y = act(z) + residual -> out.  Called by threads that own (row, n .. n+31);
+// z = v + bias -> checkpoint of z, y = act(z) + residual -> out.  Called by whole warps (rows past M store nothing);
 // `bias`: the 32 biases as fp32 in shared memory (zeros past N or without one).
 template <int DT>
-__device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row, int64_t n, const float* bias, float2 (&v)[16]) {
+__device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row, int64_t n, const float* bias, float2 (&v)[16], uint32_t* stage) {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
         const float4 b = *(const float4*)(bias + 2 * i);
@@ -202,10 +226,12 @@ __device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row
 #pragma unroll
             for (int i = 0; i < 8; i++) w[i] = byte == 255u ? 0u : clamp_codes63(w[i]);
         }
-        st_v8(a.zcodes + at, w);
-        a.zscales[at >> 5] = (uint8_t)byte;
+        if (row < a.M) {
+            st_v8(a.zcodes + at, w);
+            a.zscales[at >> 5] = (uint8_t)byte;
+        }
     }
-    if (a.z) store32<DT>(a.z, a.N, a.zvec, row, n, a.N, v);
+    if (a.z) store32<DT>(a.z, a.N, a.zvec, row, a.M, n, a.N, v, stage);
     switch (a.act) {
     case GACT_ACT_RELU: activate32<GACT_ACT_RELU>(v); break;
     case GACT_ACT_GELU: activate32<GACT_ACT_GELU>(v); break;
@@ -213,8 +239,8 @@ __device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row
     case GACT_ACT_SILU: activate32<GACT_ACT_SILU>(v); break;
     default: break;
     }
-    if (a.res) add32<DT>(a.res, a.ldr, a.rvec, row, n, a.N, v);
-    store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
+    if (a.res) add32<DT>(a.res, a.ldr, a.rvec, row, a.M, n, a.N, v, stage);
+    store32<DT>(a.out, a.ldo, a.ovec, row, a.M, n, a.N, v, stage);
 }
 template <int DT> __device__ __forceinline__ float bias_at(const GemmArgs& a, int64_t n) {
     return a.bias && n < a.N ? Elem<DT>::to_float(((const typename Elem<DT>::T*)a.bias)[n]) : 0.0f;
@@ -264,6 +290,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const uint32_t full = smem_addr(bars), empty = full + 8 * S, acc_full = empty + 8 * S, acc_empty = acc_full + 16, drain = acc_empty + 16;
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float bias[2][EPI == kEpiLinear ? BN : 4];
+    __shared__ uint32_t stage[EPI == kEpiPartial ? 1 : kEpiWarps][EPI == kEpiPartial ? 1 : kStageWords];
     __shared__ volatile int dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 1 ? 0u : cluster_rank();
@@ -380,23 +407,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (col >= a.N) break;
                 uint32_t r[32];
                 tmem_load32(tmem + ((uint32_t)(q * 32) << 16) + acc * BN + half * kSpan + c, r);
-                if (row < a.M) {
-                    if constexpr (EPI == kEpiPartial) {
+                if constexpr (EPI == kEpiPartial) {
+                    if (row < a.M) {
                         float* p = a.partial + ((int64_t)x.split * a.M + row) * a.ldp + col;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint32_t w[8] = {r[8 * i], r[8 * i + 1], r[8 * i + 2], r[8 * i + 3], r[8 * i + 4], r[8 * i + 5], r[8 * i + 6], r[8 * i + 7]};
                             st_v8(p + 8 * i, w);
                         }
-                    } else {
-                        float2 v[16];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                        if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, col, bias[acc] + half * kSpan + c, v);
-                        else store32<DT>(a.out, a.ldo, a.ovec, row, col, a.N, v);
                     }
+                    __syncwarp();
+                } else {
+                    float2 v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, col, bias[acc] + half * kSpan + c, v, stage[warp - 4]);
+                    else store32<DT>(a.out, a.ldo, a.ovec, row, a.M, col, a.N, v, stage[warp - 4]);
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             tc_fence_before();
             if (lane == 0) {
@@ -418,17 +446,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 template <int DT, int EPI>
 __global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ GemmArgs a) {
     __shared__ __align__(16) float bias[32];
+    __shared__ uint32_t stage[4][kStageWords];
     const int64_t n = (int64_t)blockIdx.y * 32;
     if constexpr (EPI == kEpiLinear) {
         if (threadIdx.x < 32) bias[threadIdx.x] = bias_at<DT>(a, n + threadIdx.x);
         __syncthreads();
     }
     const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (row >= a.M) return;
     float2 v[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = splat2(0.0f);
-    for (int s = 0; s < a.splits; s++) {
+    for (int s = 0; s < a.splits && row < a.M; s++) {
         const float4* p = (const float4*)(a.partial + ((int64_t)s * a.M + row) * a.ldp + n);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -437,8 +465,8 @@ __global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ 
             v[2 * j + 1] = add2(v[2 * j + 1], make_float2(f.z, f.w));
         }
     }
-    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, bias, v);
-    else store32<DT>(a.out, a.ldo, a.ovec, row, n, a.N, v);
+    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, bias, v, stage[threadIdx.x >> 5]);
+    else store32<DT>(a.out, a.ldo, a.ovec, row, a.M, n, a.N, v, stage[threadIdx.x >> 5]);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -554,14 +582,15 @@ struct ActBwdArgs {
 };
 constexpr int kAWarps = 8;
 
-// A warp owns 256 columns (8 per lane) and walks rows; eight warps of a block take eight rows at a time, and the next rows'
-// loads are issued before the current ones are worked on.
+// A warp owns 256 columns (8 per lane) and walks rows, kARows of them side by side; a block takes eight such sets at a time.
+// The next rows' loads are issued before the current ones are worked on.
+constexpr int kARows = 2;
 template <int DT, bool VEC, bool COMP, int ACT>
 __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid_constant__ ActBwdArgs a) {
     using T = typename Elem<DT>::T;
     using Row = Row8<DT, VEC, 32>;
     constexpr bool kAct = ACT != GACT_ACT_NONE;
-    constexpr int U = 2;
+    constexpr int U = kARows;
     __shared__ float fold[kAWarps][8][33];
     __shared__ __align__(16) uint8_t staging[VEC ? 16 : kAWarps * Stage8<DT, VEC>::kBytes];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -585,7 +614,7 @@ __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid
                 if (row < a.rows && col < a.cols) {
                     const int64_t chunk = row * a.chunks + (col >> 3);
                     pq[u] = ld_stream_u2(a.codes + chunk * 8);
-                    pe[u] = a.scales[chunk >> 2];
+                    pe[u] = __ldg(a.scales + (chunk >> 2));
                 }
             } else if constexpr (kAct) {
                 pz[u].load((const T*)a.z, a.ldz, row, a.rows, col, a.cols);
@@ -595,32 +624,34 @@ __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid
     int64_t r = (int64_t)blockIdx.y * kAWarps + warp;
     fetch(r);
     for (; r < a.rows; r += U * step) {
-        float2 g[U][4], z[U][4];
+        uint32_t rawy[U][RawRegs<DT>::N], rawz[U][RawRegs<DT>::N];
+        uint2 q[U];
+        float down[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            uint32_t raw[RawRegs<DT>::N];
-            py[u].get(stage, raw);
-            raw_to_pairs<DT>(raw, g[u]);
+            py[u].get(stage, rawy[u]);
             if constexpr (kAct && COMP) {
-                restore_pairs(pq[u], scale_down8(pe[u]), z[u]);
+                q[u] = pq[u];
+                down[u] = scale_down8(pe[u]);
             } else if constexpr (kAct) {
-                pz[u].get(stage, raw);
-                raw_to_pairs<DT>(raw, z[u]);
+                pz[u].get(stage, rawz[u]);
             }
         }
         fetch(r + U * step);
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            float2 g[4], z[4];
+            raw_to_pairs<DT>(rawy[u], g);
             if constexpr (kAct) {
+                if constexpr (COMP) restore_pairs(q[u], down[u], z);
+                else raw_to_pairs<DT>(rawz[u], z);
 #pragma unroll
-                for (int i = 0; i < 4; i++) g[u][i] = mul2(g[u][i], act_slope2<ACT>(z[u][i]));
-                Row::store((T*)a.dz, a.ldo, r + u * step, a.rows, col, a.cols, stage, g[u]);
+                for (int i = 0; i < 4; i++) g[i] = mul2(g[i], act_slope2<ACT>(z[i]));
+                Row::store((T*)a.dz, a.ldo, r + u * step, a.rows, col, a.cols, stage, g);
             }
+            // (the sum takes the products before they are rounded; rows past the end have dy = 0 and a finite slope)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // rows past the end: dy = 0 and z = 0, the slope is finite, nothing is added
-                db[i] = add2(db[i], g[u][i]);
-            }
+            for (int i = 0; i < 4; i++) db[i] = add2(db[i], g[i]);
         }
     }
     if (!a.partial) return;
@@ -770,7 +801,8 @@ extern "C" int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_
     a.dy = dy; a.ldy = ld_dy; a.z = z; a.ldz = ld_z; a.codes = z ? nullptr : (const int8_t*)zcodes; a.scales = (const uint8_t*)zscales;
     a.chunks = (int)(pitch8(cols) / 8); a.act = act; a.rows = rows; a.cols = (int)cols; a.dz = dz; a.ldo = ld_dz;
     a.partial = dbias ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
-    const bool vec = rows_aligned(dy, ld_dy, cols, 2) && (act == GACT_ACT_NONE || ((!z || rows_aligned(z, ld_z, cols, 2)) && rows_aligned(dz, ld_dz, cols, 2)));
+    const bool vec = rows_aligned(dy, ld_dy, cols, 2) &&
+                     (act == GACT_ACT_NONE || ((!z || rows_aligned(z, ld_z, cols, 2)) && rows_aligned(dz, ld_dz, cols, 2)));
     const int64_t parts = act_bwd_parts(rows, cols);
     const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)parts);
     if (dtype == GACT_F16) dispatch_act_bwd<GACT_F16>(a, vec, grid, s);

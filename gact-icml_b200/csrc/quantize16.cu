@@ -720,9 +720,11 @@ int launch_quantize16(const QuantArgs& a, int dtype, int bits, int rng, cudaStre
     return dtype == GACT_F16 ? dispatch_bits16<GACT_F16>(a, bits, rng, s) : dispatch_bits16<GACT_BF16>(a, bits, rng, s);
 }
 
-// the error word of the linear layers' pipeline (linear.cu)
+// the error words of the linear layers' pipeline (linear.cu) and of layer norm's rings (layernorm.cu)
 int linear_error_word();
 int linear_error_clear();
+int norm_error_word();
+int norm_error_clear();
 
 }  // namespace gact
 
@@ -731,11 +733,13 @@ using namespace gact;
 extern "C" int gact_pipeline_error(void) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_pipeline_error, sizeof(int)) != cudaSuccess) return -1;
-    return v ? v : linear_error_word();
+    if (v == 0) v = linear_error_word();
+    return v ? v : norm_error_word();
 }
 
 extern "C" int gact_pipeline_error_reset(void) {
     const int zero = 0;
     if (cudaMemcpyToSymbol(g_pipeline_error, &zero, sizeof(int)) != cudaSuccess) return GACT_ERR_LAUNCH;
-    return linear_error_clear();
+    const int a = linear_error_clear(), b = norm_error_clear();
+    return a != GACT_OK ? a : b;
 }

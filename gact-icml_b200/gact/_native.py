@@ -53,9 +53,9 @@ _SIGNATURES = {
     "gact_checkpoint8": ([_vp, _i, _i64, _i64, _i64, _i, _u64, _vp, _vp, _vp], _i),
     "gact_restore8": ([_vp, _vp, _i64, _i64, _i, _vp, _i64, _vp], _i),
     "gact_repitch16": ([_vp, _i64, _i64, _i64, _vp, _i64, _vp], _i),
-    "gact_layer_norm": ([_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _d, _vp, _vp, _vp, _vp, _vp, _i, _u64, _vp], _i),
+    "gact_layer_norm": ([_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _d, _vp, _vp, _vp, _vp, _i, _u64, _vp], _i),
     "gact_layer_norm_backward_scratch_bytes": ([_i64, _i64], _i64),
-    "gact_layer_norm_backward": ([_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
+    "gact_layer_norm_backward": ([_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
     "gact_linear_scratch_bytes": ([_i64, _i64, _i64, _i], _i64),
     "gact_linear": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _i, _u64, _vp, _vp], _i),
     "gact_linear_dgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp], _i),

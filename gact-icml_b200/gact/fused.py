@@ -61,7 +61,7 @@ def op_restore8(c, dtype=None):
 # ---------------------------------------------------------------------------------------------------------------
 class LayerNormSaved:
     """What layer norm's backward pass needs: the input (a Checkpoint8, or the tensor itself), the row statistics
-    (mean and 1 / deviation, fp32 (2, rows)) and the weight."""
+    (mean and 1 / deviation, fp32 (rows, 2)) and the weight."""
     __slots__ = ("x", "stats", "weight", "shape", "dtype", "param_dtype")
 
     def __init__(self, x, stats, weight, shape, dtype, param_dtype):

@@ -265,20 +265,20 @@ int gact_repitch16(const void* src, int64_t ld, int64_t rows, int64_t cols, void
 
 /*
  * Layer norm over rows of `cols`: y = (x - mean) / sqrt(var + eps) * weight + bias; weight / bias may be null, their type
- * is `param_dtype` (that of x, or GACT_F32).  y is contiguous.  mean / rstd (both or neither): fp32 per row, for the
- * backward pass.  codes / scales (optional): checkpoint of x, made in the same pass.
+ * is `param_dtype` (that of x, or GACT_F32).  y is contiguous.  stats (optional, 8-byte aligned): (mean, 1 / deviation)
+ * per row in fp32, for the backward pass.  codes / scales (optional): checkpoint of x, made in the same pass.
  */
 int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight, const void* bias,
-                    int param_dtype, double eps, void* y, float* mean, float* rstd, void* codes, void* scales, int stochastic,
-                    uint64_t seed, void* stream);
+                    int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int stochastic, uint64_t seed,
+                    void* stream);
 /*
  * Its backward pass from x, or (x null) from the checkpoint of x.  dx (contiguous), dweight, dbias: each may be null.
  * Sums over rows are added in a fixed order (no atomics).  scratch: only with dweight or dbias.
  */
 int64_t gact_layer_norm_backward_scratch_bytes(int64_t rows, int64_t cols);
 int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, const void* x, int64_t ld_x,
-                             const void* codes, const void* scales, const float* mean, const float* rstd, const void* weight,
-                             int param_dtype, void* dx, void* dweight, void* dbias, void* scratch, void* stream);
+                             const void* codes, const void* scales, const float* stats, const void* weight, int param_dtype,
+                             void* dx, void* dweight, void* dbias, void* scratch, void* stream);
 
 /*
  * y = act(x W^T + bias) + residual for fp16 / bf16, fp32 accumulation; weight is [cout][cin].  x and weight: base and row

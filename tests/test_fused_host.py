@@ -37,18 +37,18 @@ def test_layer_norm_abi_refusals():
     from gact import _native as nv
     L = nv.lib
     b, p = buf()
-    f = lambda x=p, dt=2, rows=2, cols=32, ld=32, w=p, bias=p, pdt=2, y=p, mean=p, rstd=p, codes=p, scales=p: L.gact_layer_norm(
-        x, dt, rows, cols, ld, w, bias, pdt, 1e-5, y, mean, rstd, codes, scales, 0, 0, None)
+    f = lambda x=p, dt=2, rows=2, cols=32, ld=32, w=p, bias=p, pdt=2, y=p, stats=p, codes=p, scales=p: L.gact_layer_norm(
+        x, dt, rows, cols, ld, w, bias, pdt, 1e-5, y, stats, codes, scales, 0, 0, None)
     assert f(dt=4) == 2 and f(pdt=1) == 2 and f(dt=0, pdt=2) == 2
     assert f(rows=-1) == 5 and f(cols=0) == 5 and f(cols=16385, ld=16385) == 5 and f(ld=31) == 5
-    assert f(x=None) == 3 and f(y=None) == 3 and f(scales=None) == 3 and f(mean=None) == 3
-    assert f(x=p + 1) == 4 and f(y=p + 1) == 4 and f(codes=p + 16) == 4 and f(w=p + 1) == 4 and f(bias=p + 2, pdt=0) == 4
+    assert f(x=None) == 3 and f(y=None) == 3 and f(scales=None) == 3
+    assert f(x=p + 1) == 4 and f(y=p + 1) == 4 and f(codes=p + 16) == 4 and f(stats=p + 4) == 4 and f(w=p + 1) == 4 and f(bias=p + 2, pdt=0) == 4
     assert f(rows=0, x=None) == 0
     assert L.gact_layer_norm_backward_scratch_bytes(-1, 32) == -1 and L.gact_layer_norm_backward_scratch_bytes(1, 20000) == -1
-    g = lambda dy=p, dt=2, rows=2, cols=32, ld=32, x=None, ldx=32, codes=p, scales=p, mean=p, rstd=p, w=p, pdt=2, dx=p, dw=p, db=p, scr=p: \
-        L.gact_layer_norm_backward(dy, dt, rows, cols, ld, x, ldx, codes, scales, mean, rstd, w, pdt, dx, dw, db, scr, None)
+    g = lambda dy=p, dt=2, rows=2, cols=32, ld=32, x=None, ldx=32, codes=p, scales=p, stats=p, w=p, pdt=2, dx=p, dw=p, db=p, scr=p: \
+        L.gact_layer_norm_backward(dy, dt, rows, cols, ld, x, ldx, codes, scales, stats, w, pdt, dx, dw, db, scr, None)
     assert g(dt=7) == 2 and g(cols=0) == 5 and g(ld=8) == 5 and g(x=p, ldx=8) == 5
-    assert g(dy=None) == 3 and g(codes=None) == 3 and g(scales=None) == 3 and g(mean=None) == 3 and g(scr=None) == 3
+    assert g(dy=None) == 3 and g(codes=None) == 3 and g(scales=None) == 3 and g(stats=None) == 3 and g(scr=None) == 3
     assert g(dy=p + 1) == 4 and g(codes=p + 8) == 4 and g(scr=p + 4) == 4 and g(dx=p + 1) == 4
     assert g(dx=None, dw=None, db=None) == 0
 
