@@ -67,6 +67,29 @@ static __device__ __noinline__ uint32_t clamp_codes63(uint32_t w) {
     return out;
 }
 
+// Loads that are issued a step ahead of their use.  As volatile statements they stay where they are written; plain loads were
+// moved down to their first use, where every step waited for them.
+__device__ __forceinline__ uint32_t ld_ahead_byte(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float2 ld_ahead_float2(const float2* p) {
+    float2 v;
+    asm volatile("ld.global.nc.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_ahead_u16(const uint16_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_ahead_u32(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // ---- eight consecutive elements of a row, as four pairs (two fp32 operations per instruction) -----------------------
 template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (DT == GACT_F16) {
@@ -192,7 +215,11 @@ template <int DT, bool VEC, int SUB> struct Row8 {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int e = i * 32 + lane, g = e / (SUB * 8), c = col0 + e % (SUB * 8);
-                r[i] = (row0 + g < rows && c < cols) ? (uint32_t)__ldg((const U*)base + (row0 + g) * ld + c) : 0u;
+                r[i] = 0u;
+                if (row0 + g < rows && c < cols) {
+                    if constexpr (DT == GACT_F32) r[i] = ld_ahead_u32((const uint32_t*)base + (row0 + g) * ld + c);
+                    else r[i] = ld_ahead_u16((const uint16_t*)base + (row0 + g) * ld + c);
+                }
             }
         }
     }

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
         for (int k = 0; k < R; k++) {
             const int64_t row = base + k * GROUPS + grp;
             const bool live = row < a.rows;
-            ps[k] = live ? __ldg((const float2*)a.stats + row) : make_float2(0.0f, 0.0f);
+            ps[k] = live ? ld_ahead_float2((const float2*)a.stats + row) : make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 py[k][c].load((const T*)a.dy, a.ldy, row, a.rows, (t + c * TPR) * 8, a.cols);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128, 512 / (TPR > 128 ? TPR 
                     if (live && t + c * TPR < a.chunks) {
                         const int64_t chunk = row * a.chunks + (t + c * TPR);
                         pq[k][c] = ld_stream_u2(a.codes + chunk * 8);
-                        pe[k][c] = a.scales[chunk >> 2];
+                        pe[k][c] = ld_ahead_byte(a.scales + (chunk >> 2));
                     }
                 } else {
                     px[k][c].load((const T*)a.x, a.ldx, row, a.rows, (t + c * TPR) * 8, a.cols);
@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
     uint32_t pe[CH];
     auto fetch = [&](int64_t w) {
         if (w < a.rows) {
-            ps = __ldg((const float2*)a.stats + w);
+            ps = ld_ahead_float2((const float2*)a.stats + w);
             if (COMP) {
                 const uint8_t* p = a.scales + ((w * a.chunks + t) >> 2);
 #pragma unroll
                 for (int c = 0; c < CH; c++)
-                    if (t + c * TPR < a.chunks) pe[c] = __ldg(p + c * (TPR / 4));
+                    if (t + c * TPR < a.chunks) pe[c] = ld_ahead_byte(p + c * (TPR / 4));
             }
         }
     };

@@ -443,15 +443,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 
 // Adds the partial sums of the splits in order and runs the epilogue: one thread per 32 columns of a row, 128 rows and the
 // same 32 columns per block.
-template <int DT, int EPI>
-__global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ GemmArgs a) {
+template <int DT>
+__global__ void __launch_bounds__(128) gemm_join_linear_kernel(const __grid_constant__ GemmArgs a) {
     __shared__ __align__(16) float bias[32];
     __shared__ uint32_t stage[4][kStageWords];
     const int64_t n = (int64_t)blockIdx.y * 32;
-    if constexpr (EPI == kEpiLinear) {
-        if (threadIdx.x < 32) bias[threadIdx.x] = bias_at<DT>(a, n + threadIdx.x);
-        __syncthreads();
-    }
+    if (threadIdx.x < 32) bias[threadIdx.x] = bias_at<DT>(a, n + threadIdx.x);
+    __syncthreads();
     const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
     float2 v[16];
 #pragma unroll
@@ -465,8 +463,35 @@ __global__ void __launch_bounds__(128) gemm_join_kernel(const __grid_constant__ 
             v[2 * j + 1] = add2(v[2 * j + 1], make_float2(f.z, f.w));
         }
     }
-    if constexpr (EPI == kEpiLinear) linear_epilogue32<DT>(a, row, n, bias, v, stage[threadIdx.x >> 5]);
-    else store32<DT>(a.out, a.ldo, a.ovec, row, a.M, n, a.N, v, stage[threadIdx.x >> 5]);
+    linear_epilogue32<DT>(a, row, n, bias, v, stage[threadIdx.x >> 5]);
+}
+
+// The same without an epilogue: one thread per 8 columns, neighbours side by side.
+template <int DT>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const __grid_constant__ GemmArgs a) {
+    using T = typename Elem<DT>::T;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.M * (a.ldp / 8)) return;
+    const int64_t row = i / (a.ldp / 8), n = (i - row * (a.ldp / 8)) * 8;
+    if (n >= a.N) return;
+    float2 v[4] = {splat2(0.0f), splat2(0.0f), splat2(0.0f), splat2(0.0f)};
+    const float* p = a.partial + row * a.ldp + n;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; s++, p += a.M * a.ldp) {
+        const float4 x = *(const float4*)p, y = *(const float4*)(p + 4);
+        v[0] = add2(v[0], make_float2(x.x, x.y));
+        v[1] = add2(v[1], make_float2(x.z, x.w));
+        v[2] = add2(v[2], make_float2(y.x, y.y));
+        v[3] = add2(v[3], make_float2(y.z, y.w));
+    }
+    T* out = (T*)a.out + row * a.ldo + n;
+    if (a.ovec >= 16 && n + 8 <= a.N) {
+        *(uint4*)out = make_uint4(pack2<DT>(v[0].x, v[0].y), pack2<DT>(v[1].x, v[1].y), pack2<DT>(v[2].x, v[2].y), pack2<DT>(v[3].x, v[3].y));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (n + j < a.N) out[j] = Elem<DT>::from_float(j & 1 ? v[j / 2].y : v[j / 2].x);
+    }
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -497,12 +522,13 @@ static bool make_map(CUtensorMap* m, int dtype, const void* p, int64_t rows, int
 
 struct Plan { int cg, bn, splits, per_split; int64_t tiles_m, tiles_n; };
 
-// Tile shape (two blocks on 256 x 256, one on 128 x 128 or 128 x 64) and splits of the reduction.  For each shape: rounds
-// of tiles over the SMs times the time of a tile, in nanoseconds as measured (a stage of 64 K-elements and the fixed part of
-// a tile), and the join of splits (a launch, and the partial sums written and read).  The cheapest wins.
+// Tile shape (two blocks on 256 x 256, one on 128 x 128 or 128 x 64) and splits of the reduction: the combination with the
+// least estimated time.  Measured on products of 16 to 8192 rows (nanoseconds): a launch with one stage takes `fixed`, every
+// further stage of a block `stage` (a stage moves 24 to 32 KB into an SM, which at these sizes is what takes the time), so the
+// busiest block's stages count; joining splits costs a second launch and the partial sums' way through L2.
 static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
-    struct Shape { int cg, bn; double stage, tile; };
-    static const Shape shapes[3] = {{2, 256, 300.0, 2500.0}, {1, 128, 190.0, 2200.0}, {1, 64, 130.0, 2000.0}};
+    struct Shape { int cg, bn; double fixed, stage; };
+    static const Shape shapes[3] = {{2, 256, 5600.0, 390.0}, {1, 128, 4400.0, 370.0}, {1, 64, 4100.0, 335.0}};
     const int sms = sm_count();
     const int64_t kt = (K + kBK - 1) / kBK;
     Plan best = {};
@@ -513,13 +539,13 @@ static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
         p.tiles_m = (M + kBM * h.cg - 1) / (kBM * h.cg);
         p.tiles_n = (N + h.bn - 1) / h.bn;
         const int64_t tiles = p.tiles_m * p.tiles_n, slots = sms / h.cg;
-        for (int64_t splits = 1; splits <= 16; splits *= 2) {
+        for (int64_t splits = 1; splits <= 16 && (splits == 1 || tiles * splits <= 4 * slots); splits++) {
             p.per_split = (int)((kt + splits - 1) / splits);
             p.splits = (int)((kt + p.per_split - 1) / p.per_split);
-            if (p.splits != splits || (splits > 1 && p.per_split < 4)) break;
+            if (p.splits != splits || (splits > 1 && p.per_split < 2)) continue;
             const int64_t rounds = (tiles * splits + slots - 1) / slots;
-            double t = 2000.0 + (double)rounds * (p.per_split * h.stage) + h.tile;
-            if (splits > 1) t += 2500.0 + (double)(splits + 1) * (double)M * (double)N * 4.0 / 4000.0;
+            double t = h.fixed + (double)(rounds * p.per_split - 1) * h.stage;
+            if (splits > 1) t += 2800.0 + (double)(splits * 2 + 1) * (double)M * (double)N * 4.0 / 8000.0;
             if (t < best_t) { best_t = t; best = p; }
         }
     }
@@ -568,7 +594,12 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
     a.ldp = pitch8(a.N);
     const int st = launch_gemm_shape<DT, A_MN, B_MN, kEpiPartial>(p, ma, mb, a, s);
     if (st != GACT_OK) return st;
-    gemm_join_kernel<DT, kEpi><<<dim3((unsigned)((a.M + 127) / 128), (unsigned)(a.ldp / 32)), 128, 0, s>>>(a);
+    if constexpr (LINEAR) {
+        gemm_join_linear_kernel<DT><<<dim3((unsigned)((a.M + 127) / 128), (unsigned)(a.ldp / 32)), 128, 0, s>>>(a);
+    } else {
+        const int64_t threads = a.M * (a.ldp / 8);
+        gemm_join_kernel<DT><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a);
+    }
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
 
@@ -614,7 +645,7 @@ __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid
                 if (row < a.rows && col < a.cols) {
                     const int64_t chunk = row * a.chunks + (col >> 3);
                     pq[u] = ld_stream_u2(a.codes + chunk * 8);
-                    pe[u] = __ldg(a.scales + (chunk >> 2));
+                    pe[u] = ld_ahead_byte(a.scales + (chunk >> 2));
                 }
             } else if constexpr (kAct) {
                 pz[u].load((const T*)a.z, a.ldz, row, a.rows, col, a.cols);
