@@ -270,6 +270,25 @@ template <int DT, bool VEC, int SUB> struct Row8 {
 // bytes of shared memory per warp that Row8 needs
 template <int DT, bool VEC> struct Stage8 { static constexpr int kBytes = VEC ? 0 : 256 * Elem<DT>::kBytes; };
 
+// Division by a number known at launch: for i < 2^31 one multiplication, i / d = i * mul >> (31 + s) with s = ceil(log2 d)
+// and mul = floor(2^(31+s) / d) + 1 < 2^32 (the excess mul * d - 2^(31+s) is at most d <= 2^s, so the error stays below 1 / d).
+// Larger indices take the 64-bit division (a hundred instructions, which would bound the kernel).
+struct Divisor {
+    uint32_t mul, shift; int64_t d;
+    static Divisor of(int64_t d) {
+        Divisor v;
+        int s = 0;
+        while ((1LL << s) < d) s++;
+        v.mul = (uint32_t)((1ULL << (31 + s)) / (uint64_t)d + 1);
+        v.shift = 31 + s;
+        v.d = d;
+        return v;
+    }
+    __device__ __forceinline__ int64_t div(int64_t i) const {
+        return i < (1LL << 31) ? (int64_t)(((uint64_t)(uint32_t)i * mul) >> shift) : i / d;
+    }
+};
+
 // Blocks of a kernel that one SM holds, asked of the runtime once per device.
 template <class K> static inline int resident_blocks(K kernel, int threads, size_t smem, std::atomic<int> (&cache)[kMaxDevices]) {
     int dev = 0;

@@ -345,12 +345,12 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (res.defined()) rr = as_rows(res);
     if (c.codes.defined()) check_codes(c, xr.rows, cin, &x);
     const Tensor y = at::empty(out_shape, x.options());
-    Codes zc;
+    Codes zc, xc;                                        // xc: the checkpoint of x that this call makes
     Tensor z;
     if (save) {
         if (act && compress) zc = empty_codes(xr.rows, cout, x);
         else if (act) z = at::empty({xr.rows, cout}, x.options());
-        if (compress && !c.codes.defined()) c = checkpoint8(x, seed);
+        if (compress && !c.codes.defined()) c = xc = empty_codes(xr.rows, cin, x);
     }
     if (xr.rows > 0) {
         void* s = stream_of(x);
@@ -358,9 +358,8 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         wr = as_operand(wr, cin, s);
         const int64_t bytes = gact_linear_scratch_bytes(xr.rows, cin, cout, 0);
         const Tensor scr = scratch(bytes, x);
-        // the codes of the pre-activation draw their noise from another key than those of the input
         check(gact_linear(xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, ptr(b), ptr(rr.t), rr.ld, type_code(x.scalar_type()), xr.rows, cin, cout, act,
-                          y.data_ptr(), ptr(z), ptr(zc.codes), ptr(zc.scales), seed.stochastic, seed.value + 0x9E3779B97F4A7C15ull, ptr(scr), s),
+                          y.data_ptr(), ptr(xc.codes), ptr(xc.scales), ptr(z), ptr(zc.codes), ptr(zc.scales), seed.stochastic, seed.value, ptr(scr), s),
               "gact_linear");
         g_launches += 1 + (bytes > 0);
     }
@@ -400,11 +399,13 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         return tuple_of({dx, dw, db});
     }
     void* s = stream_of(dy);
-    // one scratch buffer serves the three steps, which run one after the other on this stream
-    const int64_t ab = nb ? gact_act_backward_scratch_bytes(rows, cout) : 0, xb = nx ? gact_linear_scratch_bytes(rows, cin, cout, 1) : 0,
-                  wb = nw ? gact_linear_scratch_bytes(rows, cin, cout, 2) : 0;
-    const Tensor scr = scratch(std::max(ab, std::max(xb, wb)), dy);
-    if (nb || (act && (nx || nw))) {
+    const int64_t xb = nx ? gact_linear_scratch_bytes(rows, cin, cout, 1) : 0, wb = nw ? gact_linear_scratch_bytes(rows, cin, cout, 2) : 0;
+    const Tensor scr = scratch(std::max(xb, wb), dy);          // (the two products run one after the other on this stream)
+    const Tensor sums = scratch(nb ? gact_act_backward_scratch_bytes(rows, cout) : 0, dy);
+    // dz = dy act'(z) and the partial sums of the bias gradient; without an activation, dy itself if a product can read it
+    const bool readable = dz.ld % 8 == 0 && ((uintptr_t)dz.t.data_ptr() & 15) == 0;
+    const bool make_dz = (nx || nw) && (act || !readable);
+    if (nb || make_dz) {
         Rows z{Tensor(), 0, 0};
         Codes zc;
         Tensor out;
@@ -420,36 +421,42 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
                                   "saved pre-activation does not fit grad_output");
                 z = as_rows(zk);
             }
-            out = at::empty({rows, pitch}, dy.options());
         }
-        check(gact_act_backward(dz.t.data_ptr(), code, rows, cout, dz.ld, act, ptr(z.t), z.ld, ptr(zc.codes), ptr(zc.scales), ptr(out), pitch, ptr(db),
-                                ptr(scr), s), "gact_act_backward");
-        g_launches += 1 + nb;
-        if (act) dz = {out, rows, pitch};
+        if (act || make_dz) out = at::empty({rows, pitch}, dy.options());
+        check(gact_act_backward(dz.t.data_ptr(), code, rows, cout, dz.ld, act, ptr(z.t), z.ld, ptr(zc.codes), ptr(zc.scales), ptr(out), pitch,
+                                nx || nw ? nullptr : ptr(db), ptr(sums), s), "gact_act_backward");
+        g_launches += 1 + !(nx || nw);
+        if (out.defined()) dz = {out, rows, pitch};
     }
-    if (nx || nw) dz = as_operand(dz, cout, s);
-    if (nx) {
-        const Rows wr = as_operand(as_rows(w), cin, s);
-        check(gact_linear_dgrad(dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, code, rows, cin, cout, dx.data_ptr(), ptr(scr), s), "gact_linear_dgrad");
-        g_launches += 1 + (xb > 0);
-    }
+    Codes xc;
+    Rows x{Tensor(), 0, 0};
     if (nw) {
         TORCH_CHECK_VALUE(xk.defined(), "the input was not saved");
-        Rows x{Tensor(), 0, 0};
         if (xs.defined()) {
-            const Codes c{xk, xs};
-            check_codes(c, rows, cin, &dy);
-            const int64_t pitch = xk.size(1);
-            x = {at::empty({rows, pitch}, dy.options()), rows, pitch};
-            check(gact_restore8(xk.data_ptr(), xs.data_ptr(), rows, cin, code, x.t.data_ptr(), pitch, s), "gact_restore8");
-            g_launches++;
+            xc = {xk, xs};
+            check_codes(xc, rows, cin, &dy);
+            x = {at::empty({rows, xk.size(1)}, dy.options()), rows, xk.size(1)};
         } else {
             check_tensor(xk, "saved input", true, &dy);
             TORCH_CHECK_VALUE(xk.dim() > 0 && xk.size(-1) == cin && rows_of(xk) == rows && xk.scalar_type() == dy.scalar_type(),
                               "saved input does not fit grad_output");
             x = as_operand(as_rows(xk), cin, s);
         }
-        check(gact_linear_wgrad(dz.t.data_ptr(), dz.ld, x.t.data_ptr(), x.ld, code, rows, cin, cout, dw.data_ptr(), ptr(scr), s), "gact_linear_wgrad");
+    }
+    // beside the data gradient: the bias gradient's sums, and x restored for the weight gradient; without it the weight
+    // gradient takes the sums and x is restored on its own
+    if (nx) {
+        const Rows wr = as_operand(as_rows(w), cin, s);
+        check(gact_linear_dgrad(dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, code, rows, cin, cout, dx.data_ptr(), ptr(sums), ptr(db), ptr(xc.codes),
+                                ptr(xc.scales), xc.codes.defined() ? x.t.data_ptr() : nullptr, ptr(scr), s), "gact_linear_dgrad");
+        g_launches += 1 + (xb > 0);
+    } else if (xc.codes.defined()) {
+        check(gact_restore8(xk.data_ptr(), xs.data_ptr(), rows, cin, code, x.t.data_ptr(), x.ld, s), "gact_restore8");
+        g_launches++;
+    }
+    if (nw) {
+        check(gact_linear_wgrad(dz.t.data_ptr(), dz.ld, x.t.data_ptr(), x.ld, code, rows, cin, cout, dw.data_ptr(), nx ? nullptr : ptr(sums),
+                                nx ? nullptr : ptr(db), ptr(scr), s), "gact_linear_wgrad");
         g_launches += 1 + (wb > 0);
     }
     return tuple_of({dx, dw, db});

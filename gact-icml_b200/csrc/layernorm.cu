@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
     using T = typename Elem<DT>::T;
     constexpr int SUB = TPR < 32 ? TPR : 32, W = TPR * CH * 8, WARPS = TPR > 32 ? TPR / 32 : 1;
     using Row = Row8<DT, VEC, SUB>;
-    extern __shared__ __align__(16) uint8_t dyn[];
+    extern __shared__ __align__(128) uint8_t dyn[];
     float* pw = (float*)dyn;
     float* pb = pw + W;
     void* stage = dyn + 2 * W * sizeof(float) + (threadIdx.x >> 5) * Stage8<DT, VEC>::kBytes;

@@ -16,10 +16,22 @@ namespace gact {
 __device__ int g_linear_error = 0;
 
 constexpr int kBM = 128, kBK = 64;            // tile rows, reduction per stage (64 16-bit elements = one 128-byte swizzle row)
-constexpr int kGThreads = 384;                // warps: 0 copies, 1 products, 2 TMEM, 3 idle, 4..11 epilogue
+constexpr int kGThreads = 384;                // warps: 0 copies, 1 products, 2 TMEM, 2 and 3 side jobs, 4..11 epilogue
 constexpr int kEpiWarps = 8;
 
 enum { kEpiStore = 0, kEpiLinear = 1, kEpiPartial = 2 };
+
+// Work that the two idle warps of a product's blocks do beside it, in its shadow and without launches of their own:
+// the checkpoint of x beside the forward product (kind 1), x restored from its checkpoint beside the data gradient, for the
+// weight gradient that follows (kind 2), and the bias gradient's partial sums added up beside either gradient.
+struct SideJob {
+    int kind;
+    const void* x; int64_t ld; int stochastic; PhiloxKeys rk;      // 1: rows of cols elements on 16-byte boundaries
+    int8_t* codes; uint8_t* scales;
+    void* out;                                                     // 2: rows of the codes' pitch
+    int64_t rows; int cols, chunks; Divisor by;
+    const float* partial; int parts; int64_t width; void* sums; int64_t n;     // column sums, or partial null
+};
 
 struct GemmArgs {
     int64_t M, N; int ktiles;                 // output rows, columns, reduction in stages
@@ -34,6 +46,7 @@ struct GemmArgs {
     int stochastic; PhiloxKeys rk;
     float* partial;                           // [splits][M][pitchN] fp32
     int64_t ldp;
+    SideJob side;
 };
 
 __device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
@@ -246,6 +259,91 @@ template <int DT> __device__ __forceinline__ float bias_at(const GemmArgs& a, in
     return a.bias && n < a.N ? Elem<DT>::to_float(((const typename Elem<DT>::T*)a.bias)[n]) : 0.0f;
 }
 
+// ---- side jobs ---------------------------------------------------------------------------------------------------------
+// Worker `w` of `n` warps.  Eight chunks per lane are loaded before the first is worked on: with two warps per SM the loads in
+// flight decide (measured beside a product: about 1.2 TB/s over the GPU).
+template <int DT>
+__device__ __forceinline__ void side_job(const SideJob& j, int w, int n) {
+    using T = typename Elem<DT>::T;
+    const int lane = threadIdx.x & 31;
+    constexpr int U = 8;
+    if (j.partial) {
+        // 32 columns per warp, in the order of the parts
+        for (int64_t c = (int64_t)w * 32 + lane; c - lane < j.n; c += (int64_t)n * 32) {
+            if (c < j.n) {
+                float sum = 0.0f;
+                const float* q = j.partial + c;
+                for (int p = 0; p < j.parts; p += 8, q += 8 * j.width) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = p + i < j.parts ? q[i * j.width] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum += v[i];
+                }
+                ((T*)j.sums)[c] = Elem<DT>::from_float(sum);
+            }
+        }
+    }
+    const int64_t total = j.rows * j.chunks;
+    if (j.kind == 1) {
+        for (int64_t i0 = (int64_t)w * 32 * U; i0 < total; i0 += (int64_t)n * 32 * U) {
+            uint32_t raw[U][4];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t i = i0 + u * 32 + lane, row = j.by.div(i);
+                const int col = (int)(i - row * j.chunks) * 8;
+                const T* p = (const T*)j.x + row * j.ld + col;
+                raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
+                if (i < total && col + 8 <= j.cols) {
+                    const uint4 a = ld_stream_u4(p);
+                    raw[u][0] = a.x; raw[u][1] = a.y; raw[u][2] = a.z; raw[u][3] = a.w;
+                } else if (i < total) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (col + e < j.cols) raw[u][e >> 1] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t i = i0 + u * 32 + lane;
+                float2 v[4];
+                raw_to_pairs<DT>(raw[u], v);
+                uint32_t byte;
+                const uint32_t m = absmax8<DT>(raw[u]);
+                const uint2 q = j.stochastic ? codes8<DT, true>(v, m, j.rk, (uint64_t)i, byte) : codes8<DT, false>(v, m, j.rk, (uint64_t)i, byte);
+                if (i < total) {
+                    st_stream_u2(j.codes + i * 8, q);
+                    if ((lane & 3) == 0) j.scales[i >> 2] = (uint8_t)byte;
+                }
+            }
+        }
+    } else if (j.kind == 2) {
+        for (int64_t i0 = (int64_t)w * 32 * U; i0 < total; i0 += (int64_t)n * 32 * U) {
+            uint2 q[U];
+            uint32_t b[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t i = i0 + u * 32 + lane;
+                q[u] = make_uint2(0u, 0u);
+                b[u] = 1;
+                if (i < total) {
+                    q[u] = ld_stream_u2(j.codes + i * 8);
+                    b[u] = ld_ahead_byte(j.scales + (i >> 2));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t i = i0 + u * 32 + lane;
+                if (i < total) {
+                    float2 v[4];
+                    restore_pairs(q[u], scale_down8(b[u]), v);
+                    *(uint4*)((T*)j.out + i * 8) = make_uint4(pack2<DT>(v[0].x, v[0].y), pack2<DT>(v[1].x, v[1].y), pack2<DT>(v[2].x, v[2].y), pack2<DT>(v[3].x, v[3].y));
+                }
+            }
+        }
+    }
+}
+
 // ---- the matrix product ----------------------------------------------------------------------------------------------
 // CG blocks (a cluster) work on one tile of CG * 128 rows and BN columns: each holds its own 128 rows of A, BN / CG columns
 // of B and the accumulators of its rows.  A pair reads every B tile once for 256 rows, which halves the shared-memory
@@ -382,7 +480,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             for (uint32_t i = 0; i < kWaitLimit && !mbar_try(drain, 0); i++) {}
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp < 4) {
+        side_job<DT>(a.side, (int)blockIdx.x * 2 + warp - 2, (int)gridDim.x * 2);
+    } else {
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t acc_empty0 = CG == 1 ? acc_empty : peer_addr(acc_empty, 0);
         uint32_t n = 0;
@@ -520,7 +620,7 @@ static bool make_map(CUtensorMap* m, int dtype, const void* p, int64_t rows, int
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Plan { int cg, bn, splits, per_split; int64_t tiles_m, tiles_n; };
+struct Plan { int cg, bn, splits, per_split; int64_t tiles_m, tiles_n; double ns; };
 
 // Tile shape (two blocks on 256 x 256, one on 128 x 128 or 128 x 64) and splits of the reduction: the combination with the
 // least estimated time.  Measured on products of 16 to 8192 rows (nanoseconds): a launch with one stage takes `fixed`, every
@@ -546,7 +646,7 @@ static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
             const int64_t rounds = (tiles * splits + slots - 1) / slots;
             double t = h.fixed + (double)(rounds * p.per_split - 1) * h.stage;
             if (splits > 1) t += 2800.0 + (double)(splits * 2 + 1) * (double)M * (double)N * 4.0 / 8000.0;
-            if (t < best_t) { best_t = t; best = p; }
+            if (t < best_t) { best_t = t; best = p; best.ns = t; }
         }
     }
     return best;
@@ -613,17 +713,38 @@ struct ActBwdArgs {
 };
 constexpr int kAWarps = 8;
 
-// A warp owns 256 columns (8 per lane) and walks rows, kARows of them side by side; a block takes eight such sets at a time.
-// The next rows' loads are issued before the current ones are worked on.
+// A warp owns 256 columns (8 per lane) and walks rows, kARows of them side by side.  A block takes eight such sets at a time.
+// 64 registers and four blocks per SM: loading the next rows ahead instead took 84 registers and was a quarter slower.
 constexpr int kARows = 2;
-template <int DT, bool VEC, bool COMP, int ACT>
-__global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid_constant__ ActBwdArgs a) {
+//
+// TABLE: a pre-activation from a checkpoint is an 8-bit code times a power of two, so there are 256 slopes per exponent.  Those
+// of the exponents -14 .. 4 are computed once per block; a slope is then one shared-memory read instead of about 20
+// instructions (the kernel was bound by issuing them: GELU on 8192 x 4096 took 59 us, with the table 32; floor 26).  Larger exponents
+// equal the last row (a code's step is past the bend); below, |z| < 0.004 and the slope is its tangent at 0 (the next term,
+// z^3 / 4, is below 2^-25); a NaN block's tangent is NaN.
+constexpr int kLowExp = -14, kHighExp = 4, kTableRows = kHighExp - kLowExp + 1;
+
+template <int DT, bool VEC, bool COMP, int ACT, bool TABLE>
+__global__ void __launch_bounds__(kAWarps * 32, 4) act_backward_kernel(const __grid_constant__ ActBwdArgs a) {
     using T = typename Elem<DT>::T;
     using Row = Row8<DT, VEC, 32>;
     constexpr bool kAct = ACT != GACT_ACT_NONE;
     constexpr int U = kARows;
+    constexpr float kSlope0 = ACT == GACT_ACT_SILU ? 0.5f : 0.79788456080286536f;       // second derivative at 0
+    static_assert(!TABLE || (COMP && kAct), "the table is indexed by codes");
     __shared__ float fold[kAWarps][8][33];
     __shared__ __align__(16) uint8_t staging[VEC ? 16 : kAWarps * Stage8<DT, VEC>::kBytes];
+    __shared__ __align__(1024) float table[TABLE ? kTableRows : 1][TABLE ? 256 : 1];
+    if constexpr (TABLE) {
+        for (int i = threadIdx.x; i < kTableRows * 128; i += kAWarps * 32) {
+            // entries 2 i and 2 i + 1: row by exponent, column by the code's byte
+            const int e = i / 128 + kLowExp, c = (i % 128) * 2;
+            const float step = __uint_as_float((uint32_t)(127 + e) << 23);
+            const float2 v = act_slope2<ACT>(make_float2((float)(int8_t)c * step, (float)(int8_t)(c + 1) * step));
+            *(float2*)(&table[0][0] + 2 * i) = v;
+        }
+        __syncthreads();
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     void* stage = staging + warp * Stage8<DT, VEC>::kBytes;
     const int col = (blockIdx.x * 32 + lane) * 8;
@@ -653,31 +774,48 @@ __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid
         }
     };
     int64_t r = (int64_t)blockIdx.y * kAWarps + warp;
-    fetch(r);
     for (; r < a.rows; r += U * step) {
+        fetch(r);
         uint32_t rawy[U][RawRegs<DT>::N], rawz[U][RawRegs<DT>::N];
         uint2 q[U];
         float down[U];
+        int row_of[U];                                   // the table's row, or -1
 #pragma unroll
         for (int u = 0; u < U; u++) {
             py[u].get(stage, rawy[u]);
             if constexpr (kAct && COMP) {
                 q[u] = pq[u];
                 down[u] = scale_down8(pe[u]);
+                const int e = (int)pe[u] - 127 - kLowExp;
+                row_of[u] = pe[u] == 255u ? -1 : e < kTableRows ? e : kTableRows - 1;       // (e < 0: the tangent)
             } else if constexpr (kAct) {
                 pz[u].get(stage, rawz[u]);
             }
         }
-        fetch(r + U * step);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float2 g[4], z[4];
             raw_to_pairs<DT>(rawy[u], g);
             if constexpr (kAct) {
-                if constexpr (COMP) restore_pairs(q[u], down[u], z);
-                else raw_to_pairs<DT>(rawz[u], z);
+                if (TABLE && row_of[u] >= 0) {
+                    const uint32_t t = smem_addr(table) + (uint32_t)row_of[u] * 1024u;       // (rows start on 1024 bytes)
+                    auto slope = [&](uint32_t off) {
+                        float v;
+                        asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"((off & 0x3fcu) | t));
+                        return v;
+                    };
+                    g[0] = mul2(g[0], make_float2(slope(q[u].x << 2), slope(q[u].x >> 6)));
+                    g[1] = mul2(g[1], make_float2(slope(q[u].x >> 14), slope(q[u].x >> 22)));
+                    g[2] = mul2(g[2], make_float2(slope(q[u].y << 2), slope(q[u].y >> 6)));
+                    g[3] = mul2(g[3], make_float2(slope(q[u].y >> 14), slope(q[u].y >> 22)));
+                } else {
+                    if constexpr (COMP) restore_pairs(q[u], down[u], z);
+                    else raw_to_pairs<DT>(rawz[u], z);
 #pragma unroll
-                for (int i = 0; i < 4; i++) g[i] = mul2(g[i], act_slope2<ACT>(z[i]));
+                    for (int i = 0; i < 4; i++) g[i] = mul2(g[i], TABLE ? fma2(z[i], splat2(kSlope0), splat2(0.5f)) : act_slope2<ACT>(z[i]));
+                }
+                Row::store((T*)a.dz, a.ldo, r + u * step, a.rows, col, a.cols, stage, g);
+            } else if (a.dz) {
                 Row::store((T*)a.dz, a.ldo, r + u * step, a.rows, col, a.cols, stage, g);
             }
             // (the sum takes the products before they are rounded; rows past the end have dy = 0 and a finite slope)
@@ -701,9 +839,12 @@ __global__ void __launch_bounds__(kAWarps * 32) act_backward_kernel(const __grid
     if (c < a.width) a.partial[(int64_t)blockIdx.y * a.width + c] = sum;
 }
 
+// Filling the table takes about a microsecond: worth it from 64 rows per warp on (with the grid below).
+static bool act_bwd_table(int64_t rows, int64_t cols) { return rows * ((cols + 255) / 256) >= (int64_t)sm_count() * 4 * kAWarps * 4; }
+// Parts of the rows (blocks per strip of 256 columns): four blocks per SM.  The count must not depend on anything but the sizes.
 static int64_t act_bwd_parts(int64_t rows, int64_t cols) {
     const int64_t strips = (cols + 255) / 256;
-    int64_t parts = ((int64_t)sm_count() * 8 + strips - 1) / strips;
+    int64_t parts = ((int64_t)sm_count() * 4 + strips - 1) / strips;
     const int64_t most = (rows + kAWarps - 1) / kAWarps;
     if (parts > most) parts = most;
     return parts < 1 ? 1 : parts > 65535 ? 65535 : parts;
@@ -712,14 +853,17 @@ static int64_t act_bwd_parts(int64_t rows, int64_t cols) {
 template <int DT, int ACT> static void launch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
     const int block = kAWarps * 32;
     if constexpr (ACT == GACT_ACT_NONE) {
-        if (vec) act_backward_kernel<DT, true, false, ACT><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, false, ACT><<<grid, block, 0, s>>>(a);
+        if (vec) act_backward_kernel<DT, true, false, ACT, false><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, ACT, false><<<grid, block, 0, s>>>(a);
     } else if (a.codes) {
-        if (vec) act_backward_kernel<DT, true, true, ACT><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, true, ACT><<<grid, block, 0, s>>>(a);
+        // (ReLU's slope is a comparison: no table)
+        constexpr bool kHasTable = ACT != GACT_ACT_RELU;
+        if (vec && kHasTable && act_bwd_table(a.rows, a.cols)) act_backward_kernel<DT, true, true, ACT, kHasTable><<<grid, block, 0, s>>>(a);
+        else if (vec) act_backward_kernel<DT, true, true, ACT, false><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, true, ACT, false><<<grid, block, 0, s>>>(a);
     } else {
-        if (vec) act_backward_kernel<DT, true, false, ACT><<<grid, block, 0, s>>>(a);
-        else act_backward_kernel<DT, false, false, ACT><<<grid, block, 0, s>>>(a);
+        if (vec) act_backward_kernel<DT, true, false, ACT, false><<<grid, block, 0, s>>>(a);
+        else act_backward_kernel<DT, false, false, ACT, false><<<grid, block, 0, s>>>(a);
     }
 }
 template <int DT> static void dispatch_act_bwd(const ActBwdArgs& a, bool vec, dim3 grid, cudaStream_t s) {
@@ -758,16 +902,34 @@ extern "C" int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t 
     return direction == 0 ? gemm_scratch(rows, cout, cin) : direction == 1 ? gemm_scratch(rows, cin, cout) : gemm_scratch(cout, cin, rows);
 }
 
+static SideJob sums_job(const void* partial, int64_t rows, int64_t cols, void* sums) {
+    SideJob j = {};
+    j.partial = (const float*)partial; j.parts = (int)act_bwd_parts(rows, cols); j.width = (cols + 7) / 8 * 8; j.sums = sums; j.n = cols;
+    return j;
+}
+// Whether a side job beside a product is worth it.  Measured: a pair of idle warps makes 14 elements of a checkpoint or restores
+// 20 a nanosecond while it is alone on its SM; beside full epilogues and copies all of them together make 204, or restore 345.
+// A checkpoint beside the product slows its epilogue by more than the kernel of its own takes, except where it saves little
+// more than the launch; a restored x is free while it ends well before the product (8192 x 1024 beside 4096 -> 1024: 2 us
+// instead of 6.5; 8192 x 4096 beside 1024 -> 4096: 44 us instead of 18).
+static bool beside(int kind, int64_t M, int64_t N, int64_t K, int64_t elements) {
+    const Plan p = plan_gemm(M, N, K);
+    const double blocks = (double)(p.tiles_m * p.tiles_n * p.splits * p.cg), sms = sm_count();
+    const double pairs = blocks < sms ? blocks : sms, each = kind == 1 ? 14.0 : 20.0, all = kind == 1 ? 204.0 : 345.0;
+    const double alone = (double)elements / (each * pairs), ns = alone > (double)elements / all ? alone : (double)elements / all;
+    return ns <= 5000.0 || (kind == 2 && ns <= 0.75 * p.ns);
+}
+
 extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
-                           int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* z, void* zcodes, void* zscales,
-                           int stochastic, uint64_t seed, void* scratch, void* stream) {
+                           int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* xcodes, void* xscales, void* z, void* zcodes,
+                           void* zscales, int stochastic, uint64_t seed, void* scratch, void* stream) {
     if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
     if (act < GACT_ACT_NONE || act > GACT_ACT_SILU) return GACT_ERR_MODE;
     if (!dims_ok(rows, cin, cout) || ld_x < cin || ld_w < cin || (residual && ld_res < cout)) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
-    if (!x || !weight || !y || (zcodes && !zscales)) return GACT_ERR_NULL;
+    if (!x || !weight || !y || (xcodes && !xscales) || (zcodes && !zscales)) return GACT_ERR_NULL;
     if (!map_ok(x, ld_x) || !map_ok(weight, ld_w) || (((uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)residual) & 1) ||
-        ((uintptr_t)zcodes & 31) || ((uintptr_t)scratch & 31))
+        ((uintptr_t)zcodes & 31) || ((uintptr_t)xcodes & 31) || ((uintptr_t)scratch & 31))
         return GACT_ERR_ALIGN;
     if (gemm_scratch(rows, cout, cin) && !scratch) return GACT_ERR_NULL;
     GemmArgs a = {};
@@ -776,37 +938,71 @@ extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int6
     a.res = residual; a.ldr = ld_res; a.rvec = vec_bytes(residual, ld_res);
     a.act = act; a.z = z; a.zvec = vec_bytes(z, cout);
     a.zcodes = (int8_t*)zcodes; a.zscales = (uint8_t*)zscales; a.zpitch = pitch8(cout);
-    a.stochastic = stochastic; a.rk = philox_round_keys(seed);
+    // the codes of the pre-activation draw their noise from another key than those of the input
+    a.stochastic = stochastic; a.rk = philox_round_keys(seed + 0x9E3779B97F4A7C15ull);
+    if (xcodes) {
+        if (beside(1, rows, cout, cin, rows * cin)) {
+            SideJob& j = a.side;
+            j.kind = 1; j.x = x; j.ld = ld_x; j.stochastic = stochastic; j.rk = philox_round_keys(seed);
+            j.codes = (int8_t*)xcodes; j.scales = (uint8_t*)xscales; j.rows = rows; j.cols = (int)cin; j.chunks = (int)(pitch8(cin) / 8);
+            j.by = Divisor::of(j.chunks);
+        } else {
+            const int st = gact_checkpoint8(x, dtype, rows, cin, ld_x, stochastic, seed, xcodes, xscales, stream);
+            if (st != GACT_OK) return st;
+        }
+    }
     cudaStream_t s = (cudaStream_t)stream;
     return dtype == GACT_F16 ? run_gemm<GACT_F16, false, false, true>(x, ld_x, weight, ld_w, cin, a, scratch, s)
                              : run_gemm<GACT_BF16, false, false, true>(x, ld_x, weight, ld_w, cin, a, scratch, s);
 }
 
 extern "C" int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weight, int64_t ld_w, int dtype, int64_t rows, int64_t cin, int64_t cout,
-                                 void* dx, void* scratch, void* stream) {
+                                 void* dx, const void* dbias_partial, void* dbias, const void* xcodes, const void* xscales, void* x_restored,
+                                 void* scratch, void* stream) {
     if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
     if (!dims_ok(rows, cin, cout) || ld_dz < cout || ld_w < cin) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
-    if (!dz || !weight || !dx || (gemm_scratch(rows, cin, cout) && !scratch)) return GACT_ERR_NULL;
-    if (!map_ok(dz, ld_dz) || !map_ok(weight, ld_w) || ((uintptr_t)dx & 1) || ((uintptr_t)scratch & 31)) return GACT_ERR_ALIGN;
+    if (!dz || !weight || !dx || (gemm_scratch(rows, cin, cout) && !scratch) || (!dbias_partial != !dbias) || (x_restored && (!xcodes || !xscales)))
+        return GACT_ERR_NULL;
+    if (!map_ok(dz, ld_dz) || !map_ok(weight, ld_w) || ((uintptr_t)dx & 1) || ((uintptr_t)dbias & 1) || ((uintptr_t)dbias_partial & 3) ||
+        ((uintptr_t)xcodes & 31) || ((uintptr_t)x_restored & 15) || ((uintptr_t)scratch & 31))
+        return GACT_ERR_ALIGN;
     GemmArgs a = {};
     a.M = rows; a.N = cin; a.out = dx; a.ldo = cin; a.ovec = vec_bytes(dx, cin);
+    if (dbias) a.side = sums_job(dbias_partial, rows, cout, dbias);
+    if (x_restored) {
+        const int64_t pitch = pitch8(cin);
+        if (beside(2, rows, cin, cout, rows * cin)) {
+            SideJob& j = a.side;
+            j.kind = 2; j.codes = (int8_t*)xcodes; j.scales = (uint8_t*)xscales; j.out = x_restored;
+            j.rows = rows; j.cols = (int)cin; j.chunks = (int)(pitch / 8);
+        } else {
+            const int st = gact_restore8(xcodes, xscales, rows, cin, dtype, x_restored, pitch, stream);
+            if (st != GACT_OK) return st;
+        }
+    }
     cudaStream_t s = (cudaStream_t)stream;
     return dtype == GACT_F16 ? run_gemm<GACT_F16, false, true, false>(dz, ld_dz, weight, ld_w, cout, a, scratch, s)
                              : run_gemm<GACT_BF16, false, true, false>(dz, ld_dz, weight, ld_w, cout, a, scratch, s);
 }
 
 extern "C" int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cin, int64_t cout,
-                                 void* dweight, void* scratch, void* stream) {
+                                 void* dweight, const void* dbias_partial, void* dbias, void* scratch, void* stream) {
     if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
     if (!dims_ok(rows, cin, cout) || ld_dz < cout || ld_x < cin) return GACT_ERR_SIZE;
     cudaStream_t s = (cudaStream_t)stream;
     if (!dweight) return GACT_ERR_NULL;
-    if (rows == 0) return cudaMemsetAsync(dweight, 0, (size_t)(cin * cout * 2), s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
-    if (!dz || !x || (gemm_scratch(cout, cin, rows) && !scratch)) return GACT_ERR_NULL;
-    if (!map_ok(dz, ld_dz) || !map_ok(x, ld_x) || ((uintptr_t)dweight & 1) || ((uintptr_t)scratch & 31)) return GACT_ERR_ALIGN;
+    if (rows == 0) {
+        if (dbias && cudaMemsetAsync(dbias, 0, (size_t)cout * 2, s) != cudaSuccess) return GACT_ERR_LAUNCH;
+        return cudaMemsetAsync(dweight, 0, (size_t)(cin * cout * 2), s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
+    }
+    if (!dz || !x || (gemm_scratch(cout, cin, rows) && !scratch) || (!dbias_partial != !dbias)) return GACT_ERR_NULL;
+    if (!map_ok(dz, ld_dz) || !map_ok(x, ld_x) || ((uintptr_t)dweight & 1) || ((uintptr_t)dbias & 1) || ((uintptr_t)dbias_partial & 3) ||
+        ((uintptr_t)scratch & 31))
+        return GACT_ERR_ALIGN;
     GemmArgs a = {};
     a.M = cout; a.N = cin; a.out = dweight; a.ldo = cin; a.ovec = vec_bytes(dweight, cin);
+    if (dbias) a.side = sums_job(dbias_partial, rows, cout, dbias);
     return dtype == GACT_F16 ? run_gemm<GACT_F16, true, true, false>(dz, ld_dz, x, ld_x, rows, a, scratch, s)
                              : run_gemm<GACT_BF16, true, true, false>(dz, ld_dz, x, ld_x, rows, a, scratch, s);
 }
@@ -826,14 +1022,14 @@ extern "C" int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_
     cudaStream_t s = (cudaStream_t)stream;
     if (rows == 0) return !dbias || cudaMemsetAsync(dbias, 0, (size_t)cols * 2, s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
     if (!dy || (act != GACT_ACT_NONE && (!dz || (!z && (!zcodes || !zscales)))) || (dbias && !scratch)) return GACT_ERR_NULL;
-    if (act == GACT_ACT_NONE && !dbias) return GACT_OK;
+    if (act == GACT_ACT_NONE && !scratch && !dz) return GACT_OK;
     if ((((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)dbias) & 1) || ((uintptr_t)zcodes & 31) || ((uintptr_t)scratch & 15)) return GACT_ERR_ALIGN;
     ActBwdArgs a;
     a.dy = dy; a.ldy = ld_dy; a.z = z; a.ldz = ld_z; a.codes = z ? nullptr : (const int8_t*)zcodes; a.scales = (const uint8_t*)zscales;
     a.chunks = (int)(pitch8(cols) / 8); a.act = act; a.rows = rows; a.cols = (int)cols; a.dz = dz; a.ldo = ld_dz;
-    a.partial = dbias ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
-    const bool vec = rows_aligned(dy, ld_dy, cols, 2) &&
-                     (act == GACT_ACT_NONE || ((!z || rows_aligned(z, ld_z, cols, 2)) && rows_aligned(dz, ld_dz, cols, 2)));
+    a.partial = (float*)scratch; a.width = (int)((cols + 7) / 8 * 8);
+    const bool vec = rows_aligned(dy, ld_dy, cols, 2) && (!dz || rows_aligned(dz, ld_dz, cols, 2)) &&
+                     (act == GACT_ACT_NONE || !z || rows_aligned(z, ld_z, cols, 2));
     const int64_t parts = act_bwd_parts(rows, cols);
     const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)parts);
     if (dtype == GACT_F16) dispatch_act_bwd<GACT_F16>(a, vec, grid, s);

@@ -57,9 +57,9 @@ _SIGNATURES = {
     "gact_layer_norm_backward_scratch_bytes": ([_i64, _i64], _i64),
     "gact_layer_norm_backward": ([_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
     "gact_linear_scratch_bytes": ([_i64, _i64, _i64, _i], _i64),
-    "gact_linear": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _i, _u64, _vp, _vp], _i),
-    "gact_linear_dgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp], _i),
-    "gact_linear_wgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp], _i),
+    "gact_linear": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _u64, _vp, _vp], _i),
+    "gact_linear_dgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "gact_linear_wgrad": ([_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp], _i),
     "gact_act_backward_scratch_bytes": ([_i64, _i64], _i64),
     "gact_act_backward": ([_vp, _i, _i64, _i64, _i64, _i, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp], _i),
 }

@@ -283,28 +283,36 @@ int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t co
 /*
  * y = act(x W^T + bias) + residual for fp16 / bf16, fp32 accumulation; weight is [cout][cin].  x and weight: base and row
  * pitch multiples of 16 bytes (gact_repitch16 makes such a copy).  bias, residual: may be null.  y: contiguous.
- * Kept for the backward pass, each optional: z (pre-activation rounded to `dtype`, contiguous), or zcodes / zscales (its
- * checkpoint, made from the fp32 value; with GACT_ACT_RELU a positive pre-activation keeps a positive code).
+ * Kept for the backward pass, each optional: xcodes / xscales (checkpoint of x, made beside the product), z (pre-activation
+ * rounded to `dtype`, contiguous), or zcodes / zscales (its checkpoint, made from the fp32 value; with GACT_ACT_RELU a
+ * positive pre-activation keeps a positive code).  Stochastic codes of x use `seed`, those of z another key made from it.
  * scratch: gact_linear_scratch_bytes(rows, cin, cout, direction) bytes (0: none needed), direction 0 = forward,
  * 1 = data gradient, 2 = weight gradient.
  */
 int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t cout, int direction);
 int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
-                int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* z, void* zcodes, void* zscales,
-                int stochastic, uint64_t seed, void* scratch, void* stream);
-/* dx = dz W (contiguous).  dz and weight: base and row pitch multiples of 16 bytes. */
-int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weight, int64_t ld_w, int dtype, int64_t rows, int64_t cin,
-                      int64_t cout, void* dx, void* scratch, void* stream);
-/* dW = dz^T x (contiguous [cout][cin]).  dz and x: base and row pitch multiples of 16 bytes. */
-int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cin,
-                      int64_t cout, void* dweight, void* scratch, void* stream);
+                int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* xcodes, void* xscales, void* z, void* zcodes,
+                void* zscales, int stochastic, uint64_t seed, void* scratch, void* stream);
 /*
- * dz = dy act'(z) with z given as a tensor or (z null) as a checkpoint, and dbias = sum of dz over the rows, summed from
- * the unrounded products.  GACT_ACT_NONE: only the sum (dz is dy).  dbias may be null (then no scratch).
+ * dz = dy act'(z) with z given as a tensor or (z null) as a checkpoint; with GACT_ACT_NONE dz is a copy of dy (to another row
+ * pitch), or null.  scratch (optional): partial sums of dz over the rows, added from the unrounded products;
+ * dbias (optional, needs scratch): their sum.  Without dbias the partial sums are left in scratch for one of the products
+ * below to finish.
  */
 int64_t gact_act_backward_scratch_bytes(int64_t rows, int64_t cols);
 int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_t cols, int64_t ld_dy, int act, const void* z, int64_t ld_z,
                       const void* zcodes, const void* zscales, void* dz, int64_t ld_dz, void* dbias, void* scratch, void* stream);
+/*
+ * dx = dz W (contiguous).  dz and weight: base and row pitch multiples of 16 bytes.  Beside the product, each optional:
+ * dbias (cout values) from dbias_partial, the scratch that gact_act_backward(rows, cout) left; x_restored, rows of pitch
+ * gact_checkpoint8_pitch(cin), from the checkpoint of x (what gact_linear_wgrad takes next; 16-byte aligned).
+ */
+int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weight, int64_t ld_w, int dtype, int64_t rows, int64_t cin,
+                      int64_t cout, void* dx, const void* dbias_partial, void* dbias, const void* xcodes, const void* xscales,
+                      void* x_restored, void* scratch, void* stream);
+/* dW = dz^T x (contiguous [cout][cin]).  dz and x: base and row pitch multiples of 16 bytes.  dbias as for the data gradient. */
+int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cin,
+                      int64_t cout, void* dweight, const void* dbias_partial, void* dbias, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

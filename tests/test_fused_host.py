@@ -57,24 +57,28 @@ def test_linear_abi_refusals():
     from gact import _native as nv
     L = nv.lib
     b, p = buf()
-    f = lambda x=p, ldx=64, w=p, ldw=64, bias=p, res=p, ldr=32, dt=2, rows=4, cin=64, cout=32, act=2, y=p, z=None, zc=p, zs=p, scr=p: L.gact_linear(
-        x, ldx, w, ldw, bias, res, ldr, dt, rows, cin, cout, act, y, z, zc, zs, 0, 0, scr, None)
+    f = lambda x=p, ldx=64, w=p, ldw=64, bias=p, res=p, ldr=32, dt=2, rows=4, cin=64, cout=32, act=2, y=p, xc=p, xs=p, z=None, zc=p, zs=p, scr=p: \
+        L.gact_linear(x, ldx, w, ldw, bias, res, ldr, dt, rows, cin, cout, act, y, xc, xs, z, zc, zs, 0, 0, scr, None)
     assert f(dt=0) == 2 and f(dt=3) == 2 and f(act=5) == 6 and f(act=-1) == 6
     assert f(rows=-1) == 5 and f(cin=0) == 5 and f(cout=0) == 5 and f(ldx=63) == 5 and f(ldw=8) == 5 and f(ldr=31) == 5
     assert f(cin=1 << 25, ldx=1 << 25, ldw=1 << 25) == 5 and f(rows=1 << 31) == 5
-    assert f(x=None) == 3 and f(w=None) == 3 and f(y=None) == 3 and f(zs=None) == 3
+    assert f(x=None) == 3 and f(w=None) == 3 and f(y=None) == 3 and f(zs=None) == 3 and f(xs=None) == 3
     assert f(x=p + 2) == 4 and f(ldx=65) == 4 and f(w=p + 8) == 4 and f(ldw=68) == 4 and f(y=p + 1) == 4 and f(zc=p + 16) == 4 and f(scr=p + 16) == 4
-    assert f(bias=p + 1) == 4 and f(res=p + 1) == 4
+    assert f(bias=p + 1) == 4 and f(res=p + 1) == 4 and f(xc=p + 16) == 4
     assert f(rows=0, x=None) == 0
-    d = lambda dz=p, ldz=32, w=p, ldw=64, dt=2, rows=4, cin=64, cout=32, dx=p, scr=p: L.gact_linear_dgrad(dz, ldz, w, ldw, dt, rows, cin, cout, dx, scr, None)
+    d = lambda dz=p, ldz=32, w=p, ldw=64, dt=2, rows=4, cin=64, cout=32, dx=p, part=p, db=p, xc=p, xs=p, xr=p, scr=p: \
+        L.gact_linear_dgrad(dz, ldz, w, ldw, dt, rows, cin, cout, dx, part, db, xc, xs, xr, scr, None)
     assert d(dt=0) == 2 and d(ldz=31) == 5 and d(dz=None) == 3 and d(dx=None) == 3 and d(dz=p + 4) == 4 and d(ldz=36) == 4 and d(rows=0, dz=None) == 0
-    e = lambda dz=p, ldz=32, x=p, ldx=64, dt=2, rows=4, cin=64, cout=32, dw=p, scr=p: L.gact_linear_wgrad(dz, ldz, x, ldx, dt, rows, cin, cout, dw, scr, None)
+    assert d(part=None) == 3 and d(db=None) == 3 and d(xc=None) == 3 and d(xs=None) == 3 and d(xr=p + 8) == 4 and d(db=p + 1) == 4 and d(part=p + 2) == 4
+    e = lambda dz=p, ldz=32, x=p, ldx=64, dt=2, rows=4, cin=64, cout=32, dw=p, part=p, db=p, scr=p: \
+        L.gact_linear_wgrad(dz, ldz, x, ldx, dt, rows, cin, cout, dw, part, db, scr, None)
     assert e(dt=0) == 2 and e(ldx=8) == 5 and e(x=None) == 3 and e(dw=None) == 3 and e(x=p + 4) == 4 and e(ldx=65) == 4
+    assert e(part=None) == 3 and e(db=None) == 3 and e(db=p + 1) == 4
     g = lambda dy=p, dt=2, rows=4, cols=32, ld=32, act=2, z=None, ldz=32, zc=p, zs=p, dz=p, ldo=32, db=p, scr=p: L.gact_act_backward(
         dy, dt, rows, cols, ld, act, z, ldz, zc, zs, dz, ldo, db, scr, None)
     assert g(dt=0) == 2 and g(act=9) == 6 and g(cols=0) == 5 and g(ld=8) == 5 and g(ldo=8) == 5 and g(z=p, ldz=8) == 5
     assert g(dy=None) == 3 and g(dz=None) == 3 and g(zc=None) == 3 and g(scr=None) == 3 and g(zc=p + 8) == 4 and g(dy=p + 1) == 4
-    assert g(act=0, db=None) == 0 and g(rows=0, db=None, dy=None) == 0
+    assert g(act=0, db=None, scr=None, dz=None) == 0 and g(rows=0, db=None, dy=None) == 0
     assert L.gact_linear_scratch_bytes(4, 0, 32, 0) == -1 and L.gact_linear_scratch_bytes(4, 8, 8, 3) == -1 and L.gact_linear_scratch_bytes(0, 8, 8, 0) == 0
 
 
