@@ -289,6 +289,17 @@ struct Divisor {
     }
 };
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <class K> static inline bool allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[kMaxDevices]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    if (!done[dev].load(std::memory_order_relaxed)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+        done[dev].store(true, std::memory_order_relaxed);
+    }
+    return true;
+}
+
 // Blocks of a kernel that one SM holds, asked of the runtime once per device.
 template <class K> static inline int resident_blocks(K kernel, int threads, size_t smem, std::atomic<int> (&cache)[kMaxDevices]) {
     int dev = 0;

@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -73,11 +74,16 @@ Rows as_rows(const Tensor& t) {
     return {u, rows, ld};
 }
 
+// uninitialised memory of the caching allocator, without the dispatcher's detour
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+    return Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
+
 // an operand that a tensor map can describe: base and pitch multiples of 16 bytes; anything else is copied to such a pitch
 Rows as_operand(Rows r, int64_t cols, void* stream) {
     if (r.ld % 8 == 0 && ((uintptr_t)r.t.data_ptr() & 15) == 0) return r;
     const int64_t pitch = (cols + 7) / 8 * 8;
-    Tensor out = at::empty({r.rows, pitch}, r.t.options());
+    Tensor out = make({r.rows, pitch}, r.t.scalar_type(), r.t);
     check(gact_repitch16(r.t.data_ptr(), r.ld, r.rows, cols, out.data_ptr(), pitch, stream), "gact_repitch16");
     g_launches++;
     return {out, r.rows, pitch};
@@ -85,30 +91,31 @@ Rows as_operand(Rows r, int64_t cols, void* stream) {
 
 struct Seed { int stochastic = 0; uint64_t value = 0; };
 
-struct Codes { Tensor codes, scales; };
+// A checkpoint is one byte tensor: rows x pitch codes, then rows x pitch / 32 scales.
+struct Codes {
+    Tensor buf; int64_t split = 0;
+    bool defined() const { return buf.defined(); }
+    void* codes() const { return buf.defined() ? buf.data_ptr() : nullptr; }
+    void* scales() const { return buf.defined() ? (char*)buf.data_ptr() + split : nullptr; }
+};
 Codes empty_codes(int64_t rows, int64_t cols, const Tensor& like) {
-    const int64_t pitch = gact_checkpoint8_pitch(cols);
-    const auto opt = like.options().dtype(at::kChar);
-    return {at::empty({rows, pitch}, opt), at::empty({rows, pitch / GACT_BLOCK8}, opt)};
+    const int64_t n = rows * gact_checkpoint8_pitch(cols);
+    return {make({n + n / GACT_BLOCK8}, at::kChar, like), n};
 }
-void check_codes(const Codes& c, int64_t rows, int64_t cols, const Tensor* like) {
-    const int64_t pitch = gact_checkpoint8_pitch(cols);
-    const Tensor* ts[2] = {&c.codes, &c.scales};
-    const int64_t want[2] = {pitch, pitch / GACT_BLOCK8};
-    for (int i = 0; i < 2; i++) {
-        const Tensor& t = *ts[i];
-        const char* name = i ? "checkpoint scales" : "checkpoint codes";
-        TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
-        TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == want[i] && t.is_contiguous() && t.element_size() == 1, name,
-                          " must be contiguous bytes of shape (", rows, ", ", want[i], ")");
-        const Tensor& l = like ? *like : c.codes;
-        TORCH_CHECK(t.device() == l.device(), name, " is on ", t.device().str(), ", the input on ", l.device().str());
-    }
+// `buf` as the checkpoint of rows x cols
+Codes as_codes(const Tensor& buf, int64_t rows, int64_t cols, const Tensor* like) {
+    const int64_t n = rows * gact_checkpoint8_pitch(cols);
+    TORCH_CHECK(buf.is_cuda(), "checkpoint must be a CUDA tensor!");
+    TORCH_CHECK_VALUE(buf.dim() == 1 && buf.scalar_type() == at::kChar && buf.is_contiguous() && buf.size(0) == n + n / GACT_BLOCK8,
+                      "the checkpoint of ", rows, " x ", cols, " elements takes ", n + n / GACT_BLOCK8, " contiguous int8, got ", buf.sizes());
+    if (like) TORCH_CHECK(buf.device() == like->device(), "checkpoint is on ", buf.device().str(), ", the input on ", like->device().str());
+    return {buf, n};
 }
+bool is_codes(const Tensor& t) { return t.defined() && t.scalar_type() == at::kChar; }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-Tensor scratch(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
+Tensor scratch(int64_t bytes, const Tensor& like) { return bytes > 0 ? make({bytes}, at::kByte, like) : Tensor(); }
 std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
     std::vector<int64_t> s = t.sizes().vec();
     s.back() = last;
@@ -120,8 +127,8 @@ Codes checkpoint8(const Tensor& x, const Seed& seed) {
     const int64_t cols = x.size(-1);
     Codes c = empty_codes(r.rows, cols, x);
     if (x.numel() == 0) return c;
-    check(gact_checkpoint8(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, seed.stochastic, seed.value, c.codes.data_ptr(),
-                           c.scales.data_ptr(), stream_of(x)), "gact_checkpoint8");
+    check(gact_checkpoint8(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, seed.stochastic, seed.value, c.codes(), c.scales(),
+                           stream_of(x)), "gact_checkpoint8");
     g_launches++;
     return c;
 }
@@ -160,7 +167,7 @@ PyObject* tuple_of(std::initializer_list<Tensor> ts) {
 void count_args(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, "takes ", want, " arguments, got ", n); }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------
-// checkpoint8(input, seed) -> (codes, scales)
+// checkpoint8(input, seed) -> buffer
 PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     count_args(nargs, 2);
@@ -169,35 +176,34 @@ PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(x.device());
-    const Codes c = checkpoint8(x, seed_arg(args[1]));
-    return tuple_of({c.codes, c.scales});
+    return wrap(checkpoint8(x, seed_arg(args[1])).buf);
     END_HANDLE_TH_ERRORS
 }
 
-// restore8(codes, scales, shape, dtype) -> tensor
+// restore8(buffer, shape, dtype) -> tensor
 PyObject* py_restore8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 4);
-    const Codes c{tensor_arg(args[0], "codes"), tensor_arg(args[1], "scales")};
-    TORCH_CHECK_TYPE(PyTuple_Check(args[2]), "shape must be a tuple");
-    TORCH_CHECK_TYPE(THPDtype_Check(args[3]), "dtype must be a torch.dtype");
+    count_args(nargs, 3);
+    const Tensor buf = tensor_arg(args[0], "checkpoint");
+    TORCH_CHECK_TYPE(PyTuple_Check(args[1]), "shape must be a tuple");
+    TORCH_CHECK_TYPE(THPDtype_Check(args[2]), "dtype must be a torch.dtype");
     std::vector<int64_t> shape;
     int64_t rows = 1;
-    const Py_ssize_t nd = PyTuple_GET_SIZE(args[2]);
+    const Py_ssize_t nd = PyTuple_GET_SIZE(args[1]);
     for (Py_ssize_t i = 0; i < nd; i++) {
-        shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[2], i)));
+        shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], i)));
         if (PyErr_Occurred()) throw python_error();
         if (i + 1 < nd) rows *= shape.back();
     }
-    const at::ScalarType st = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+    const at::ScalarType st = reinterpret_cast<THPDtype*>(args[2])->scalar_type;
     TORCH_CHECK(type_code(st) >= 0, "The type of the result is not correct!");
     TORCH_CHECK_VALUE(nd > 0, "a checkpoint has at least one dimension");
-    check_codes(c, rows, shape.back(), nullptr);
+    const Codes c = as_codes(buf, rows, shape.back(), nullptr);
     at::AutoDispatchBelowADInplaceOrView below;
-    c10::cuda::CUDAGuard guard(c.codes.device());
-    const Tensor out = at::empty(shape, c.codes.options().dtype(st));
+    c10::cuda::CUDAGuard guard(buf.device());
+    const Tensor out = make(shape, st, buf);
     if (out.numel() > 0) {
-        check(gact_restore8(c.codes.data_ptr(), c.scales.data_ptr(), rows, shape.back(), type_code(st), out.data_ptr(), shape.back(), stream_of(out)),
+        check(gact_restore8(c.codes(), c.scales(), rows, shape.back(), type_code(st), out.data_ptr(), shape.back(), stream_of(out)),
               "gact_restore8");
         g_launches++;
     }
@@ -224,7 +230,7 @@ at::ScalarType param_type(const Tensor& w, const Tensor& b, int64_t cols, const 
     return t;
 }
 
-// layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, codes or input, scales, statistics, weight)
+// layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, checkpoint or input, statistics, weight)
 PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     count_args(nargs, 7);
@@ -244,31 +250,31 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (w.defined()) w = w.contiguous();
     if (b.defined()) b = b.contiguous();
     const Rows r = as_rows(x);
-    const Tensor y = at::empty(x.sizes(), x.options());
+    const Tensor y = make(x.sizes(), x.scalar_type(), x);
     Codes c;
     Tensor stats;
     if (save) {
-        stats = at::empty({r.rows, 2}, x.options().dtype(at::kFloat));
+        stats = make({r.rows, 2}, at::kFloat, x);
         if (compress) c = empty_codes(r.rows, cols, x);
     }
     if (r.rows > 0) {
         check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(),
-                              (float*)ptr(stats), ptr(c.codes), ptr(c.scales), seed.stochastic, seed.value, stream_of(x)),
+                              (float*)ptr(stats), c.codes(), c.scales(), seed.stochastic, seed.value, stream_of(x)),
               "gact_layer_norm");
         g_launches++;
     }
-    return tuple_of({y, !save ? Tensor() : compress ? c.codes : x, c.scales, stats, w});
+    return tuple_of({y, !save ? Tensor() : compress ? c.buf : x, stats, w});
     END_HANDLE_TH_ERRORS
 }
 
-// layer_norm_backward(grad_output, codes or input, scales or None, statistics, weight, fp32 parameters, need_input,
-//                     need_weight, need_bias) -> (grad of the input, of weight, of bias)
+// layer_norm_backward(grad_output, checkpoint or input, statistics, weight, fp32 parameters, need_input, need_weight,
+//                     need_bias) -> (grad of the input, of weight, of bias)
 PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 9);
-    const Tensor dy = tensor_arg(args[0], "grad_output"), kept = tensor_arg(args[1], "saved input"), scales = optional_arg(args[2], "saved scales"),
-                 stats = tensor_arg(args[3], "saved statistics"), w = optional_arg(args[4], "weight");
-    const bool f32 = bool_arg(args[5]), nx = bool_arg(args[6]), nw = bool_arg(args[7]), nb = bool_arg(args[8]);
+    count_args(nargs, 8);
+    const Tensor dy = tensor_arg(args[0], "grad_output"), kept = tensor_arg(args[1], "saved input"), stats = tensor_arg(args[2], "saved statistics"),
+                 w = optional_arg(args[3], "weight");
+    const bool f32 = bool_arg(args[4]), nx = bool_arg(args[5]), nw = bool_arg(args[6]), nb = bool_arg(args[7]);
     check_tensor(dy, "grad_output", false, &stats);
     TORCH_CHECK_VALUE(dy.dim() > 0, "grad_output needs at least one dimension");
     at::AutoDispatchBelowADInplaceOrView below;
@@ -279,9 +285,8 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
                       "saved statistics do not fit grad_output");
     Rows x{Tensor(), 0, 0};
     Codes c;
-    if (scales.defined()) {
-        c = {kept, scales};
-        check_codes(c, r.rows, cols, &dy);
+    if (is_codes(kept)) {
+        c = as_codes(kept, r.rows, cols, &dy);
     } else {
         check_tensor(kept, "saved input", false, &dy);
         TORCH_CHECK_VALUE(kept.sizes() == dy.sizes() && kept.scalar_type() == dy.scalar_type(), "saved input does not fit grad_output");
@@ -293,12 +298,12 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
         TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == cols && w.is_contiguous() && w.scalar_type() == pt, "weight does not fit grad_output");
     }
     Tensor dx, dw, db, scr;
-    if (nx) dx = at::empty(dy.sizes(), dy.options());
-    if (nw) dw = at::empty({cols}, dy.options().dtype(pt));
-    if (nb) db = at::empty({cols}, dy.options().dtype(pt));
+    if (nx) dx = make(dy.sizes(), dy.scalar_type(), dy);
+    if (nw) dw = make({cols}, pt, dy);
+    if (nb) db = make({cols}, pt, dy);
     if (nw || nb) scr = scratch(gact_layer_norm_backward_scratch_bytes(r.rows, cols), dy);
     if (nx || nw || nb) {
-        check(gact_layer_norm_backward(r.t.data_ptr(), type_code(dy.scalar_type()), r.rows, cols, r.ld, ptr(x.t), x.ld, ptr(c.codes), ptr(c.scales),
+        check(gact_layer_norm_backward(r.t.data_ptr(), type_code(dy.scalar_type()), r.rows, cols, r.ld, ptr(x.t), x.ld, c.codes(), c.scales(),
                                        (const float*)stats.data_ptr(), ptr(w), type_code(pt), ptr(dx), ptr(dw), ptr(db), ptr(scr), stream_of(dy)),
               "gact_layer_norm_backward");
         g_launches += 1 + (nw || nb);
@@ -307,11 +312,11 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
     END_HANDLE_TH_ERRORS
 }
 
-// linear(input, weight, bias, activation code, residual, compress, seed, save, codes, scales)
-//   -> (y, codes or input, scales, codes of z or z, scales of z)
+// linear(input, weight, bias, activation code, residual, compress, seed, save, checkpoint of the input or None)
+//   -> (y, checkpoint or input, checkpoint of z or z)
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 10);
+    count_args(nargs, 9);
     const Tensor x = tensor_arg(args[0], "input"), w = tensor_arg(args[1], "weight");
     Tensor b = optional_arg(args[2], "bias");
     const int act = (int)PyLong_AsLong(args[3]);
@@ -319,7 +324,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const Tensor res = optional_arg(args[4], "residual");
     const bool compress = bool_arg(args[5]), save = bool_arg(args[7]);
     const Seed seed = seed_arg(args[6]);
-    Codes c{optional_arg(args[8], "checkpoint codes"), optional_arg(args[9], "checkpoint scales")};
+    const Tensor given = optional_arg(args[8], "checkpoint");
     check_tensor(x, "input", true, nullptr);
     check_tensor(w, "weight", true, &x);
     TORCH_CHECK(w.scalar_type() == x.scalar_type(), "The type of weight is not correct!");
@@ -343,14 +348,15 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Rows xr = as_rows(x), wr = as_rows(w);
     Rows rr{Tensor(), 0, 0};
     if (res.defined()) rr = as_rows(res);
-    if (c.codes.defined()) check_codes(c, xr.rows, cin, &x);
-    const Tensor y = at::empty(out_shape, x.options());
+    Codes c;
+    if (given.defined()) c = as_codes(given, xr.rows, cin, &x);
+    const Tensor y = make(out_shape, x.scalar_type(), x);
     Codes zc, xc;                                        // xc: the checkpoint of x that this call makes
     Tensor z;
     if (save) {
         if (act && compress) zc = empty_codes(xr.rows, cout, x);
-        else if (act) z = at::empty({xr.rows, cout}, x.options());
-        if (compress && !c.codes.defined()) c = xc = empty_codes(xr.rows, cin, x);
+        else if (act) z = make({xr.rows, cout}, x.scalar_type(), x);
+        if (compress && !c.defined()) c = xc = empty_codes(xr.rows, cin, x);
     }
     if (xr.rows > 0) {
         void* s = stream_of(x);
@@ -359,26 +365,25 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const int64_t bytes = gact_linear_scratch_bytes(xr.rows, cin, cout, 0);
         const Tensor scr = scratch(bytes, x);
         check(gact_linear(xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, ptr(b), ptr(rr.t), rr.ld, type_code(x.scalar_type()), xr.rows, cin, cout, act,
-                          y.data_ptr(), ptr(xc.codes), ptr(xc.scales), ptr(z), ptr(zc.codes), ptr(zc.scales), seed.stochastic, seed.value, ptr(scr), s),
+                          y.data_ptr(), xc.codes(), xc.scales(), ptr(z), zc.codes(), zc.scales(), seed.stochastic, seed.value, ptr(scr), s),
               "gact_linear");
         g_launches += 1 + (bytes > 0);
     }
-    if (!save) return tuple_of({y, Tensor(), Tensor(), Tensor(), Tensor()});
-    return tuple_of({y, compress ? c.codes : x, compress ? c.scales : Tensor(), zc.codes.defined() ? zc.codes : z, zc.scales});
+    if (!save) return tuple_of({y, Tensor(), Tensor()});
+    return tuple_of({y, compress ? c.buf : x, zc.defined() ? zc.buf : z});
     END_HANDLE_TH_ERRORS
 }
 
-// linear_backward(grad_output, weight, activation code, codes or input, scales or None, codes of z or z or None, scales of z
-//                 or None, need_input, need_weight, need_bias) -> (grad of the input, of weight, of bias)
+// linear_backward(grad_output, weight, activation code, checkpoint or input, checkpoint of z or z or None, need_input,
+//                 need_weight, need_bias) -> (grad of the input, of weight, of bias)
 PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 10);
+    count_args(nargs, 8);
     const Tensor dy = tensor_arg(args[0], "grad_output"), w = tensor_arg(args[1], "weight");
     const int act = (int)PyLong_AsLong(args[2]);
     if (PyErr_Occurred()) throw python_error();
-    const Tensor xk = optional_arg(args[3], "saved input"), xs = optional_arg(args[4], "saved scales"), zk = optional_arg(args[5], "saved pre-activation"),
-                 zs = optional_arg(args[6], "saved scales");
-    const bool nx = bool_arg(args[7]), nw = bool_arg(args[8]), nb = bool_arg(args[9]);
+    const Tensor xk = optional_arg(args[3], "saved input"), zk = optional_arg(args[4], "saved pre-activation");
+    const bool nx = bool_arg(args[5]), nw = bool_arg(args[6]), nb = bool_arg(args[7]);
     check_tensor(w, "weight", true, nullptr);
     check_tensor(dy, "grad_output", true, &w);
     TORCH_CHECK(dy.scalar_type() == w.scalar_type(), "The type of grad_output is not correct!");
@@ -390,9 +395,9 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     Rows dz = as_rows(dy);
     const int64_t rows = dz.rows;
     Tensor dx, dw, db;
-    if (nx) dx = at::empty(with_last(dy, cin), dy.options());
-    if (nw) dw = at::empty({cout, cin}, dy.options());
-    if (nb) db = at::empty({cout}, dy.options());
+    if (nx) dx = make(with_last(dy, cin), dy.scalar_type(), dy);
+    if (nw) dw = make({cout, cin}, dy.scalar_type(), dy);
+    if (nb) db = make({cout}, dy.scalar_type(), dy);
     if (rows == 0) {
         if (nw) dw.zero_();
         if (nb) db.zero_();
@@ -412,9 +417,8 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         const int64_t pitch = (cout + 7) / 8 * 8;
         if (act) {
             TORCH_CHECK_VALUE(zk.defined(), "the pre-activation was not saved");
-            if (zs.defined()) {
-                zc = {zk, zs};
-                check_codes(zc, rows, cout, &dy);
+            if (is_codes(zk)) {
+                zc = as_codes(zk, rows, cout, &dy);
             } else {
                 check_tensor(zk, "saved pre-activation", true, &dy);
                 TORCH_CHECK_VALUE(zk.dim() == 2 && zk.size(0) == rows && zk.size(1) == cout && zk.scalar_type() == dy.scalar_type(),
@@ -422,8 +426,8 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
                 z = as_rows(zk);
             }
         }
-        if (act || make_dz) out = at::empty({rows, pitch}, dy.options());
-        check(gact_act_backward(dz.t.data_ptr(), code, rows, cout, dz.ld, act, ptr(z.t), z.ld, ptr(zc.codes), ptr(zc.scales), ptr(out), pitch,
+        if (act || make_dz) out = make({rows, pitch}, dy.scalar_type(), dy);
+        check(gact_act_backward(dz.t.data_ptr(), code, rows, cout, dz.ld, act, ptr(z.t), z.ld, zc.codes(), zc.scales(), ptr(out), pitch,
                                 nx || nw ? nullptr : ptr(db), ptr(sums), s), "gact_act_backward");
         g_launches += 1 + !(nx || nw);
         if (out.defined()) dz = {out, rows, pitch};
@@ -432,10 +436,10 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     Rows x{Tensor(), 0, 0};
     if (nw) {
         TORCH_CHECK_VALUE(xk.defined(), "the input was not saved");
-        if (xs.defined()) {
-            xc = {xk, xs};
-            check_codes(xc, rows, cin, &dy);
-            x = {at::empty({rows, xk.size(1)}, dy.options()), rows, xk.size(1)};
+        if (is_codes(xk)) {
+            xc = as_codes(xk, rows, cin, &dy);
+            const int64_t pitch = gact_checkpoint8_pitch(cin);
+            x = {make({rows, pitch}, dy.scalar_type(), dy), rows, pitch};
         } else {
             check_tensor(xk, "saved input", true, &dy);
             TORCH_CHECK_VALUE(xk.dim() > 0 && xk.size(-1) == cin && rows_of(xk) == rows && xk.scalar_type() == dy.scalar_type(),
@@ -447,11 +451,11 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     // gradient takes the sums and x is restored on its own
     if (nx) {
         const Rows wr = as_operand(as_rows(w), cin, s);
-        check(gact_linear_dgrad(dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, code, rows, cin, cout, dx.data_ptr(), ptr(sums), ptr(db), ptr(xc.codes),
-                                ptr(xc.scales), xc.codes.defined() ? x.t.data_ptr() : nullptr, ptr(scr), s), "gact_linear_dgrad");
+        check(gact_linear_dgrad(dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, code, rows, cin, cout, dx.data_ptr(), ptr(sums), ptr(db), xc.codes(),
+                                xc.scales(), xc.defined() ? x.t.data_ptr() : nullptr, ptr(scr), s), "gact_linear_dgrad");
         g_launches += 1 + (xb > 0);
-    } else if (xc.codes.defined()) {
-        check(gact_restore8(xk.data_ptr(), xs.data_ptr(), rows, cin, code, x.t.data_ptr(), x.ld, s), "gact_restore8");
+    } else if (xc.defined()) {
+        check(gact_restore8(xc.codes(), xc.scales(), rows, cin, code, x.t.data_ptr(), x.ld, s), "gact_restore8");
         g_launches++;
     }
     if (nw) {
@@ -467,14 +471,14 @@ PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launc
 
 #define FAST(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL
 PyMethodDef kMethods[] = {
-    {"checkpoint8", FAST(py_checkpoint8), "checkpoint8(input, seed) -> (codes, scales)"},
-    {"restore8", FAST(py_restore8), "restore8(codes, scales, shape, dtype) -> tensor"},
-    {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, kept, scales, statistics, weight)"},
+    {"checkpoint8", FAST(py_checkpoint8), "checkpoint8(input, seed) -> buffer"},
+    {"restore8", FAST(py_restore8), "restore8(buffer, shape, dtype) -> tensor"},
+    {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, kept, statistics, weight)"},
     {"layer_norm_backward", FAST(py_layer_norm_backward),
-     "layer_norm_backward(grad_output, kept, scales, statistics, weight, fp32 parameters, need_input, need_weight, need_bias) -> three gradients"},
-    {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, codes, scales) -> (y, kept, scales, z, z scales)"},
+     "layer_norm_backward(grad_output, kept, statistics, weight, fp32 parameters, need_input, need_weight, need_bias) -> three gradients"},
+    {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, checkpoint) -> (y, kept, z)"},
     {"linear_backward", FAST(py_linear_backward),
-     "linear_backward(grad_output, weight, activation, kept, scales, z, z scales, need_input, need_weight, need_bias) -> three gradients"},
+     "linear_backward(grad_output, weight, activation, kept, z, need_input, need_weight, need_bias) -> three gradients"},
     {"launches", py_launches, METH_NOARGS, "library kernels enqueued by this module"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fused", "Host side of gact.fused.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};

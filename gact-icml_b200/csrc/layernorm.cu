@@ -150,7 +150,8 @@ template <int DT, int TPR, int CH, bool VEC> static int launch_ln_vec(const LnAr
     auto* k = layer_norm_kernel<DT, TPR, CH, VEC>;
     constexpr int kBlock = TPR > 32 ? TPR : 128;
     constexpr int kSmem = 2 * TPR * CH * 8 * (int)sizeof(float) + kBlock / 32 * Stage8<DT, VEC>::kBytes;
-    if (kSmem > 40 * 1024 && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return GACT_ERR_LAUNCH;
+    static std::atomic<bool> allowed[kMaxDevices];
+    if (kSmem > 40 * 1024 && !allow_smem(k, kSmem, allowed)) return GACT_ERR_LAUNCH;
     static std::atomic<int> cache[kMaxDevices];
     const int64_t per = kBlock / TPR, want = (a.rows + per - 1) / per;
     const int64_t most = (int64_t)sm_count() * resident_blocks(k, kBlock, kSmem, cache);
@@ -595,7 +596,8 @@ static int64_t ln_bwd_blocks(bool vec, int64_t rows, int64_t cols) {
 template <int DT, int TPR, int CH, bool COMP> static int launch_ln_bwd_ring_kernel(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
     auto* k = layer_norm_backward_ring_kernel<DT, TPR, CH, COMP>;
     constexpr int W = TPR * CH * 8, E = Elem<DT>::kBytes, kSmem = W * (int)sizeof(float) + kRingStages * W * (E + (COMP ? 1 : E));
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return GACT_ERR_LAUNCH;
+    static std::atomic<bool> allowed[kMaxDevices];
+    if (!allow_smem(k, kSmem, allowed)) return GACT_ERR_LAUNCH;
     k<<<(unsigned)blocks, TPR, kSmem, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }

@@ -665,7 +665,8 @@ static int vec_bytes(const void* p, int64_t ld) {
 template <int DT, bool A_MN, bool B_MN, int CG, int BN, int EPI>
 static int launch_gemm_kernel(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& a, cudaStream_t s) {
     auto* k = gemm_kernel<DT, A_MN, B_MN, CG, BN, EPI>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<CG, BN>::kBytes) != cudaSuccess) return GACT_ERR_LAUNCH;
+    static std::atomic<bool> allowed[kMaxDevices];
+    if (!allow_smem(k, Ring<CG, BN>::kBytes, allowed)) return GACT_ERR_LAUNCH;
     const int64_t units = (int64_t)a.tiles_m * a.tiles_n * a.splits, slots = sm_count() / CG;
     const int64_t grid = (units < slots ? units : slots) * CG;
     k<<<(unsigned)grid, kGThreads, Ring<CG, BN>::kBytes, s>>>(ma, mb, a);

@@ -28,16 +28,37 @@ LAYER_NORM_MAX_COLS = 16384
 # checkpoints
 # ---------------------------------------------------------------------------------------------------------------
 class Checkpoint8:
-    """A tensor kept in 8 bits: ``codes`` int8 (rows, pitch), ``scales`` int8 (rows, pitch / 32; the bits of an unsigned
-    biased exponent), and the ``shape`` and ``dtype`` it restores to.  pitch = last dimension rounded up to 32."""
-    __slots__ = ("codes", "scales", "shape", "dtype")
+    """A tensor kept in 8 bits: ``buf`` (int8, one dimension) holds the codes and behind them the scales, ``shape`` and
+    ``dtype`` say what it restores to.  ``codes``: int8 (rows, pitch), pitch = last dimension rounded up to 32; ``scales``: int8
+    (rows, pitch / 32), the bits of an unsigned biased exponent."""
+    __slots__ = ("buf", "shape", "dtype")
 
-    def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+    def __init__(self, buf, shape, dtype):
+        self.buf, self.shape, self.dtype = buf, shape, dtype
+
+    def _layout(self):
+        rows = 1
+        for n in self.shape[:-1]:
+            rows *= n
+        return rows, (self.shape[-1] + nv.BLOCK8 - 1) // nv.BLOCK8 * nv.BLOCK8
+
+    @property
+    def codes(self):
+        rows, pitch = self._layout()
+        return self.buf[:rows * pitch].view(rows, pitch)
+
+    @property
+    def scales(self):
+        rows, pitch = self._layout()
+        return self.buf[rows * pitch:].view(rows, pitch // nv.BLOCK8)
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self.buf.numel()
+
+
+def _unwrap(kept):
+    return kept.buf if type(kept) is Checkpoint8 else kept
 
 
 def op_checkpoint8(input, seed=None):
@@ -45,15 +66,14 @@ def op_checkpoint8(input, seed=None):
 
     Rounds to nearest, or with a ``seed`` stochastically (unbiased; the same seed gives the same codes).  A block that
     holds a NaN or an infinity restores to NaN throughout."""
-    codes, scales = _fused.checkpoint8(input, seed)
-    return Checkpoint8(codes, scales, input.shape, input.dtype)
+    return Checkpoint8(_fused.checkpoint8(input, seed), input.shape, input.dtype)
 
 
 def op_restore8(c, dtype=None):
     """The tensor a checkpoint stands for, in its own type or in ``dtype``."""
-    if not isinstance(c, Checkpoint8):
+    if type(c) is not Checkpoint8:
         raise TypeError("op_restore8 takes a Checkpoint8")
-    return _fused.restore8(c.codes, c.scales, tuple(c.shape), c.dtype if dtype is None else dtype)
+    return _fused.restore8(c.buf, tuple(c.shape), c.dtype if dtype is None else dtype)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -76,12 +96,12 @@ def op_layer_norm(input, weight=None, bias=None, eps=1e-5, compress=True, seed=N
     pass; with a ``seed`` rounded stochastically) for the backward pass, else the input itself.  ``save`` False: forward
     only, saved is None.  A row whose mean is large against its deviation is better kept uncompressed: a code's step is
     1/127 to 1/64 of the largest magnitude of its 32 neighbours, mean included."""
-    y, kept, scales, stats, w = _fused.layer_norm(input, weight, bias, eps, compress, seed, save)
+    y, kept, stats, w = _fused.layer_norm(input, weight, bias, eps, compress, seed, save)
     if not save:
         return y, None
     param = weight if weight is not None else bias
     if compress:
-        kept = Checkpoint8(kept, scales, input.shape, input.dtype)
+        kept = Checkpoint8(kept, input.shape, input.dtype)
     return y, LayerNormSaved(kept, stats, w, input.shape, input.dtype, input.dtype if param is None else param.dtype)
 
 
@@ -91,9 +111,7 @@ def op_layer_norm_backward(grad_output, saved, needs=(True, True, True)):
         raise ValueError("grad_output must have shape %s, got %s" % (tuple(saved.shape), tuple(grad_output.shape)))
     if grad_output.dtype != saved.dtype:
         raise RuntimeError("The type of grad_output is not correct!")
-    x = saved.x
-    kept, scales = (x.codes, x.scales) if isinstance(x, Checkpoint8) else (x, None)
-    return _fused.layer_norm_backward(grad_output, kept, scales, saved.stats, saved.weight, saved.param_dtype == torch.float32, *needs)
+    return _fused.layer_norm_backward(grad_output, _unwrap(saved.x), saved.stats, saved.weight, saved.param_dtype == torch.float32, *needs)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -118,20 +136,20 @@ def op_linear(input, weight, bias=None, activation=None, residual=None, compress
     act = nv.ACT_CODE.get(activation)
     if act is None:
         raise ValueError("unknown activation %r" % (activation,))
-    codes = scales = None
+    given = None
     if checkpoint is not None:
-        if not isinstance(checkpoint, Checkpoint8):
+        if type(checkpoint) is not Checkpoint8:
             raise TypeError("checkpoint must be a Checkpoint8")
         if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
             raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
-        codes, scales = checkpoint.codes, checkpoint.scales
-    y, kept, xs, z, zs = _fused.linear(input, weight, bias, act, residual, compress, seed, save, codes, scales)
+        given = checkpoint.buf
+    y, kept, z = _fused.linear(input, weight, bias, act, residual, compress, seed, save, given)
     if not save:
         return y, None
     if compress:
-        kept = checkpoint if checkpoint is not None else Checkpoint8(kept, xs, input.shape, input.dtype)
+        kept = checkpoint if checkpoint is not None else Checkpoint8(kept, input.shape, input.dtype)
         if z is not None:
-            z = Checkpoint8(z, zs, y.shape, input.dtype)
+            z = Checkpoint8(z, y.shape, input.dtype)
     return y, LinearSaved(kept, z, weight, activation, y.shape, bias is not None)
 
 
@@ -140,8 +158,5 @@ def op_linear_backward(grad_output, saved, needs=(True, True, True)):
     The gradient of a residual is grad_output itself."""
     if grad_output.shape != saved.out_shape:
         raise ValueError("grad_output must have shape %s, got %s" % (tuple(saved.out_shape), tuple(grad_output.shape)))
-    x, z = saved.x, saved.z
-    kept, xs = (x.codes, x.scales) if isinstance(x, Checkpoint8) else (x, None)
-    z, zs = (z.codes, z.scales) if isinstance(z, Checkpoint8) else (z, None)
-    return _fused.linear_backward(grad_output, saved.weight, nv.ACT_CODE[saved.activation], kept, xs, z, zs, needs[0], needs[1],
+    return _fused.linear_backward(grad_output, saved.weight, nv.ACT_CODE[saved.activation], _unwrap(saved.x), _unwrap(saved.z), needs[0], needs[1],
                                   needs[2] and saved.has_bias)

@@ -39,54 +39,53 @@ def _keeps_graph(*tensors):
 
 
 def _flat(kept):
-    """(tensors, shape, dtype) of a Checkpoint8 or a tensor, for save_for_backward."""
-    if isinstance(kept, Checkpoint8):
-        return (kept.codes, kept.scales), kept.shape, kept.dtype
-    return (kept, None), None, None
+    """(tensor, shape, dtype) of a Checkpoint8 or a tensor (shape None), for save_for_backward."""
+    if type(kept) is Checkpoint8:
+        return kept.buf, kept.shape, kept.dtype
+    return kept, None, None
 
 
-def _unflat(a, b, shape, dtype):
-    return a if b is None else Checkpoint8(a, b, shape, dtype)
+def _unflat(t, shape, dtype):
+    return t if shape is None else Checkpoint8(t, shape, dtype)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, compress, seed):
         y, s = fused.op_layer_norm(x, weight, bias, eps, compress=compress, seed=seed)
-        (a, b), shape, dtype = _flat(s.x)
-        ctx.save_for_backward(a, b, s.stats, s.weight)
-        ctx.kept, ctx.meta = (shape, dtype), (s.shape, s.dtype, s.param_dtype)
+        t, *ctx.kept = _flat(s.x)
+        ctx.save_for_backward(t, s.stats, s.weight)
+        ctx.meta = (s.shape, s.dtype, s.param_dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        a, b, stats, weight = ctx.saved_tensors
-        saved = LayerNormSaved(_unflat(a, b, *ctx.kept), stats, weight, *ctx.meta)
+        t, stats, weight = ctx.saved_tensors
+        saved = LayerNormSaved(_unflat(t, *ctx.kept), stats, weight, *ctx.meta)
         n = ctx.needs_input_grad
         return (*fused.op_layer_norm_backward(dy, saved, (n[0], n[1], n[2])), None, None, None)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, compress, seed, codes, scales):
-        ck = None if codes is None else Checkpoint8(codes, scales, x.shape, x.dtype)
+    def forward(ctx, x, weight, bias, residual, activation, compress, seed, given):
+        ck = None if given is None else Checkpoint8(given, x.shape, x.dtype)
         y, s = fused.op_linear(x, weight, bias, activation, residual, compress=compress, seed=seed, checkpoint=ck)
-        (xa, xb), xshape, xdtype = _flat(s.x)
-        (za, zb), zshape, zdtype = _flat(s.z)
-        ctx.save_for_backward(xa, xb, za, zb, weight)
-        ctx.kept, ctx.meta = (xshape, xdtype, zshape, zdtype), (activation, s.out_shape, s.has_bias)
+        xt, *ctx.x = _flat(s.x)
+        zt, *ctx.z = _flat(s.z)
+        ctx.save_for_backward(xt, zt, weight)
+        ctx.meta = (activation, s.out_shape, s.has_bias)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xa, xb, za, zb, weight = ctx.saved_tensors
-        xshape, xdtype, zshape, zdtype = ctx.kept
-        saved = LinearSaved(_unflat(xa, xb, xshape, xdtype), _unflat(za, zb, zshape, zdtype), weight, *ctx.meta)
+        xt, zt, weight = ctx.saved_tensors
+        saved = LinearSaved(_unflat(xt, *ctx.x), _unflat(zt, *ctx.z), weight, *ctx.meta)
         n = ctx.needs_input_grad
         dx, dw, db = fused.op_linear_backward(dy, saved, (n[0], n[1], n[2]))
-        return dx, dw, db, (dy if n[3] else None), None, None, None, None, None
+        return dx, dw, db, (dy if n[3] else None), None, None, None, None
 
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
@@ -115,12 +114,12 @@ def linear(input, weight, bias=None, activation=None, residual=None, compress=No
     if not _keeps_graph(input, weight, bias, residual):
         return fused.op_linear(input, weight, bias, activation, residual, save=False)[0]
     compress = config.compress_activation if compress is None else compress
-    codes = scales = None
+    given = None
     if compress and checkpoint is not None:
         if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
             raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
-        codes, scales = checkpoint.codes, checkpoint.scales
-    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, codes, scales)
+        given = checkpoint.buf
+    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, given)
 
 
 class LayerNorm(nn.LayerNorm):

@@ -90,7 +90,8 @@ def test_python_refuses_host_tensors_and_wrong_arguments():
             call()
     with pytest.raises(TypeError):
         fused.op_restore8([x])
-    c = fused.Checkpoint8(torch.zeros(4, 32, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.int8), (4, 8), torch.bfloat16)
+    c = fused.Checkpoint8(torch.zeros(4 * 33, dtype=torch.int8), (4, 8), torch.bfloat16)
+    assert c.codes.shape == (4, 32) and c.scales.shape == (4, 1) and c.nbytes == 132
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         fused.op_restore8(c)
     with pytest.raises(RuntimeError, match="type"):
