@@ -317,8 +317,10 @@ static inline bool rows_aligned(const void* p, int64_t ld, int64_t cols, int ele
 }
 static inline int elem_bytes_of(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
 
-// out[c] = T(sum over p of partial[p * width + c]) in a fixed order; defined in layernorm.cu, shared by the operators
-// that reduce a bias or weight gradient over the rows.  Columns [0, n0) go to out0, [n0, n0 + n1) to out1 (null: skipped).
-int reduce_columns(const float* partial, int parts, int64_t width, void* out0, int64_t n0, void* out1, int64_t n1, int dtype, cudaStream_t s);
+// out[c] = T(sum over p of partial[p * width + c]) in a fixed order (`chains` sums, part p in sum p mod chains, then those in
+// order; 8 or 32); defined in layernorm.cu, shared by the operators that reduce a bias or weight gradient over the rows.
+// Columns [0, n0) go to out0; with out1, columns [0, width / 2) to out0 and the second half to out1 (null: skipped).
+constexpr int kSumChains = 8;                 // the chains of the linear layers' bias gradient, wherever it is finished
+int reduce_columns(const float* partial, int parts, int64_t width, void* out0, int64_t n0, void* out1, int64_t n1, int dtype, int chains, cudaStream_t s);
 
 }  // namespace gact

@@ -635,10 +635,10 @@ template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, int64
 }
 
 // ---- sums of partials over the blocks that wrote them ---------------------------------------------------------------
-constexpr int kRCols = 32, kRRows = 32;
+constexpr int kRCols = 32;
 struct ReduceArgs { const float* partial; int parts; int64_t width; void* out0; int64_t n0; void* out1; int64_t n1; };
 
-template <int DT>
+template <int DT, int kRRows>
 __global__ void __launch_bounds__(kRCols * kRRows) reduce_columns_kernel(const ReduceArgs a) {
     __shared__ float buf[kRRows][kRCols + 1];
     const int tx = threadIdx.x % kRCols, ty = threadIdx.x / kRCols;
@@ -678,13 +678,17 @@ __global__ void __launch_bounds__(kRCols * kRRows) reduce_columns_kernel(const R
     }
 }
 
-int reduce_columns(const float* partial, int parts, int64_t width, void* out0, int64_t n0, void* out1, int64_t n1, int dtype, cudaStream_t s) {
+template <int DT> static void launch_reduce(const ReduceArgs& a, int chains, cudaStream_t s) {
+    const unsigned blocks = (unsigned)((a.width + kRCols - 1) / kRCols);
+    if (chains == kSumChains) reduce_columns_kernel<DT, kSumChains><<<blocks, kRCols * kSumChains, 0, s>>>(a);
+    else reduce_columns_kernel<DT, 32><<<blocks, kRCols * 32, 0, s>>>(a);
+}
+int reduce_columns(const float* partial, int parts, int64_t width, void* out0, int64_t n0, void* out1, int64_t n1, int dtype, int chains, cudaStream_t s) {
     const ReduceArgs a{partial, parts, width, out0, n0, out1, n1};
-    const unsigned blocks = (unsigned)((width + kRCols - 1) / kRCols);
     switch (dtype) {
-    case GACT_F32: reduce_columns_kernel<GACT_F32><<<blocks, kRCols * kRRows, 0, s>>>(a); break;
-    case GACT_F16: reduce_columns_kernel<GACT_F16><<<blocks, kRCols * kRRows, 0, s>>>(a); break;
-    default: reduce_columns_kernel<GACT_BF16><<<blocks, kRCols * kRRows, 0, s>>>(a); break;
+    case GACT_F32: launch_reduce<GACT_F32>(a, chains, s); break;
+    case GACT_F16: launch_reduce<GACT_F16>(a, chains, s); break;
+    default: launch_reduce<GACT_BF16>(a, chains, s); break;
     }
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
@@ -776,5 +780,5 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
     if (st != GACT_OK || !params) return st;
     // both halves are summed; a gradient nobody asked for is not stored
     return reduce_columns((const float*)scratch, (int)blocks, 2 * (int64_t)a.width, dweight ? dweight : nullptr, dweight ? cols : 0,
-                          dbias ? dbias : dweight, dbias ? cols : 0, param_dtype, s);
+                          dbias ? dbias : dweight, dbias ? cols : 0, param_dtype, 32, s);
 }

@@ -109,7 +109,9 @@ template <int ACT> __device__ __forceinline__ float2 act_slope2(float2 z) {
         const float2 c = normal_cdf2(z, g);
         return fma2(mul2(z, splat2(0.39894228040143268f)), g, c);
     } else if constexpr (ACT == GACT_ACT_GELU_TANH) {
-        const float2 q = mul2(z, z);
+        // (z^2 is capped: where it would overflow, p (1 - p) is 0 and the product has to stay 0)
+        float2 q = mul2(z, z);
+        q = make_float2(q.x > 1e9f ? 1e9f : q.x, q.y > 1e9f ? 1e9f : q.y);
         const float2 p = sigmoid2(mul2(mul2(z, splat2(kTanhA)), fma2(q, splat2(0.044715f), splat2(1.0f))));
         const float2 r = mul2(mul2(z, p), fma2(p, splat2(-1.0f), splat2(1.0f)));
         return fma2(r, fma2(q, splat2(3.0f * 0.044715f * kTanhA), splat2(kTanhA)), p);
@@ -268,18 +270,23 @@ __device__ __forceinline__ void side_job(const SideJob& j, int w, int n) {
     const int lane = threadIdx.x & 31;
     constexpr int U = 8;
     if (j.partial) {
-        // 32 columns per warp, in the order of the parts
+        // 32 columns per warp; eight sums (part p goes to sum p mod 8), then those in order, as reduce_columns adds them
         for (int64_t c = (int64_t)w * 32 + lane; c - lane < j.n; c += (int64_t)n * 32) {
             if (c < j.n) {
-                float sum = 0.0f;
+                float v[kSumChains], sum;
+#pragma unroll
+                for (int i = 0; i < kSumChains; i++) v[i] = 0.0f;
                 const float* q = j.partial + c;
-                for (int p = 0; p < j.parts; p += 8, q += 8 * j.width) {
-                    float v[8];
+                for (int p = 0; p < j.parts; p += kSumChains, q += kSumChains * j.width) {
+                    float u[kSumChains];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = p + i < j.parts ? q[i * j.width] : 0.0f;
+                    for (int i = 0; i < kSumChains; i++) u[i] = p + i < j.parts ? q[i * j.width] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) sum += v[i];
+                    for (int i = 0; i < kSumChains; i++) v[i] += u[i];
                 }
+                sum = v[0];
+#pragma unroll
+                for (int i = 1; i < kSumChains; i++) sum += v[i];
                 ((T*)j.sums)[c] = Elem<DT>::from_float(sum);
             }
         }
@@ -625,8 +632,9 @@ struct Plan { int cg, bn, splits, per_split; int64_t tiles_m, tiles_n; double ns
 // Tile shape (two blocks on 256 x 256, one on 128 x 128 or 128 x 64) and splits of the reduction: the combination with the
 // least estimated time.  Measured on products of 16 to 8192 rows (nanoseconds): a launch with one stage takes `fixed`, every
 // further stage of a block `stage` (a stage moves 24 to 32 KB into an SM, which at these sizes is what takes the time), so the
-// busiest block's stages count; joining splits costs a second launch and the partial sums' way through L2.
-static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
+// busiest block's stages count; joining splits costs a second launch (with the linear epilogue a longer one) and the partial
+// sums' way through L2.
+static Plan plan_gemm(int64_t M, int64_t N, int64_t K, bool linear) {
     struct Shape { int cg, bn; double fixed, stage; };
     static const Shape shapes[3] = {{2, 256, 5600.0, 390.0}, {1, 128, 4400.0, 370.0}, {1, 64, 4100.0, 335.0}};
     const int sms = sm_count();
@@ -645,15 +653,15 @@ static Plan plan_gemm(int64_t M, int64_t N, int64_t K) {
             if (p.splits != splits || (splits > 1 && p.per_split < 2)) continue;
             const int64_t rounds = (tiles * splits + slots - 1) / slots;
             double t = h.fixed + (double)(rounds * p.per_split - 1) * h.stage;
-            if (splits > 1) t += 2800.0 + (double)(splits * 2 + 1) * (double)M * (double)N * 4.0 / 8000.0;
+            if (splits > 1) t += (linear ? 6000.0 : 2800.0) + (double)(splits * 2 + 1) * (double)M * (double)N * 4.0 / 8000.0;
             if (t < best_t) { best_t = t; best = p; best.ns = t; }
         }
     }
     return best;
 }
 
-static int64_t gemm_scratch(int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan_gemm(M, N, K);
+static int64_t gemm_scratch(int64_t M, int64_t N, int64_t K, bool linear) {
+    const Plan p = plan_gemm(M, N, K, linear);
     return p.splits > 1 ? (int64_t)p.splits * M * pitch8(N) * 4 : 0;
 }
 
@@ -682,7 +690,7 @@ static int launch_gemm_shape(const Plan& p, const CUtensorMap& ma, const CUtenso
 // C (M x N) = A B with the reduction over K.  A: K-major (M rows of K) or MN-major (K rows of M); B likewise with N.
 template <int DT, bool A_MN, bool B_MN, bool LINEAR>
 static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, GemmArgs a, void* scratch, cudaStream_t s) {
-    const Plan p = plan_gemm(a.M, a.N, K);
+    const Plan p = plan_gemm(a.M, a.N, K, LINEAR);
     CUtensorMap ma, mb;
     const bool ok = make_map(&ma, DT, A, A_MN ? K : a.M, A_MN ? a.M : K, lda, A_MN ? 64 : kBM) &&
                     make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn / p.cg);
@@ -900,7 +908,7 @@ using namespace gact;
 extern "C" int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t cout, int direction) {
     if (!dims_ok(rows, cin, cout) || direction < 0 || direction > 2) return -1;
     if (rows == 0) return 0;
-    return direction == 0 ? gemm_scratch(rows, cout, cin) : direction == 1 ? gemm_scratch(rows, cin, cout) : gemm_scratch(cout, cin, rows);
+    return direction == 0 ? gemm_scratch(rows, cout, cin, true) : direction == 1 ? gemm_scratch(rows, cin, cout, false) : gemm_scratch(cout, cin, rows, false);
 }
 
 static SideJob sums_job(const void* partial, int64_t rows, int64_t cols, void* sums) {
@@ -914,11 +922,11 @@ static SideJob sums_job(const void* partial, int64_t rows, int64_t cols, void* s
 // more than the launch; a restored x is free while it ends well before the product (8192 x 1024 beside 4096 -> 1024: 2 us
 // instead of 6.5; 8192 x 4096 beside 1024 -> 4096: 44 us instead of 18).
 static bool beside(int kind, int64_t M, int64_t N, int64_t K, int64_t elements) {
-    const Plan p = plan_gemm(M, N, K);
+    const Plan p = plan_gemm(M, N, K, kind == 1);
     const double blocks = (double)(p.tiles_m * p.tiles_n * p.splits * p.cg), sms = sm_count();
     const double pairs = blocks < sms ? blocks : sms, each = kind == 1 ? 14.0 : 20.0, all = kind == 1 ? 204.0 : 345.0;
-    const double alone = (double)elements / (each * pairs), ns = alone > (double)elements / all ? alone : (double)elements / all;
-    return ns <= 5000.0 || (kind == 2 && ns <= 0.75 * p.ns);
+    const double alone = (double)elements / (each * pairs), shared = (double)elements / all;
+    return (alone <= 5000.0 && shared <= 2000.0) || (kind == 2 && (alone > shared ? alone : shared) <= 0.75 * p.ns);
 }
 
 extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
@@ -932,7 +940,7 @@ extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int6
     if (!map_ok(x, ld_x) || !map_ok(weight, ld_w) || (((uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)residual) & 1) ||
         ((uintptr_t)zcodes & 31) || ((uintptr_t)xcodes & 31) || ((uintptr_t)scratch & 31))
         return GACT_ERR_ALIGN;
-    if (gemm_scratch(rows, cout, cin) && !scratch) return GACT_ERR_NULL;
+    if (gemm_scratch(rows, cout, cin, true) && !scratch) return GACT_ERR_NULL;
     GemmArgs a = {};
     a.M = rows; a.N = cout; a.out = y; a.ldo = cout; a.ovec = vec_bytes(y, cout);
     a.bias = bias;
@@ -963,7 +971,7 @@ extern "C" int gact_linear_dgrad(const void* dz, int64_t ld_dz, const void* weig
     if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
     if (!dims_ok(rows, cin, cout) || ld_dz < cout || ld_w < cin) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
-    if (!dz || !weight || !dx || (gemm_scratch(rows, cin, cout) && !scratch) || (!dbias_partial != !dbias) || (x_restored && (!xcodes || !xscales)))
+    if (!dz || !weight || !dx || (gemm_scratch(rows, cin, cout, false) && !scratch) || (!dbias_partial != !dbias) || (x_restored && (!xcodes || !xscales)))
         return GACT_ERR_NULL;
     if (!map_ok(dz, ld_dz) || !map_ok(weight, ld_w) || ((uintptr_t)dx & 1) || ((uintptr_t)dbias & 1) || ((uintptr_t)dbias_partial & 3) ||
         ((uintptr_t)xcodes & 31) || ((uintptr_t)x_restored & 15) || ((uintptr_t)scratch & 31))
@@ -997,7 +1005,7 @@ extern "C" int gact_linear_wgrad(const void* dz, int64_t ld_dz, const void* x, i
         if (dbias && cudaMemsetAsync(dbias, 0, (size_t)cout * 2, s) != cudaSuccess) return GACT_ERR_LAUNCH;
         return cudaMemsetAsync(dweight, 0, (size_t)(cin * cout * 2), s) == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
     }
-    if (!dz || !x || (gemm_scratch(cout, cin, rows) && !scratch) || (!dbias_partial != !dbias)) return GACT_ERR_NULL;
+    if (!dz || !x || (gemm_scratch(cout, cin, rows, false) && !scratch) || (!dbias_partial != !dbias)) return GACT_ERR_NULL;
     if (!map_ok(dz, ld_dz) || !map_ok(x, ld_x) || ((uintptr_t)dweight & 1) || ((uintptr_t)dbias & 1) || ((uintptr_t)dbias_partial & 3) ||
         ((uintptr_t)scratch & 31))
         return GACT_ERR_ALIGN;
@@ -1036,5 +1044,5 @@ extern "C" int gact_act_backward(const void* dy, int dtype, int64_t rows, int64_
     if (dtype == GACT_F16) dispatch_act_bwd<GACT_F16>(a, vec, grid, s);
     else dispatch_act_bwd<GACT_BF16>(a, vec, grid, s);
     if (cudaGetLastError() != cudaSuccess) return GACT_ERR_LAUNCH;
-    return dbias ? reduce_columns((const float*)scratch, (int)parts, a.width, dbias, cols, nullptr, 0, dtype, s) : GACT_OK;
+    return dbias ? reduce_columns((const float*)scratch, (int)parts, a.width, dbias, cols, nullptr, 0, dtype, kSumChains, s) : GACT_OK;
 }

@@ -144,7 +144,10 @@ class Linear(nn.Linear):
         self._shared = None
 
     def forward(self, input, residual=None):
-        checkpoint, self._shared = self._shared, None
+        shared, self._shared = self._shared, None
+        checkpoint = None
+        if shared is not None and shared[1] is input and shared[2] == input._version:
+            checkpoint = shared[0]
         return linear(input, self.weight, self.bias, self.activation, residual, checkpoint=checkpoint)
 
     def extra_repr(self):
@@ -153,17 +156,18 @@ class Linear(nn.Linear):
 
 def share_input(parent, children):
     """Lets linear layers that ``parent`` calls with its own first argument share one checkpoint of it (the query, key and
-    value layers of an attention block): made when ``parent`` is called, used by the next call of each child."""
+    value layers of an attention block): made when ``parent`` is called, used by the next call of each child that is given
+    that very tensor, unmodified, and dropped when ``parent`` returns."""
     children = list(children)
 
     def before(module, args):
         x = args[0] if args else None
         if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(x, *(c.weight for c in children)):
-            x = _autocast(x)[0]
-            if x.dtype in (torch.float16, torch.bfloat16):
-                ck = fused.op_checkpoint8(x.detach(), _next_seed())
+            cast = _autocast(x)[0]
+            if cast.dtype in (torch.float16, torch.bfloat16):
+                ck = fused.op_checkpoint8(cast.detach(), _next_seed())
                 for c in children:
-                    c._shared = ck
+                    c._shared = (ck, x, x._version)
 
     def after(module, args, output):
         for c in children:

@@ -343,3 +343,44 @@ def test_bert_workload_on_fused_layers():
         c.uninstall_hook()
         assert torch.isfinite(loss)
         assert all(torch.isfinite(p).all() for p in wl.model.parameters())
+
+
+@gpu
+def test_share_input_notices_another_tensor():
+    """A child that is given something else than the parent's argument (here: the argument changed in place, and a sum) keeps its
+    own checkpoint."""
+    from gact import layers
+
+    class Other(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a, self.b = layers.Linear(64, 64), layers.Linear(64, 64)
+
+        def forward(self, x):
+            return self.a(x + 1) + self.b(x)
+
+    torch.manual_seed(0)
+    m = Other().cuda().bfloat16()
+    x = rand(32, 64, seed=1)
+    grads = []
+    for share in (False, True):
+        if share:
+            layers.share_input(m, (m.a, m.b))
+        m.zero_grad()
+        m(x).float().square().sum().backward()
+        grads.append([p.grad.clone() for p in m.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@gpu
+def test_second_derivatives_are_refused_and_kept_graphs_work():
+    from gact import layers
+    x, w = rand(16, 32, seed=1).requires_grad_(), rand(8, 32, seed=2).requires_grad_()
+    y = layers.layer_norm(layers.linear(x, w, None, "gelu"))
+    a = torch.autograd.grad(y.float().square().sum(), [x, w], retain_graph=True)
+    b = torch.autograd.grad(y.float().square().sum(), [x, w])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    y = layers.linear(x, w)
+    (g,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
