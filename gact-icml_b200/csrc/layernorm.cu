@@ -200,6 +200,7 @@ struct LnBwdArgs {
     void* dx;                                          // null: weight gradients only
     float* partial;                                    // [gridDim][2 * width]: dw, db; null: no weight gradients
     int width;
+    uint32_t wait_limit; int withhold;                 // rings: bounded waits; diagnostics
 };
 
 // For short rows, few rows and rows that do not start on 16-byte boundaries.  A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
@@ -388,12 +389,12 @@ constexpr int kRingStages = 3;
 __device__ int g_norm_error = 0;
 
 struct RowRing {
-    uint32_t bar; volatile int* dead; uint32_t issued, taken;      // rows issued and taken so far
+    uint32_t bar, limit; volatile int* dead; uint32_t issued, taken;      // rows issued and taken so far
     __device__ __forceinline__ uint32_t stage(uint32_t n) const { return n % kRingStages; }
     // the next row to work on has landed; returns its stage
     __device__ __forceinline__ uint32_t take() {
         const uint32_t s = stage(taken);
-        mbar_wait(bar + 8 * s, (taken / kRingStages) & 1, dead);
+        mbar_wait(bar + 8 * s, (taken / kRingStages) & 1, limit, dead);
         taken++;
         return s;
     }
@@ -409,7 +410,7 @@ struct RowRing {
         if (!*dead) return;
         atomicExch(&g_norm_error, 1);
         for (uint32_t j = issued > (uint32_t)kRingStages ? issued - kRingStages : 0; j < issued; j++)
-            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(bar + 8 * (j % kRingStages), (j / kRingStages) & 1); i++) {}
+            mbar_drain(bar + 8 * (j % kRingStages), (j / kRingStages) & 1, limit);
     }
 };
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -446,14 +447,16 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    RowRing r{smem_addr(bars), &dead, 0, 0};
+    RowRing r{smem_addr(bars), a.wait_limit, &dead, 0, 0};
     const int64_t step = gridDim.x;
     int64_t row = blockIdx.x;
     const uint32_t ybytes = (uint32_t)a.cols * Elem<DT>::kBytes, xbytes = COMP ? (uint32_t)a.chunks * 8 : ybytes;
     auto issue = [&](int64_t w) {
-        if (w < a.rows) {
+        // (a ring that gave up issues nothing more: announcing bytes on a phase that never completed would be a second arrival
+        // on it, which faults)
+        if (w < a.rows && !dead) {
             const uint32_t s = r.announce(ybytes + xbytes), to = smem_addr(ring + s * ROW), bar = r.bar + 8 * s;
-            bulk_copy(to, (const T*)a.dy + w * a.ldy, ybytes, bar);
+            if (!(a.withhold && w == 0)) bulk_copy(to, (const T*)a.dy + w * a.ldy, ybytes, bar);      // (withhold: diagnostics)
             if (COMP) bulk_copy(to + YROW, a.codes + w * a.chunks * 8, xbytes, bar);
             else bulk_copy(to + YROW, (const T*)a.x + w * a.ldx, xbytes, bar);
         }
@@ -768,6 +771,8 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
     a.chunks = (int)(pitch8(cols) / 8); a.stats = stats; a.w = weight; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.dx = dx;
     a.partial = params ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
+    const PipelineHook hook = pipeline_hook();
+    a.wait_limit = hook.limit; a.withhold = hook.withhold;
     const int eb = elem_bytes_of(dtype);
     const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb));
     const int64_t blocks = ln_bwd_blocks(vec, rows, cols);

@@ -47,6 +47,7 @@ struct GemmArgs {
     float* partial;                           // [splits][M][pitchN] fp32
     int64_t ldp;
     SideJob side;
+    uint32_t wait_limit; int withhold;        // bounded waits; diagnostics
 };
 
 __device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
@@ -429,7 +430,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 const int m0 = (int)(x.m0 + rank * kBM), n0 = (int)(x.n0 + rank * R::kCols);
                 for (int k = x.k0; k < x.k1; k++, it++) {
                     const uint32_t s = it % S, ph = (it / S) & 1;
-                    if (!mbar_wait(empty + 8 * s, ph ^ 1, &dead)) break;
+                    if (!mbar_wait(empty + 8 * s, ph ^ 1, a.wait_limit, &dead)) break;
                     const uint32_t bar = full0 + 8 * s, da = ring + s * R::kStage, db = da + R::kA;
                     // block 0 announces the bytes of both (the other's may land first: the phase still waits for this arrival)
                     if (rank == 0) mbar_expect_tx(full + 8 * s, CG * R::kStage);
@@ -439,7 +440,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     } else {
                         tma_load_2d<CG>(da, &map_a, k * kBK, m0, bar);
                     }
-                    if (B_MN) {
+                    if (a.withhold && it == 0 && blockIdx.x == 0) {
+                        // (diagnostics: this stage never fills)
+                    } else if (B_MN) {
 #pragma unroll
                         for (int i = 0; i < R::kCols / 64; i++) tma_load_2d<CG>(db + i * 8192, &map_b, n0 + 64 * i, k * kBK, bar);
                     } else {
@@ -447,13 +450,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     }
                 }
             }
+            // the last stages have been read by the products, or the block gives up: then the copies that were issued (at most
+            // one per stage; block 0's barriers count both blocks') land before the blocks end
+            const uint32_t tail = it > (uint32_t)S ? it - S : 0;
+            for (uint32_t j = tail; j < it; j++) mbar_wait(empty + 8 * (j % S), (j / S) & 1, a.wait_limit, &dead);
             if (dead) {
-                // give up in order: the copies that were issued (at most one per stage; block 0's barriers count both blocks')
-                // land before the blocks end
                 atomicExch(&g_linear_error, 1);
                 if (rank == 0)
-                    for (uint32_t j = it > (uint32_t)S ? it - S : 0; j < it; j++)
-                        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full + 8 * (j % S), (j / S) & 1); i++) {}
+                    for (uint32_t j = tail; j < it; j++) mbar_drain(full + 8 * (j % S), (j / S) & 1, a.wait_limit);
             }
         }
         __syncwarp();
@@ -464,12 +468,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             for (int64_t u = first; u < units && !dead; u += stride, n++) {
                 const Unit x = unit_at<CG, BN>(a, u);
                 const uint32_t acc = n & 1;
-                if (!mbar_wait(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, &dead)) break;
+                if (!mbar_wait(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, a.wait_limit, &dead)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
                 for (int k = x.k0; k < x.k1; k++, it++) {
                     const uint32_t s = it % S, ph = (it / S) & 1;
-                    if (!mbar_wait(full + 8 * s, ph, &dead)) break;
+                    if (!mbar_wait(full + 8 * s, ph, a.wait_limit, &dead)) break;
                     tc_fence_after();
                     const uint32_t sa = ring + s * R::kStage, sb = sa + R::kA;
 #pragma unroll
@@ -484,7 +488,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
             // every product has finished before TMEM is given back
             mma_commit<CG>(drain);
-            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(drain, 0); i++) {}
+            mbar_drain(drain, 0, a.wait_limit);
         }
         __syncwarp();
     } else if (warp < 4) {
@@ -504,7 +508,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
             }
             // (a warp that gave up goes on through the tiles without storing: every warp meets every barrier)
-            const bool ok = mbar_wait(acc_full + 8 * acc, (n >> 1) & 1, &dead);
+            const bool ok = mbar_wait(acc_full + 8 * acc, (n >> 1) & 1, a.wait_limit, &dead);
             if (!__all_sync(kFull, ok)) continue;
             tc_fence_after();
             const int64_t row = x.m0 + rank * kBM + q * 32 + lane;
@@ -695,6 +699,8 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
     const bool ok = make_map(&ma, DT, A, A_MN ? K : a.M, A_MN ? a.M : K, lda, A_MN ? 64 : kBM) &&
                     make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn / p.cg);
     if (!ok) return GACT_ERR_LAUNCH;
+    const PipelineHook hook = pipeline_hook();
+    a.wait_limit = hook.limit; a.withhold = hook.withhold;
     a.ktiles = (int)((K + kBK - 1) / kBK);
     a.tiles_m = (int)p.tiles_m; a.tiles_n = (int)p.tiles_n; a.splits = p.splits; a.per_split = p.per_split;
     constexpr int kEpi = LINEAR ? kEpiLinear : kEpiStore;

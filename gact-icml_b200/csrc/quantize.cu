@@ -237,6 +237,12 @@ __global__ void __launch_bounds__(kQThreads) minimax_kernel(const void* x, int64
 // process-wide diagnostics knobs of the bulk-copy pipeline (gact_pipeline_test_hook)
 static std::atomic<uint32_t> g_wait_limit{1u << 20};
 static std::atomic<int> g_withhold_copy{0};
+// the knobs as the products and layer norm's rings use them (they poll 2^23 times by default: their waits span whole products)
+struct PipelineHook { uint32_t limit; int withhold; };
+PipelineHook pipeline_hook() {
+    const uint32_t n = g_wait_limit.load(std::memory_order_relaxed);
+    return {n == (1u << 20) ? (1u << 23) : n, g_withhold_copy.load(std::memory_order_relaxed)};
+}
 
 }  // namespace gact
 

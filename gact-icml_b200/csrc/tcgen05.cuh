@@ -25,17 +25,24 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Waits for a phase of a barrier, at most `kWaitLimit` polls.  A wait that runs out sets *dead (shared memory); every later
-// wait of the block then returns at once, so the block runs to its end without waiting for anything again.
+// Waits for a phase of a barrier, at most `limit` polls.  A wait that runs out sets *dead (shared memory); every later wait of
+// the block then returns at once, so the block runs to its end without waiting for anything again.
 constexpr uint32_t kWaitLimit = 1u << 23;
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* dead) {
+    for (uint32_t i = 0; i < limit; i++) {
         if (mbar_try(bar, parity)) return true;
         if (*dead) return false;
     }
     *dead = 1;
     return false;
 }
+// the same for copies that are still in flight when a block has given up
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint32_t limit) {
+    for (uint32_t i = 0; i < limit && !mbar_try(bar, parity); i++) {}
+}
+// what gact_pipeline_test_hook asks for (quantize.cu): the limit, and whether block 0 leaves its first copy unissued
+struct PipelineHook { uint32_t limit; int withhold; };
+PipelineHook pipeline_hook();
 
 // address of the same shared-memory variable in block `rank` of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {

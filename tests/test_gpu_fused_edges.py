@@ -235,14 +235,33 @@ def test_refusals_with_tensors_on_the_gpu():
 
 
 @gpu
-def test_wait_that_runs_out_is_reported_like_the_quantizers():
-    """The products and layer norm's rings share the sticky error word: clear when nothing ran out."""
+@pytest.mark.parametrize("what", ["pair of blocks", "one block", "ring"])
+def test_a_wait_that_runs_out_ends_the_launch_and_is_reported(what):
+    """With one copy withheld (the diagnostics switch of the quantizer's pipeline) the products and layer norm's rings give up
+    after the wait limit, record the error and end by themselves; after a reset the next call is right again."""
     from gact import _native as nv, fused
-    x = rand(2000, 2048)
-    y, s = fused.op_layer_norm(x)
-    fused.op_layer_norm_backward(y, s)
-    fused.op_linear(x, rand(64, 2048))
-    assert nv.lib.gact_pipeline_error() == 0 and nv.lib.gact_pipeline_error_reset() == 0
+    if what == "ring":
+        x = rand(2000, 2048)
+        _, s = fused.op_layer_norm(x)
+        call = lambda: fused.op_layer_norm_backward(x, s)
+    else:
+        x, w = (rand(2048, 1024), rand(2048, 1024, seed=1)) if what == "pair of blocks" else (rand(100, 256), rand(64, 256, seed=1))
+        call = lambda: fused.op_linear(x, w, save=False)[:1]
+    want = call()
+    torch.cuda.synchronize()
+    assert nv.lib.gact_pipeline_error() == 0
+    nv.lib.gact_pipeline_test_hook(2000, 1)
+    try:
+        call()
+        torch.cuda.synchronize()                                   # the launch finished on its own
+        assert nv.lib.gact_pipeline_error() > 0
+        with pytest.raises(nv.GactError):
+            nv.check_pipeline("test")                              # (clears the word)
+    finally:
+        nv.lib.gact_pipeline_test_hook(0, 0)
+        nv.lib.gact_pipeline_error_reset()
+    assert nv.lib.gact_pipeline_error() == 0
+    assert all(torch.equal(a, b) for a, b in zip(call(), want))
 
 
 @gpu
