@@ -922,17 +922,18 @@ static SideJob sums_job(const void* partial, int64_t rows, int64_t cols, void* s
     j.partial = (const float*)partial; j.parts = (int)act_bwd_parts(rows, cols); j.width = (cols + 7) / 8 * 8; j.sums = sums; j.n = cols;
     return j;
 }
-// Whether a side job beside a product is worth it.  Measured: a pair of idle warps makes 14 elements of a checkpoint or restores
-// 20 a nanosecond while it is alone on its SM; beside full epilogues and copies all of them together make 204, or restore 345.
+// Whether a side job beside a product is worth it.  Measured: a block's pair of idle warps makes 2 elements of a checkpoint or
+// restores 4 a nanosecond (64 x 1024 beside a single block: 32 us); beside full epilogues and copies all of them together make
+// 204, or restore 345.
 // A checkpoint beside the product slows its epilogue by more than the kernel of its own takes, except where it saves little
 // more than the launch; a restored x is free while it ends well before the product (8192 x 1024 beside 4096 -> 1024: 2 us
 // instead of 6.5; 8192 x 4096 beside 1024 -> 4096: 44 us instead of 18).
 static bool beside(int kind, int64_t M, int64_t N, int64_t K, int64_t elements) {
     const Plan p = plan_gemm(M, N, K, kind == 1);
     const double blocks = (double)(p.tiles_m * p.tiles_n * p.splits * p.cg), sms = sm_count();
-    const double pairs = blocks < sms ? blocks : sms, each = kind == 1 ? 14.0 : 20.0, all = kind == 1 ? 204.0 : 345.0;
+    const double pairs = blocks < sms ? blocks : sms, each = kind == 1 ? 2.0 : 4.0, all = kind == 1 ? 204.0 : 345.0;
     const double alone = (double)elements / (each * pairs), shared = (double)elements / all;
-    return (alone <= 5000.0 && shared <= 2000.0) || (kind == 2 && (alone > shared ? alone : shared) <= 0.75 * p.ns);
+    return (alone <= 4000.0 && shared <= 2000.0) || (kind == 2 && (alone > shared ? alone : shared) <= 0.75 * p.ns);
 }
 
 extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
