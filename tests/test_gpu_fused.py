@@ -385,6 +385,18 @@ def test_linear_epilogues(act, compress):
 
 
 @gpu
+@pytest.mark.parametrize("size", [(5, 3, 7), (70, 40, 33), (300, 1024, 2)])
+def test_linear_without_bias_and_with_odd_outputs(size):
+    """No activation and no bias: the gradient itself is the products' operand, copied to 16-byte rows where it has none."""
+    m, k, n = size
+    x, w, dy = inputs(m, k, dtype=torch.bfloat16, seed=1), inputs(n, k, dtype=torch.bfloat16, seed=2, std=0.1), inputs(m, n, dtype=torch.bfloat16, seed=3)
+    for compress in (True, False):
+        check_linear(x, w, None, None, None, dy, compress)
+        check_linear(x, w, None, "silu", None, dy, compress, (False, True, False))
+        check_linear(x, w, None, None, None, dy, compress, (True, False, False))
+
+
+@gpu
 def test_linear_strides_and_shapes():
     dt = torch.bfloat16
     big = inputs(90, 500, dtype=dt, seed=1)
