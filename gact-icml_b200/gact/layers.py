@@ -126,7 +126,9 @@ class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm that keeps its input in 8 bits."""
 
     def forward(self, input):
-        shape = self.normalized_shape
+        shape = tuple(self.normalized_shape)
+        if input.shape[-len(shape):] != shape:
+            raise RuntimeError("normalized_shape %s does not fit an input of shape %s" % (shape, tuple(input.shape)))
         if len(shape) == 1:
             return layer_norm(input, self.weight, self.bias, self.eps)
         x = input.flatten(-len(shape))

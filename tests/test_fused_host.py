@@ -121,6 +121,15 @@ def test_convert_on_the_host():
         m[0](torch.zeros(2, 4))
 
 
+@pytest.mark.parametrize("shape, size", [((5,), (3, 7)), ((4, 6), (2, 6, 4)), ((4, 6), (24,)), ((2, 3), (6, 2, 4)), ((1,), ())])
+def test_layer_norm_module_refuses_other_shapes(shape, size):
+    """As nn.LayerNorm does, with and without parameters: an equal number of elements is not enough."""
+    from gact import layers
+    for affine in (True, False):
+        with pytest.raises(RuntimeError, match="normalized_shape"):
+            layers.LayerNorm(shape, elementwise_affine=affine)(torch.zeros(size))
+
+
 def test_config_has_the_rounding_switch():
     import gact
     assert gact.config.stochastic_checkpoints is False
