@@ -101,7 +101,7 @@ def _autocast(*tensors):
     if not torch.is_autocast_enabled("cuda"):
         return tensors
     dt = torch.get_autocast_dtype("cuda")
-    return tuple(t if t is None or not t.is_floating_point() else t.to(dt) for t in tensors)
+    return tuple(t if t is None or not t.is_floating_point() or t.dtype == torch.float64 else t.to(dt) for t in tensors)
 
 
 def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None):

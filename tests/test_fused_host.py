@@ -130,6 +130,17 @@ def test_layer_norm_module_refuses_other_shapes(shape, size):
             layers.LayerNorm(shape, elementwise_affine=affine)(torch.zeros(size))
 
 
+def test_autocast_leaves_doubles_alone(monkeypatch):
+    """As torch does: they are refused, not lowered to 16 bits."""
+    from gact import layers
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device: True)
+    x = torch.zeros(2, 4, dtype=torch.float64)
+    assert [t if t is None else t.dtype for t in layers._autocast(x, x.float(), None, x.int())] == \
+        [torch.float64, torch.get_autocast_dtype("cuda"), None, torch.int32]
+    with pytest.raises(RuntimeError, match="float64"):
+        layers.Linear(4, 3)(x)
+
+
 def test_config_has_the_rounding_switch():
     import gact
     assert gact.config.stochastic_checkpoints is False
