@@ -549,6 +549,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 else mbar_arrive_cluster(acc_empty0 + 8 * acc);
             }
         }
+        // the last commit arrives in both blocks: block 1 too must have seen it before its shared memory may end (every other
+        // arrival from block 0 has been waited for above).  One thread that is through its tiles waits, so the bound counts from there.
+        if constexpr (CG == 2)
+            if (rank == 1 && warp == 4 && lane == 0) mbar_drain(drain, 0, a.wait_limit);
     }
     __syncwarp();
     tc_fence_before();
