@@ -70,22 +70,27 @@ class _LayerNorm(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, compress, seed, given):
+        # Under autocast the parameters are cast here and again in backward: what is saved is the parameter itself, which hooks
+        # know and leave alone.  (A copy that requires a gradient looks like an activation to them and would be quantized.)
+        w, b = _autocast(weight, bias)
         ck = None if given is None else Checkpoint8(given, x.shape, x.dtype)
-        y, s = fused.op_linear(x, weight, bias, activation, residual, compress=compress, seed=seed, checkpoint=ck)
+        y, s = fused.op_linear(x, w, b, activation, residual, compress=compress, seed=seed, checkpoint=ck)
         xt, *ctx.x = _flat(s.x)
         zt, *ctx.z = _flat(s.z)
         ctx.save_for_backward(xt, zt, weight)
         ctx.meta = (activation, s.out_shape, s.has_bias)
+        ctx.param_dtypes = weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xt, zt, weight = ctx.saved_tensors
-        saved = LinearSaved(_unflat(xt, *ctx.x), _unflat(zt, *ctx.z), weight, *ctx.meta)
+        saved = LinearSaved(_unflat(xt, *ctx.x), _unflat(zt, *ctx.z), weight.to(dy.dtype), *ctx.meta)
         n = ctx.needs_input_grad
         dx, dw, db = fused.op_linear_backward(dy, saved, (n[0], n[1], n[2]))
-        return dx, dw, db, (dy if n[3] else None), None, None, None, None
+        wt, bt = ctx.param_dtypes
+        return dx, None if dw is None else dw.to(wt), None if db is None else db.to(bt), (dy if n[3] else None), None, None, None, None
 
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
@@ -107,12 +112,12 @@ def _autocast(*tensors):
 def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None):
     """activation(input W^T + bias) + residual, differentiable; see ``gact.fused.op_linear``.  ``compress`` as in
     ``layer_norm``; ``checkpoint``: a Checkpoint8 of the input (in the type it is computed in) to share."""
-    input, weight, bias, residual = _autocast(input, weight, bias, residual)
+    input, residual = _autocast(input, residual)
     if input.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("gact.layers.linear computes in float16 or bfloat16: cast the model or use torch.autocast "
                            "(got an input of %s)" % input.dtype)
     if not _keeps_graph(input, weight, bias, residual):
-        return fused.op_linear(input, weight, bias, activation, residual, save=False)[0]
+        return fused.op_linear(input, *_autocast(weight, bias), activation, residual, save=False)[0]
     compress = config.compress_activation if compress is None else compress
     given = None
     if compress and checkpoint is not None:

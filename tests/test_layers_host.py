@@ -1,0 +1,68 @@
+"""gact.layers without a GPU: what the autograd functions hand to autograd and to the operators, with plain stand-ins for the
+operators of gact.fused."""
+import pytest
+import torch
+
+from gact import fused, layers
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    """op_linear and its backward pass in plain torch on the host; collects the keyword arguments of each call."""
+    calls = []
+
+    def op_linear(input, weight, bias=None, activation=None, residual=None, compress=True, seed=None, save=True, checkpoint=None, **kw):
+        assert weight.dtype == input.dtype and (bias is None or bias.dtype == input.dtype)
+        assert residual is None or residual.dtype == input.dtype
+        calls.append(dict(kw, save=save, checkpoint=checkpoint, compress=compress, seed=seed, residual=residual is not None))
+        y = torch.nn.functional.linear(input.float(), weight.float(), None if bias is None else bias.float())
+        y = (y if residual is None else y + residual.float()).to(input.dtype)
+        if not save:
+            return y, None
+        kept = fused.Checkpoint8(torch.zeros(1, dtype=torch.int8), input.shape, input.dtype) if compress else input
+        return y, fused.LinearSaved(kept if kw.get("keep_input", True) else None, None, weight, activation, y.shape, bias is not None)
+
+    def op_linear_backward(dy, saved, needs=(True, True, True)):
+        assert saved.weight is None or saved.weight.dtype == dy.dtype
+        return tuple(None if not n else dy @ saved.weight if i == 0 else torch.ones(dy.shape[-1], saved.x.shape[-1], dtype=dy.dtype) if i == 1
+                     else dy.sum(0) for i, n in enumerate(needs))
+
+    monkeypatch.setattr(fused, "op_linear", op_linear)
+    monkeypatch.setattr(fused, "op_linear_backward", op_linear_backward)
+    return calls
+
+
+@pytest.fixture
+def autocast(monkeypatch):
+    """Autocast of CUDA tensors to bfloat16, as the layers see it."""
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device: True)
+    monkeypatch.setattr(torch, "get_autocast_dtype", lambda device: torch.bfloat16)
+
+
+def saved_by(call):
+    seen = []
+
+    def pack(t):
+        seen.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = call()
+    return out, seen
+
+
+@pytest.mark.parametrize("compress", [True, False])
+def test_under_autocast_the_parameters_themselves_are_saved(plain, autocast, compress):
+    """Saved-tensor hooks know a parameter by its address; a cast copy that requires a gradient they would quantize."""
+    m = layers.Linear(8, 4)
+    x = torch.randn(5, 8, requires_grad=True)
+    y, seen = saved_by(lambda: layers.linear(x, m.weight, m.bias, compress=compress))
+    address = {p.data_ptr() for p in m.parameters()}
+    strange = [t for t in seen if t.is_floating_point() and t.requires_grad and t.data_ptr() not in address]
+    # (without compression the input in the computed type is an activation like any other)
+    assert [tuple(t.shape) for t in strange] == ([] if compress else [(5, 8)])
+    assert any(t.data_ptr() == m.weight.data_ptr() for t in seen)
+    y.float().sum().backward()
+    assert y.dtype == torch.bfloat16 and x.grad.dtype == m.weight.grad.dtype == m.bias.grad.dtype == torch.float32
+    want = torch.ones(5, 4, dtype=torch.bfloat16) @ m.weight.detach().bfloat16()
+    assert torch.equal(x.grad, want.float())
