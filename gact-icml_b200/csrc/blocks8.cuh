@@ -113,6 +113,11 @@ template <int DT> __device__ __forceinline__ void pairs_to_raw(const float2 (&v)
         else raw[i] = pack2<DT>(v[i].x, v[i].y);
     }
 }
+// the larger of m and two magnitudes; NaN if there is one
+__device__ __forceinline__ float absmax3(float m, float2 v) {
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v.x), "f"(v.y));
+    return m;
+}
 // the largest magnitude of the eight, as an fp32 bit pattern
 template <int DT> __device__ __forceinline__ uint32_t absmax8(const uint32_t (&raw)[RawRegs<DT>::N]) {
     uint32_t m;
@@ -135,9 +140,10 @@ template <int DT> __device__ __forceinline__ uint32_t absmax8(const uint32_t (&r
 }
 
 // The codes of 8 consecutive elements (chunk number `chunk` of the padded rows); a block of 32 lies in 4 neighbouring
-// lanes and every lane of the warp must call.  `m`: the lane's largest magnitude.  Returns the scale byte too.
-template <int DT, bool STOCH>
-__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const PhiloxKeys& rk, uint64_t chunk, uint32_t& byte) {
+// lanes and every lane of the warp must call.  `m`: the lane's largest magnitude; `last`: top_byte8 of the type that the codes
+// are restored to.  Returns the scale byte too.
+template <bool STOCH>
+__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const PhiloxKeys& rk, uint64_t chunk, uint32_t& byte, uint32_t last) {
     m = max(m, __shfl_xor_sync(kFull, m, 1));
     m = max(m, __shfl_xor_sync(kFull, m, 2));
     byte = scale_byte8(m);
@@ -159,7 +165,7 @@ __device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const 
         }
     }
     uint2 w = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-    if (byte >= top_byte8<DT>()) {
+    if (byte >= last) {
         if (byte == 255u) w = make_uint2(0u, 0u);
         else w = make_uint2(clamp_codes63(w.x), clamp_codes63(w.y));
     }

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kCThreads) checkpoint8_kernel(const __grid_con
         float2 v[4];
         raw_to_pairs<DT>(raw[u], v);
         uint32_t byte;
-        const uint2 c = codes8<DT, STOCH>(v, absmax8<DT>(raw[u]), a.rk, (uint64_t)w.chunk[u], byte);
+        const uint2 c = codes8<STOCH>(v, absmax8<DT>(raw[u]), a.rk, (uint64_t)w.chunk[u], byte, top_byte8<DT>());
         if (w.chunk[u] >= 0) {
             st_stream_u2(a.codes + w.chunk[u] * 8, c);
             if ((threadIdx.x & 3) == 0) a.scales[w.chunk[u] >> 2] = (uint8_t)byte;

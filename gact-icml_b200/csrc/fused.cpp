@@ -230,15 +230,15 @@ at::ScalarType param_type(const Tensor& w, const Tensor& b, int64_t cols, const 
     return t;
 }
 
-// layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, checkpoint or input, statistics, weight)
+// layer_norm(input, weight, bias, eps, compress, seed, save, center) -> (y, checkpoint or input, statistics, weight)
 PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 7);
+    count_args(nargs, 8);
     const Tensor x = tensor_arg(args[0], "input");
     Tensor w = optional_arg(args[1], "weight"), b = optional_arg(args[2], "bias");
     const double eps = PyFloat_AsDouble(args[3]);
     if (PyErr_Occurred()) throw python_error();
-    const bool compress = bool_arg(args[4]), save = bool_arg(args[6]);
+    const bool compress = bool_arg(args[4]), save = bool_arg(args[6]), center = bool_arg(args[7]);
     const Seed seed = seed_arg(args[5]);
     check_tensor(x, "input", false, nullptr);
     TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
@@ -259,7 +259,8 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (r.rows > 0) {
         check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(),
-                              (float*)ptr(stats), c.codes(), c.scales(), seed.stochastic, seed.value, stream_of(x)),
+                              (float*)ptr(stats), c.codes(), c.scales(),
+                              (seed.stochastic ? GACT_CODES_STOCHASTIC : 0) | (center ? GACT_CODES_CENTERED : 0), seed.value, stream_of(x)),
               "gact_layer_norm");
         g_launches++;
     }
@@ -473,7 +474,7 @@ PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launc
 PyMethodDef kMethods[] = {
     {"checkpoint8", FAST(py_checkpoint8), "checkpoint8(input, seed) -> buffer"},
     {"restore8", FAST(py_restore8), "restore8(buffer, shape, dtype) -> tensor"},
-    {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save) -> (y, kept, statistics, weight)"},
+    {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save, center) -> (y, kept, statistics, weight)"},
     {"layer_norm_backward", FAST(py_layer_norm_backward),
      "layer_norm_backward(grad_output, kept, statistics, weight, fp32 parameters, need_input, need_weight, need_bias) -> three gradients"},
     {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, checkpoint) -> (y, kept, z)"},

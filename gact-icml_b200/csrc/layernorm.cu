@@ -2,6 +2,8 @@
 //
 //   mean = sum(x) / H,  r = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) r w + b
 //   x^ = (x' - mean) r with x' the kept input (restored codes, or x itself),  g = dy w
+//   centred codes keep x - mean instead:  x^ = x' r.  Half a code's step is then at most 1/127 of the largest deviation from the
+//   mean; that of x grows with the mean, and seen through r it has no bound (rows of 100 +- 1: dw 28 % off, centred 0.8 %)
 //   dx = r (g - sum(g)/H - x^ sum(g x^)/H),  dw = sum over rows of dy x^,  db = sum over rows of dy
 //
 // Both passes are bound by HBM: forward reads x and writes y and 33/32 bytes of codes per element, backward reads dy and
@@ -19,8 +21,8 @@ struct LnArgs {
     const void* w; const void* b; int wf32;          // weight / bias in fp32 (else in the type of x); null: 1 and 0
     int64_t rows; int cols; float inv_cols; float eps;
     void* y;
-    float* stats;                                    // (mean, 1 / deviation) per row, or null
-    int8_t* codes; uint8_t* scales; int chunks; int stochastic; PhiloxKeys rk;
+    float* stats;                                    // (mean, or 0 with `center`; 1 / deviation) per row, or null
+    int8_t* codes; uint8_t* scales; int chunks; int stochastic, center; PhiloxKeys rk;
 };
 
 // 8 weights starting at column `col` (fp32 or the type of x); `none` without a weight, 0 past the end
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
         float2 s2 = splat2(0.0f);
 #pragma unroll
         for (int c = 0; c < CH; c++) s2 = add2(s2, add2(add2(v[c][0], v[c][1]), add2(v[c][2], v[c][3])));
-        const float mean = row_sum(s2.x + s2.y, buf[phase][0]) * a.inv_cols;
+        float mean = row_sum(s2.x + s2.y, buf[phase][0]) * a.inv_cols;
         float2 q2 = splat2(0.0f);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
@@ -123,7 +125,31 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
         // rsqrtf: at most 2 steps off
         const float rstd = rsqrtf(row_sum(q2.x + q2.y, buf[phase][1]) * a.inv_cols + a.eps);
         const bool live = row < a.rows;
-        if (live && t == 0 && a.stats) ((float2*)a.stats)[row] = make_float2(mean, rstd);
+        uint32_t last = top_byte8<DT>();
+        // what the backward pass has to take off the kept values, and 1 / deviation: centred codes have lost the mean already
+        if (live && t == 0 && a.stats) ((float2*)a.stats)[row] = make_float2(a.center ? 0.0f : mean, rstd);
+        if (a.center) {
+            // (in place: what follows is written for the deviations and a mean of 0; they are fp32 and restored as such, so the
+            // range of x's type does not bound them)
+            last = top_byte8<GACT_F32>();
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                const int col = (t + c * TPR) * 8;
+                float m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[c][i] = add2(v[c][i], splat2(-mean));
+                    if (VEC) { if (col >= a.cols) v[c][i] = splat2(0.0f); }
+                    else {
+                        if (col + 2 * i >= a.cols) v[c][i].x = 0.0f;
+                        if (col + 2 * i + 1 >= a.cols) v[c][i].y = 0.0f;
+                    }
+                    m = absmax3(m, v[c][i]);
+                }
+                top[c] = __float_as_uint(m) & 0x7fffffffu;
+            }
+            mean = 0.0f;
+        }
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int col = (t + c * TPR) * 8;
@@ -131,7 +157,7 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
             if (a.codes) {
                 uint32_t byte;
                 const uint64_t chunk = (uint64_t)row * a.chunks + (t + c * TPR);
-                const uint2 q = a.stochastic ? codes8<DT, true>(v[c], top[c], a.rk, chunk, byte) : codes8<DT, false>(v[c], top[c], a.rk, chunk, byte);
+                const uint2 q = a.stochastic ? codes8<true>(v[c], top[c], a.rk, chunk, byte, last) : codes8<false>(v[c], top[c], a.rk, chunk, byte, last);
                 if (live && t + c * TPR < a.chunks) {
                     st_stream_u2(a.codes + chunk * 8, q);
                     if ((t & 3) == 0) a.scales[chunk >> 2] = (uint8_t)byte;
@@ -717,11 +743,12 @@ static bool param_ok(const void* p, int dtype) { return !p || ((uintptr_t)p & (u
 using namespace gact;
 
 extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight, const void* bias,
-                               int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int stochastic,
+                               int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int rounding,
                                uint64_t seed, void* stream) {
     if (dtype < GACT_F32 || dtype > GACT_BF16 || (param_dtype != dtype && param_dtype != GACT_F32)) return GACT_ERR_DTYPE;
     if (!ln_sizes_ok(rows, cols) || ld < cols) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
+    if (rounding & ~(GACT_CODES_STOCHASTIC | GACT_CODES_CENTERED)) return GACT_ERR_MODE;
     if (!x || !y || (codes && !scales)) return GACT_ERR_NULL;
     const uintptr_t em = (uintptr_t)(elem_bytes_of(dtype) - 1);
     if (((uintptr_t)x & em) || ((uintptr_t)y & em) || ((uintptr_t)codes & 31) || ((uintptr_t)stats & 7) || !param_ok(weight, param_dtype) ||
@@ -731,7 +758,8 @@ extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t c
     a.x = x; a.ldx = ld; a.w = weight; a.b = bias; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.eps = (float)eps;
     a.y = y; a.stats = stats; a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales;
-    a.chunks = (int)(pitch8(cols) / 8); a.stochastic = stochastic; a.rk = philox_round_keys(seed);
+    a.chunks = (int)(pitch8(cols) / 8); a.rk = philox_round_keys(seed);
+    a.stochastic = (rounding & GACT_CODES_STOCHASTIC) != 0; a.center = codes && (rounding & GACT_CODES_CENTERED);
     const bool vec = rows_aligned(x, ld, cols, elem_bytes_of(dtype)) && rows_aligned(y, cols, cols, elem_bytes_of(dtype));
     cudaStream_t s = (cudaStream_t)stream;
     switch (dtype) {

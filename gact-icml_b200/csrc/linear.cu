@@ -217,7 +217,7 @@ __device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row
         // columns past N are zero: their weights and biases are
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i].x), "f"(v[i].y));
+        for (int i = 0; i < 16; i++) m = absmax3(m, v[i]);
         const uint32_t byte = scale_byte8(__float_as_uint(m) & 0x7fffffffu);
         const float up = scale_up8(byte);
         const uint64_t at = (uint64_t)row * a.zpitch + n;
@@ -324,7 +324,7 @@ __device__ __forceinline__ void side_job(const SideJob& j, int w, int n) {
                 raw_to_pairs<DT>(raw[u], v);
                 uint32_t byte;
                 const uint32_t m = absmax8<DT>(raw[u]);
-                const uint2 q = j.stochastic ? codes8<DT, true>(v, m, j.rk, (uint64_t)i, byte) : codes8<DT, false>(v, m, j.rk, (uint64_t)i, byte);
+                const uint2 q = j.stochastic ? codes8<true>(v, m, j.rk, (uint64_t)i, byte, top_byte8<DT>()) : codes8<false>(v, m, j.rk, (uint64_t)i, byte, top_byte8<DT>());
                 if (i < total) {
                     st_stream_u2(j.codes + i * 8, q);
                     if ((lane & 3) == 0) j.scales[i >> 2] = (uint8_t)byte;

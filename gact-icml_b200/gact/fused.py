@@ -80,8 +80,8 @@ def op_restore8(c, dtype=None):
 # layer norm
 # ---------------------------------------------------------------------------------------------------------------
 class LayerNormSaved:
-    """What layer norm's backward pass needs: the input (a Checkpoint8, or the tensor itself), the row statistics
-    (mean and 1 / deviation, fp32 (rows, 2)) and the weight."""
+    """What layer norm's backward pass needs: the input (a Checkpoint8 of it or of its deviation from the rows' means, or the
+    tensor itself), per row what is still to be taken off (the mean, or 0) and 1 / deviation (fp32 (rows, 2)), and the weight."""
     __slots__ = ("x", "stats", "weight", "shape", "dtype", "param_dtype")
 
     def __init__(self, x, stats, weight, shape, dtype, param_dtype):
@@ -89,19 +89,21 @@ class LayerNormSaved:
         self.shape, self.dtype, self.param_dtype = shape, dtype, param_dtype
 
 
-def op_layer_norm(input, weight=None, bias=None, eps=1e-5, compress=True, seed=None, save=True):
+def op_layer_norm(input, weight=None, bias=None, eps=1e-5, compress=True, seed=None, save=True, center=False):
     """(y, saved): layer norm over the last dimension (at most 16384) of a float32 / float16 / bfloat16 tensor.
 
     weight, bias: of the input's type or float32, or None.  ``compress``: keep the input as a Checkpoint8 (made in the same
     pass; with a ``seed`` rounded stochastically) for the backward pass, else the input itself.  ``save`` False: forward
-    only, saved is None.  A row whose mean is large against its deviation is better kept uncompressed: a code's step is
-    1/127 to 1/64 of the largest magnitude of its 32 neighbours, mean included."""
-    y, kept, stats, w = _fused.layer_norm(input, weight, bias, eps, compress, seed, save)
+    only, saved is None.  ``center``: the checkpoint is that of the input minus its row's mean, and its error stays below 1/127
+    of the row's largest deviation.  Codes of the input itself (which other operators can share) have a step of 1/127 to
+    1/64 of the largest magnitude of 32 neighbours, mean included: where a row's mean is large against its deviation they
+    leave the gradients little to work from."""
+    y, kept, stats, w = _fused.layer_norm(input, weight, bias, eps, compress, seed, save, center)
     if not save:
         return y, None
     param = weight if weight is not None else bias
     if compress:
-        kept = Checkpoint8(kept, input.shape, input.dtype)
+        kept = Checkpoint8(kept, input.shape, torch.float32 if center else input.dtype)
     return y, LayerNormSaved(kept, stats, w, input.shape, input.dtype, input.dtype if param is None else param.dtype)
 
 

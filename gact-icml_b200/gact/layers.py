@@ -52,7 +52,7 @@ def _unflat(t, shape, dtype):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, compress, seed):
-        y, s = fused.op_layer_norm(x, weight, bias, eps, compress=compress, seed=seed)
+        y, s = fused.op_layer_norm(x, weight, bias, eps, compress=compress, seed=seed, center=True)
         t, *ctx.kept = _flat(s.x)
         ctx.save_for_backward(t, s.stats, s.weight)
         ctx.meta = (s.shape, s.dtype, s.param_dtype)
@@ -95,7 +95,7 @@ class _Linear(torch.autograd.Function):
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
     """Layer norm over the last dimension, differentiable; what it keeps is decided by ``compress`` (None: by the level,
-    ``config.compress_activation``)."""
+    ``config.compress_activation``): the checkpoint of the input minus its row's mean, or the input itself."""
     if not _keeps_graph(input, weight, bias):
         return fused.op_layer_norm(input, weight, bias, eps, save=False)[0]
     compress = config.compress_activation if compress is None else compress

@@ -252,6 +252,9 @@ int gact_calc_precision_host(int32_t* b, const float* C, const int64_t* w, int L
 #define GACT_MAX_ELEMENTS (1LL << 38)
 #define GACT_LAYER_NORM_MAX_COLS 16384
 
+/* how gact_layer_norm makes its codes */
+enum { GACT_CODES_STOCHASTIC = 1, GACT_CODES_CENTERED = 4 };
+
 /* activations of gact_linear; GELU is the erf form, GELU_TANH its tanh approximation */
 enum { GACT_ACT_NONE = 0, GACT_ACT_RELU = 1, GACT_ACT_GELU = 2, GACT_ACT_GELU_TANH = 3, GACT_ACT_SILU = 4 };
 
@@ -268,9 +271,12 @@ int gact_repitch16(const void* src, int64_t ld, int64_t rows, int64_t cols, void
  * Layer norm over rows of `cols`: y = (x - mean) / sqrt(var + eps) * weight + bias; weight / bias may be null, their type
  * is `param_dtype` (that of x, or GACT_F32).  y is contiguous.  stats (optional, 8-byte aligned): (mean, 1 / deviation)
  * per row in fp32, for the backward pass.  codes / scales (optional): checkpoint of x, made in the same pass.
+ * rounding: 0, or GACT_CODES_STOCHASTIC, and with GACT_CODES_CENTERED the codes are those of x - mean (an fp32 tensor) and
+ * stats hold (0, 1 / deviation): what the backward pass takes off the kept values.  Codes of x itself are as coarse as the
+ * largest |x| of their block; in rows whose mean is large against their deviation that leaves little of x - mean.
  */
 int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* weight, const void* bias,
-                    int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int stochastic, uint64_t seed,
+                    int param_dtype, double eps, void* y, float* stats, void* codes, void* scales, int rounding, uint64_t seed,
                     void* stream);
 /*
  * Its backward pass from x, or (x null) from the checkpoint of x.  dx (contiguous), dweight, dbias: each may be null.

@@ -39,6 +39,21 @@ def autocast(monkeypatch):
     monkeypatch.setattr(torch, "get_autocast_dtype", lambda device: torch.bfloat16)
 
 
+def test_layer_norm_keeps_the_checkpoint_of_its_deviations(monkeypatch):
+    """Codes of the input itself would lose rows whose mean is large against their deviation."""
+    seen = []
+
+    def op_layer_norm(input, weight=None, bias=None, eps=1e-5, compress=True, seed=None, save=True, center=False):
+        seen.append((compress, center))
+        kept = fused.Checkpoint8(torch.zeros(1, dtype=torch.int8), input.shape, input.dtype) if compress else input
+        return input * 1, fused.LayerNormSaved(kept, torch.zeros(2, 2), weight, input.shape, input.dtype, input.dtype)
+
+    monkeypatch.setattr(fused, "op_layer_norm", op_layer_norm)
+    layers.LayerNorm(4)(torch.zeros(2, 4))
+    layers.layer_norm(torch.zeros(2, 4, requires_grad=True))
+    assert seen == [(True, True)] * 2
+
+
 def saved_by(call):
     seen = []
 
@@ -66,3 +81,12 @@ def test_under_autocast_the_parameters_themselves_are_saved(plain, autocast, com
     assert y.dtype == torch.bfloat16 and x.grad.dtype == m.weight.grad.dtype == m.bias.grad.dtype == torch.float32
     want = torch.ones(5, 4, dtype=torch.bfloat16) @ m.weight.detach().bfloat16()
     assert torch.equal(x.grad, want.float())
+
+
+def test_layer_norm_refuses_unknown_ways_of_rounding():
+    import ctypes
+    from gact import _native as nv
+    b = ctypes.create_string_buffer(1 << 12)
+    p = (ctypes.addressof(b) + 255) & ~255
+    for rounding, status in ((2, 6), (8, 6), (-1, 6)):
+        assert nv.lib.gact_layer_norm(p, 2, 2, 32, 32, p, p, 2, 1e-5, p, p, p, p, rounding, 0, None) == status
