@@ -29,6 +29,11 @@ static inline int sm_count() {
     return n;
 }
 
+// What gact_pipeline_test_hook asks for (quantize.cu): the limit of a pipeline's waits, or the pipeline's own default, and whether
+// block 0 leaves its first copy unissued.
+struct PipelineHook { uint32_t limit; int withhold; };
+PipelineHook pipeline_hook(uint32_t default_limit);
+
 // ---------------------------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon et al., SC'11).  Ten rounds; round r uses the key bumped r times by the Weyl
 // constants.  The 20 round keys depend only on the seed, so the host computes them once per launch and they

@@ -801,7 +801,7 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
     a.chunks = (int)(pitch8(cols) / 8); a.stats = stats; a.w = weight; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.dx = dx;
     a.partial = params ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
-    const PipelineHook hook = pipeline_hook();
+    const PipelineHook hook = pipeline_hook(kWaitLimit);
     a.wait_limit = hook.limit; a.withhold = hook.withhold;
     const int eb = elem_bytes_of(dtype);
     const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb));

@@ -709,7 +709,7 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
     const bool ok = make_map(&ma, DT, A, A_MN ? K : a.M, A_MN ? a.M : K, lda, A_MN ? 64 : kBM) &&
                     make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn / p.cg);
     if (!ok) return GACT_ERR_LAUNCH;
-    const PipelineHook hook = pipeline_hook();
+    const PipelineHook hook = pipeline_hook(kWaitLimit);
     a.wait_limit = hook.limit; a.withhold = hook.withhold;
     a.ktiles = (int)((K + kBK - 1) / kBK);
     a.tiles_m = (int)p.tiles_m; a.tiles_n = (int)p.tiles_n; a.splits = p.splits; a.per_split = p.per_split;

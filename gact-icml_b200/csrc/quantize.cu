@@ -234,14 +234,12 @@ __global__ void __launch_bounds__(kQThreads) minimax_kernel(const void* x, int64
     }
 }
 
-// process-wide diagnostics knobs of the bulk-copy pipeline (gact_pipeline_test_hook)
-static std::atomic<uint32_t> g_wait_limit{1u << 20};
+// process-wide diagnostics knobs of the pipelines (gact_pipeline_test_hook); limit 0: each pipeline's own default
+static std::atomic<uint32_t> g_wait_limit{0};
 static std::atomic<int> g_withhold_copy{0};
-// the knobs as the products and layer norm's rings use them (they poll 2^23 times by default: their waits span whole products)
-struct PipelineHook { uint32_t limit; int withhold; };
-PipelineHook pipeline_hook() {
+PipelineHook pipeline_hook(uint32_t default_limit) {
     const uint32_t n = g_wait_limit.load(std::memory_order_relaxed);
-    return {n == (1u << 20) ? (1u << 23) : n, g_withhold_copy.load(std::memory_order_relaxed)};
+    return {n ? n : default_limit, g_withhold_copy.load(std::memory_order_relaxed)};
 }
 
 }  // namespace gact
@@ -278,8 +276,8 @@ extern "C" int gact_quantize(const void* x, int dtype, int64_t n, int bits, uint
     a.R = (a.G + 8 / bits - 1) / (8 / bits);
     a.seed = seed; a.noise = noise; a.packed = (uint8_t*)packed; a.qmin = qmin; a.qscale = qscale;
     a.align = misaligned(x, 16) ? 0 : (misaligned(x, 32) ? 16 : 32);
-    a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
-    a.withhold_copy = g_withhold_copy.load(std::memory_order_relaxed);
+    const PipelineHook hook = pipeline_hook(1u << 20);
+    a.wait_limit = hook.limit; a.withhold_copy = hook.withhold;
     a.rk = philox_round_keys(seed);
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == GACT_F32) return dispatch_bits32(a, bits, rng_mode, fma_mode, s);
@@ -287,7 +285,7 @@ extern "C" int gact_quantize(const void* x, int dtype, int64_t n, int bits, uint
 }
 
 extern "C" void gact_pipeline_test_hook(uint32_t wait_limit, int withhold_one_copy) {
-    g_wait_limit.store(wait_limit == 0 ? (1u << 20) : wait_limit, std::memory_order_relaxed);
+    g_wait_limit.store(wait_limit, std::memory_order_relaxed);
     g_withhold_copy.store(withhold_one_copy ? 1 : 0, std::memory_order_relaxed);
 }
 

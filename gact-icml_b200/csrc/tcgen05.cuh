@@ -26,7 +26,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 
 // Waits for a phase of a barrier, at most `limit` polls.  A wait that runs out sets *dead (shared memory); every later wait of
-// the block then returns at once, so the block runs to its end without waiting for anything again.
+// the block then returns at once, so the block runs to its end without waiting for anything again.  The default spans whole
+// products: a poll takes a quarter of a microsecond (layer norm's rings: 8), the longest reductions a few tenths of a second.
 constexpr uint32_t kWaitLimit = 1u << 23;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* dead) {
     for (uint32_t i = 0; i < limit; i++) {
@@ -40,9 +41,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint32_t limit) {
     for (uint32_t i = 0; i < limit && !mbar_try(bar, parity); i++) {}
 }
-// what gact_pipeline_test_hook asks for (quantize.cu): the limit, and whether block 0 leaves its first copy unissued
-struct PipelineHook { uint32_t limit; int withhold; };
-PipelineHook pipeline_hook();
 
 // address of the same shared-memory variable in block `rank` of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
