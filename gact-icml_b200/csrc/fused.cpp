@@ -45,6 +45,12 @@ void check(int status, const char* what) {
     C10_THROW_ERROR(Error, msg);
 }
 
+// An earlier call's copy that never arrived left its results incomplete: said by the next call, whoever made the first one.
+void check_reports() {
+    TORCH_CHECK(gact_pipeline_reported() == 0, "gact.fused: a copy of a product or of layer norm's rows did not arrive within its wait limit; results "
+                "of calls since the last check are incomplete");
+}
+
 void check_tensor(const Tensor& t, const char* name, bool half_only, const Tensor* like) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
     TORCH_CHECK(t.layout() == at::kStrided, name, " must be a dense tensor");
@@ -165,12 +171,17 @@ PyObject* tuple_of(std::initializer_list<Tensor> ts) {
     return out;
 }
 void count_args(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, "takes ", want, " arguments, got ", n); }
+// what every entry point begins with
+void enter(Py_ssize_t n, Py_ssize_t want) {
+    count_args(n, want);
+    check_reports();
+}
 
 // ---- entry points -----------------------------------------------------------------------------------------------------
 // checkpoint8(input, seed) -> buffer
 PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 2);
+    enter(nargs, 2);
     const Tensor x = tensor_arg(args[0], "input");
     check_tensor(x, "input", false, nullptr);
     TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
@@ -183,7 +194,7 @@ PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // restore8(buffer, shape, dtype) -> tensor
 PyObject* py_restore8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 3);
+    enter(nargs, 3);
     const Tensor buf = tensor_arg(args[0], "checkpoint");
     TORCH_CHECK_TYPE(PyTuple_Check(args[1]), "shape must be a tuple");
     TORCH_CHECK_TYPE(THPDtype_Check(args[2]), "dtype must be a torch.dtype");
@@ -233,7 +244,7 @@ at::ScalarType param_type(const Tensor& w, const Tensor& b, int64_t cols, const 
 // layer_norm(input, weight, bias, eps, compress, seed, save, center) -> (y, checkpoint or input, statistics, weight)
 PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 8);
+    enter(nargs, 8);
     const Tensor x = tensor_arg(args[0], "input");
     Tensor w = optional_arg(args[1], "weight"), b = optional_arg(args[2], "bias");
     const double eps = PyFloat_AsDouble(args[3]);
@@ -272,7 +283,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 //                     need_bias) -> (grad of the input, of weight, of bias)
 PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 8);
+    enter(nargs, 8);
     const Tensor dy = tensor_arg(args[0], "grad_output"), kept = tensor_arg(args[1], "saved input"), stats = tensor_arg(args[2], "saved statistics"),
                  w = optional_arg(args[3], "weight");
     const bool f32 = bool_arg(args[4]), nx = bool_arg(args[5]), nw = bool_arg(args[6]), nb = bool_arg(args[7]);
@@ -317,7 +328,7 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
 //   -> (y, checkpoint or input, checkpoint of z or z)
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 9);
+    enter(nargs, 9);
     const Tensor x = tensor_arg(args[0], "input"), w = tensor_arg(args[1], "weight");
     Tensor b = optional_arg(args[2], "bias");
     const int act = (int)PyLong_AsLong(args[3]);
@@ -379,7 +390,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 //                 need_weight, need_bias) -> (grad of the input, of weight, of bias)
 PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    count_args(nargs, 8);
+    enter(nargs, 8);
     const Tensor dy = tensor_arg(args[0], "grad_output"), w = tensor_arg(args[1], "weight");
     const int act = (int)PyLong_AsLong(args[2]);
     if (PyErr_Occurred()) throw python_error();

@@ -33,6 +33,9 @@ static inline int sm_count() {
 // block 0 leaves its first copy unissued.
 struct PipelineHook { uint32_t limit; int withhold; };
 PipelineHook pipeline_hook(uint32_t default_limit);
+// a word of pinned host memory that a kernel sets when a wait of its ran out, for the host to see without synchronising
+// (gact_pipeline_reported); null if there is none to be had
+int* pipeline_report_word();
 
 // ---------------------------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon et al., SC'11).  Ten rounds; round r uses the key bumped r times by the Weyl

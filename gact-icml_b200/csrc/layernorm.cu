@@ -228,7 +228,7 @@ struct LnBwdArgs {
     void* dx;                                          // null: weight gradients only
     float* partial;                                    // [gridDim][2 * width]: dw, db; null: no weight gradients
     int width;
-    uint32_t wait_limit; int withhold;                 // rings: bounded waits; diagnostics
+    uint32_t wait_limit; int withhold; int* report;    // rings: bounded waits; diagnostics; the host's word
 };
 
 // For short rows, few rows and rows that do not start on 16-byte boundaries.  A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
@@ -434,9 +434,9 @@ struct RowRing {
         return s;
     }
     // elected thread, at the end: a ring that gave up waits (again bounded) for the copies that may still be in flight
-    __device__ __forceinline__ void close() {
+    __device__ __forceinline__ void close(int* host_word) {
         if (!*dead) return;
-        atomicExch(&g_norm_error, 1);
+        report_wait(&g_norm_error, host_word);
         for (uint32_t j = issued > (uint32_t)kRingStages ? issued - kRingStages : 0; j < issued; j++)
             mbar_drain(bar + 8 * (j % kRingStages), (j / kRingStages) & 1, limit);
     }
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
         }
         dx += step * a.cols;
     }
-    if (t == 0) r.close();
+    if (t == 0) r.close(a.report);
     if (!a.partial) return;
     float* p = a.partial + (int64_t)blockIdx.x * 2 * a.width;
 #pragma unroll
@@ -802,7 +802,7 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.dx = dx;
     a.partial = params ? (float*)scratch : nullptr; a.width = (int)((cols + 7) / 8 * 8);
     const PipelineHook hook = pipeline_hook(kWaitLimit);
-    a.wait_limit = hook.limit; a.withhold = hook.withhold;
+    a.wait_limit = hook.limit; a.withhold = hook.withhold; a.report = pipeline_report_word();
     const int eb = elem_bytes_of(dtype);
     const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb));
     const int64_t blocks = ln_bwd_blocks(vec, rows, cols);

@@ -53,7 +53,7 @@ struct GemmArgs {
     float* partial;                           // [splits][M][pitchN] fp32
     int64_t ldp;
     SideJob side;
-    uint32_t wait_limit; int withhold;        // bounded waits; diagnostics
+    uint32_t wait_limit; int withhold; int* report;      // bounded waits; diagnostics; the host's word
 };
 
 __device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
@@ -461,7 +461,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const uint32_t tail = it > (uint32_t)S ? it - S : 0;
             for (uint32_t j = tail; j < it; j++) mbar_wait(empty + 8 * (j % S), (j / S) & 1, a.wait_limit, &dead);
             if (dead) {
-                atomicExch(&g_linear_error, 1);
+                report_wait(&g_linear_error, a.report);
                 if (rank == 0)
                     for (uint32_t j = tail; j < it; j++) mbar_drain(full + 8 * (j % S), (j / S) & 1, a.wait_limit);
             }
@@ -710,7 +710,7 @@ static int run_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int6
                     make_map(&mb, DT, B, B_MN ? K : a.N, B_MN ? a.N : K, ldb, B_MN ? 64 : p.bn / p.cg);
     if (!ok) return GACT_ERR_LAUNCH;
     const PipelineHook hook = pipeline_hook(kWaitLimit);
-    a.wait_limit = hook.limit; a.withhold = hook.withhold;
+    a.wait_limit = hook.limit; a.withhold = hook.withhold; a.report = pipeline_report_word();
     a.ktiles = (int)((K + kBK - 1) / kBK);
     a.tiles_m = (int)p.tiles_m; a.tiles_n = (int)p.tiles_n; a.splits = p.splits; a.per_split = p.per_split;
     constexpr int kEpi = LINEAR ? kEpiLinear : kEpiStore;

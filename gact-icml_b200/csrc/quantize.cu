@@ -13,6 +13,7 @@
 // Rounding without conversions: w + 1.5*2^23 leaves rint(w) (ties to even, like __float2int_rn) in the low
 // mantissa bits; the bits above it fall off when the byte is cut out.
 #include <atomic>
+#include <mutex>
 
 #include "quantize_common.cuh"
 
@@ -241,6 +242,24 @@ PipelineHook pipeline_hook(uint32_t default_limit) {
     const uint32_t n = g_wait_limit.load(std::memory_order_relaxed);
     return {n ? n : default_limit, g_withhold_copy.load(std::memory_order_relaxed)};
 }
+static std::atomic<int*> g_report{nullptr};
+int* pipeline_report_word() {
+    static std::once_flag once;
+    std::call_once(once, [] {
+        // (the first call may be one that is being captured: pinned memory may be had then in relaxed mode only)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool exchanged = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+        int* p = nullptr;
+        if (cudaHostAlloc((void**)&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+            *p = 0;
+            g_report.store(p, std::memory_order_release);
+        } else {
+            (void)cudaGetLastError();
+        }
+        if (exchanged) cudaThreadExchangeStreamCaptureMode(&mode);
+    });
+    return g_report.load(std::memory_order_acquire);
+}
 
 }  // namespace gact
 
@@ -282,6 +301,11 @@ extern "C" int gact_quantize(const void* x, int dtype, int64_t n, int bits, uint
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == GACT_F32) return dispatch_bits32(a, bits, rng_mode, fma_mode, s);
     return launch_quantize16(a, dtype, bits, rng_mode, s);
+}
+
+extern "C" int gact_pipeline_reported(void) {
+    int* p = g_report.load(std::memory_order_acquire);
+    return p && *(volatile int*)p ? __atomic_exchange_n(p, 0, __ATOMIC_RELAXED) : 0;
 }
 
 extern "C" void gact_pipeline_test_hook(uint32_t wait_limit, int withhold_one_copy) {

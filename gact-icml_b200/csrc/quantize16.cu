@@ -741,5 +741,6 @@ extern "C" int gact_pipeline_error_reset(void) {
     const int zero = 0;
     if (cudaMemcpyToSymbol(g_pipeline_error, &zero, sizeof(int)) != cudaSuccess) return GACT_ERR_LAUNCH;
     const int a = linear_error_clear(), b = norm_error_clear();
+    gact_pipeline_reported();
     return a != GACT_OK ? a : b;
 }

@@ -42,6 +42,15 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint32
     for (uint32_t i = 0; i < limit && !mbar_try(bar, parity); i++) {}
 }
 
+// a block that gave up: the device's error word and, for the host's next call, the word in its memory
+__device__ __forceinline__ void report_wait(int* error_word, int* host_word) {
+    atomicExch(error_word, 1);
+    if (host_word) {
+        *(volatile int*)host_word = 1;
+        __threadfence_system();
+    }
+}
+
 // address of the same shared-memory variable in block `rank` of the cluster
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     uint32_t r;

@@ -49,6 +49,7 @@ _SIGNATURES = {
     "gact_sensitivity": ([_vp, _d, _vp, _i, _vp], _i),
     "gact_calc_precision": ([_vp, _vp, _vp, _i, _d, _vp, _vp], _i),
     "gact_calc_precision_host": ([_vp, _vp, _vp, _i, _d], _i),
+    "gact_pipeline_reported": ([], _i),
     "gact_checkpoint8_pitch": ([_i64], _i64),
     "gact_checkpoint8": ([_vp, _i, _i64, _i64, _i64, _i, _u64, _vp, _vp, _vp], _i),
     "gact_restore8": ([_vp, _vp, _i64, _i64, _i, _vp, _i64, _vp], _i),

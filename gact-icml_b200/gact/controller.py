@@ -17,8 +17,9 @@ from gact import _native as _nv
 
 
 def _device_live():
-    """True when this process has a CUDA context (asking the library about its device state would create one)."""
-    return torch.cuda.is_available() and torch.cuda.is_initialized()
+    """True when this process has a CUDA context (asking the library about its device state would create one) and may read from the
+    device (a read-back would end a capture)."""
+    return torch.cuda.is_available() and torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing()
 
 
 class Controller:
@@ -83,7 +84,8 @@ class Controller:
         if getattr(self, "_hook_installed", False):
             torch._C._autograd._pop_saved_tensors_default_hooks()
             self._hook_installed = False
-            if config.compress_activation and _device_live():
+            # (whatever the level: layers that keep their own checkpoints run the same pipelines without compression)
+            if _device_live():
                 _nv.check_pipeline("Controller.uninstall_hook")
 
     def iterate(self, get_grad):

@@ -10,6 +10,10 @@
 The compression of saved tensors (``gact.ops``) restores a tensor in full before a library kernel reads it; these
 operators read the codes themselves.  ``gact.layers`` wraps them for autograd.  Like ``gact.ops``, nothing here falls
 back to another implementation, and kernels run on the current stream of the tensors' device.
+
+Products and layer norm's rings wait for their copies with a limit.  A wait that runs out leaves results incomplete, and the next
+call of any operator here that finds it has happened raises RuntimeError; ``check()`` waits for the device and raises for
+everything up to then (after the last step of a run, say).
 """
 import torch
 
@@ -22,6 +26,13 @@ except ImportError as e:
                       "gact has no fallback path." % e)
 
 LAYER_NORM_MAX_COLS = 16384
+
+
+def check():
+    """Waits for the current device and raises RuntimeError if a wait of an operator's copies has run out there since the last check
+    (one that a call has raised for already among them)."""
+    torch.cuda.synchronize()
+    nv.check_pipeline("gact.fused")
 
 
 # ---------------------------------------------------------------------------------------------------------------

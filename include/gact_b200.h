@@ -10,7 +10,8 @@
  *   - per-device caches filled on first use: the SM count, each kernel's resident-block count and
  *     shared-memory opt-in, the device address of the gact_sq_diffs3_noalloc scratch array (none of them
  *     survives cudaDeviceReset: do not reset a device the library has been used on and then go on using it);
- *   - the sticky error word of the bulk-copy pipeline (gact_pipeline_error / gact_pipeline_error_reset);
+ *   - the sticky error word of the bulk-copy pipeline (gact_pipeline_error / gact_pipeline_error_reset), and 4 bytes of pinned
+ *     host memory, allocated by the first call that needs them (gact_pipeline_reported);
  *   - the diagnostics knobs of gact_pipeline_test_hook;
  *   - the scratch array of gact_sq_diffs3_noalloc (documented there).
  *
@@ -98,6 +99,14 @@ int gact_quantize(const void* x, int dtype, int64_t n, int bits, uint64_t seed, 
  */
 int gact_pipeline_error(void);
 int gact_pipeline_error_reset(void);
+
+/*
+ * 1 when a wait of gact_linear, gact_linear_dgrad, gact_linear_wgrad or gact_layer_norm_backward ran out on any device
+ * since the last time this was asked (and clears that), else 0: what those calls wrote is incomplete.  Reads a word of pinned host
+ * memory that the kernel set; does not synchronise, so it answers for work that has finished.  gact_pipeline_error keeps its own
+ * word; gact_pipeline_error_reset clears this one too.
+ */
+int gact_pipeline_reported(void);
 
 /*
  * Diagnostics, no counterpart in the reference.  wait_limit: polls after which a wait of the pipeline above gives

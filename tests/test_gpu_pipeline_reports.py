@@ -41,3 +41,65 @@ def test_every_limit_is_taken_as_it_is_given(withheld):
 
     short = ms(1 << 18)
     assert 2 * short < ms(1 << 20) < 8 * short
+
+
+CALLS = ["checkpoint", "restore", "norm", "norm backward", "linear", "linear backward", "replay"]
+
+
+@gpu
+@pytest.mark.parametrize("first", ["linear", "norm backward"])
+@pytest.mark.parametrize("second", CALLS)
+def test_the_next_call_says_that_a_copy_was_lost(withheld, first, second):
+    """No Controller, no level: the call after one that lost a copy raises, once, whatever it is; check() does too."""
+    from gact import _native as nv, fused
+    x, w = rand(2000, 2048), rand(64, 2048, seed=1)
+    n, norm = fused.op_layer_norm(x)
+    y, lin = fused.op_linear(x, w)
+    c = fused.op_checkpoint8(x[:4])
+    calls = {"checkpoint": lambda: fused.op_checkpoint8(x[:4]).buf, "restore": lambda: fused.op_restore8(c), "norm": lambda: fused.op_layer_norm(x[:4])[0],
+             "norm backward": lambda: fused.op_layer_norm_backward(x, norm)[0], "linear": lambda: fused.op_linear(x, w)[0],
+             "linear backward": lambda: fused.op_linear_backward(y, lin)[1]}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = calls["norm"]()
+    calls["replay"] = lambda: (graph.replay(), calls["norm"](), captured)[2]
+    want = {k: f().clone() for k, f in calls.items()}
+    torch.cuda.synchronize()
+    withheld(2000)
+    calls[first]()
+    torch.cuda.synchronize()
+    nv.lib.gact_pipeline_test_hook(0, 0)
+    with pytest.raises(RuntimeError, match="did not arrive"):
+        calls[second]()
+    assert torch.equal(calls[second](), want[second])
+    with pytest.raises(RuntimeError, match="did not arrive"):
+        fused.check()
+    fused.check()
+    assert torch.equal(calls[first](), want[first])
+
+
+@gpu
+def test_check_without_another_call(withheld):
+    from gact import _native as nv, fused
+    x, w = rand(100, 256), rand(64, 256, seed=1)
+    withheld(2000)
+    fused.op_linear(x, w, save=False)
+    nv.lib.gact_pipeline_test_hook(0, 0)
+    with pytest.raises(RuntimeError, match="did not arrive"):
+        fused.check()
+    fused.op_linear(x, w, save=False)              # (said once)
+    fused.check()
+
+
+@gpu
+def test_a_controller_without_compression_reports_too(withheld):
+    import gact
+    from gact import fused
+    gact.set_optimization_level("L0")
+    c = gact.Controller(torch.nn.Linear(2, 2))
+    c.install_hook()
+    x, w = rand(100, 256), rand(64, 256, seed=1)
+    withheld(2000)
+    fused.op_linear(x, w, save=False)
+    with pytest.raises(RuntimeError, match="did not arrive"):
+        c.uninstall_hook()

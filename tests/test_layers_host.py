@@ -90,3 +90,22 @@ def test_layer_norm_refuses_unknown_ways_of_rounding():
     p = (ctypes.addressof(b) + 255) & ~255
     for rounding, status in ((2, 6), (8, 6), (-1, 6)):
         assert nv.lib.gact_layer_norm(p, 2, 2, 32, 32, p, p, 2, 1e-5, p, p, p, p, rounding, 0, None) == status
+
+
+def test_a_controller_without_compression_still_asks_for_lost_copies(monkeypatch):
+    import gact
+    import gact.controller
+    asked = []
+    monkeypatch.setattr(gact.controller, "_device_live", lambda: True)
+    monkeypatch.setattr(gact.controller._nv, "check_pipeline", asked.append)
+    gact.set_optimization_level("L0")
+    c = gact.Controller(torch.nn.Linear(2, 2))
+    c.install_hook()
+    c.uninstall_hook()
+    c.uninstall_hook()
+    assert asked == ["Controller.uninstall_hook"]
+
+
+def test_no_report_without_a_device():
+    from gact import _native as nv
+    assert nv.lib.gact_pipeline_reported() == 0
