@@ -324,17 +324,17 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t na
     END_HANDLE_TH_ERRORS
 }
 
-// linear(input, weight, bias, activation code, residual, compress, seed, save, checkpoint of the input or None)
+// linear(input, weight, bias, activation code, residual, compress, seed, save, checkpoint of the input or None, keep input)
 //   -> (y, checkpoint or input, checkpoint of z or z)
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    enter(nargs, 9);
+    enter(nargs, 10);
     const Tensor x = tensor_arg(args[0], "input"), w = tensor_arg(args[1], "weight");
     Tensor b = optional_arg(args[2], "bias");
     const int act = (int)PyLong_AsLong(args[3]);
     if (PyErr_Occurred()) throw python_error();
     const Tensor res = optional_arg(args[4], "residual");
-    const bool compress = bool_arg(args[5]), save = bool_arg(args[7]);
+    const bool compress = bool_arg(args[5]), save = bool_arg(args[7]), keep = save && bool_arg(args[9]);
     const Seed seed = seed_arg(args[6]);
     const Tensor given = optional_arg(args[8], "checkpoint");
     check_tensor(x, "input", true, nullptr);
@@ -368,7 +368,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (save) {
         if (act && compress) zc = empty_codes(xr.rows, cout, x);
         else if (act) z = make({xr.rows, cout}, x.scalar_type(), x);
-        if (compress && !c.defined()) c = xc = empty_codes(xr.rows, cin, x);
+        if (keep && compress && !c.defined()) c = xc = empty_codes(xr.rows, cin, x);
     }
     if (xr.rows > 0) {
         void* s = stream_of(x);
@@ -382,25 +382,32 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         g_launches += 1 + (bytes > 0);
     }
     if (!save) return tuple_of({y, Tensor(), Tensor()});
-    return tuple_of({y, compress ? c.buf : x, zc.defined() ? zc.buf : z});
+    return tuple_of({y, !keep ? Tensor() : compress ? c.buf : x, zc.defined() ? zc.buf : z});
     END_HANDLE_TH_ERRORS
 }
 
-// linear_backward(grad_output, weight, activation code, checkpoint or input, checkpoint of z or z or None, need_input,
-//                 need_weight, need_bias) -> (grad of the input, of weight, of bias)
+// linear_backward(grad_output, weight or None, activation code, checkpoint or input or None, checkpoint of z or z or None,
+//                 need_input, need_weight, need_bias, input features) -> (grad of the input, of weight, of bias)
 PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    enter(nargs, 8);
-    const Tensor dy = tensor_arg(args[0], "grad_output"), w = tensor_arg(args[1], "weight");
+    enter(nargs, 9);
+    const Tensor dy = tensor_arg(args[0], "grad_output"), w = optional_arg(args[1], "weight");
     const int act = (int)PyLong_AsLong(args[2]);
     if (PyErr_Occurred()) throw python_error();
     const Tensor xk = optional_arg(args[3], "saved input"), zk = optional_arg(args[4], "saved pre-activation");
     const bool nx = bool_arg(args[5]), nw = bool_arg(args[6]), nb = bool_arg(args[7]);
-    check_tensor(w, "weight", true, nullptr);
-    check_tensor(dy, "grad_output", true, &w);
-    TORCH_CHECK(dy.scalar_type() == w.scalar_type(), "The type of grad_output is not correct!");
-    TORCH_CHECK_VALUE(w.dim() == 2 && dy.dim() > 0 && dy.size(-1) == w.size(0), "grad_output ", dy.sizes(), " does not fit weight ", w.sizes());
-    const int64_t cout = w.size(0), cin = w.size(1);
+    const int64_t cin = PyLong_AsLongLong(args[8]);
+    if (PyErr_Occurred()) throw python_error();
+    check_tensor(dy, "grad_output", true, nullptr);
+    TORCH_CHECK_VALUE(dy.dim() > 0 && dy.size(-1) > 0 && cin > 0, "grad_output ", dy.sizes(), " is not that of a linear layer");
+    const int64_t cout = dy.size(-1);
+    if (w.defined()) {
+        check_tensor(w, "weight", true, &dy);
+        TORCH_CHECK(dy.scalar_type() == w.scalar_type(), "The type of grad_output is not correct!");
+        TORCH_CHECK_VALUE(w.dim() == 2 && cout == w.size(0) && cin == w.size(1), "grad_output ", dy.sizes(), " does not fit weight ", w.sizes());
+    }
+    TORCH_CHECK_VALUE(w.defined() || !nx, "the weight was not saved");
+    TORCH_CHECK_VALUE(xk.defined() || !nw, "the input was not saved");
     const int code = type_code(dy.scalar_type());
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(dy.device());
@@ -447,7 +454,6 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     Codes xc;
     Rows x{Tensor(), 0, 0};
     if (nw) {
-        TORCH_CHECK_VALUE(xk.defined(), "the input was not saved");
         if (is_codes(xk)) {
             xc = as_codes(xk, rows, cin, &dy);
             const int64_t pitch = gact_checkpoint8_pitch(cin);
@@ -488,9 +494,9 @@ PyMethodDef kMethods[] = {
     {"layer_norm", FAST(py_layer_norm), "layer_norm(input, weight, bias, eps, compress, seed, save, center) -> (y, kept, statistics, weight)"},
     {"layer_norm_backward", FAST(py_layer_norm_backward),
      "layer_norm_backward(grad_output, kept, statistics, weight, fp32 parameters, need_input, need_weight, need_bias) -> three gradients"},
-    {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, checkpoint) -> (y, kept, z)"},
+    {"linear", FAST(py_linear), "linear(input, weight, bias, activation, residual, compress, seed, save, checkpoint, keep_input) -> (y, kept, z)"},
     {"linear_backward", FAST(py_linear_backward),
-     "linear_backward(grad_output, weight, activation, kept, z, need_input, need_weight, need_bias) -> three gradients"},
+     "linear_backward(grad_output, weight, activation, kept, z, need_input, need_weight, need_bias, input features) -> three gradients"},
     {"launches", py_launches, METH_NOARGS, "library kernels enqueued by this module"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fused", "Host side of gact.fused.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -131,21 +131,22 @@ def op_layer_norm_backward(grad_output, saved, needs=(True, True, True)):
 # linear
 # ---------------------------------------------------------------------------------------------------------------
 class LinearSaved:
-    """What the backward pass of a linear layer needs: its input and (with an activation) its pre-activation, each a
-    Checkpoint8 or a tensor, and the weight."""
-    __slots__ = ("x", "z", "weight", "activation", "out_shape", "has_bias")
+    """What the backward pass of a linear layer needs: its input (for the weight's gradient) and, with an activation, its
+    pre-activation, each a Checkpoint8 or a tensor, and the weight (for the input's gradient; without it ``in_features``)."""
+    __slots__ = ("x", "z", "weight", "activation", "out_shape", "has_bias", "in_features")
 
-    def __init__(self, x, z, weight, activation, out_shape, has_bias):
+    def __init__(self, x, z, weight, activation, out_shape, has_bias, in_features=None):
         self.x, self.z, self.weight, self.activation, self.out_shape, self.has_bias = x, z, weight, activation, out_shape, has_bias
+        self.in_features = weight.shape[-1] if in_features is None else in_features
 
 
-def op_linear(input, weight, bias=None, activation=None, residual=None, compress=True, seed=None, save=True, checkpoint=None):
+def op_linear(input, weight, bias=None, activation=None, residual=None, compress=True, seed=None, save=True, checkpoint=None, keep_input=True):
     """(y, saved): y = activation(input W^T + bias) + residual for float16 / bfloat16 tensors, fp32 accumulation.
 
     activation: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  ``compress``: keep input and pre-activation as
     Checkpoint8 for the backward pass (with a ``seed`` rounded stochastically), else as tensors.  ``checkpoint``: a
     Checkpoint8 of this very input that is already there (several layers reading one tensor share it).  ``save`` False:
-    forward only, saved is None."""
+    forward only, saved is None; ``keep_input`` False: a frozen weight, whose gradient nobody will ask for, keeps no input."""
     act = nv.ACT_CODE.get(activation)
     if act is None:
         raise ValueError("unknown activation %r" % (activation,))
@@ -156,11 +157,12 @@ def op_linear(input, weight, bias=None, activation=None, residual=None, compress
         if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
             raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
         given = checkpoint.buf
-    y, kept, z = _fused.linear(input, weight, bias, act, residual, compress, seed, save, given)
+    y, kept, z = _fused.linear(input, weight, bias, act, residual, compress, seed, save, given, keep_input)
     if not save:
         return y, None
     if compress:
-        kept = checkpoint if checkpoint is not None else Checkpoint8(kept, input.shape, input.dtype)
+        if kept is not None:
+            kept = checkpoint if checkpoint is not None else Checkpoint8(kept, input.shape, input.dtype)
         if z is not None:
             z = Checkpoint8(z, y.shape, input.dtype)
     return y, LinearSaved(kept, z, weight, activation, y.shape, bias is not None)
@@ -172,4 +174,4 @@ def op_linear_backward(grad_output, saved, needs=(True, True, True)):
     if grad_output.shape != saved.out_shape:
         raise ValueError("grad_output must have shape %s, got %s" % (tuple(saved.out_shape), tuple(grad_output.shape)))
     return _fused.linear_backward(grad_output, saved.weight, nv.ACT_CODE[saved.activation], _unwrap(saved.x), _unwrap(saved.z), needs[0], needs[1],
-                                  needs[2] and saved.has_bias)
+                                  needs[2] and saved.has_bias, saved.in_features)

@@ -69,28 +69,35 @@ class _LayerNorm(torch.autograd.Function):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, compress, seed, given):
+    def forward(ctx, x, weight, bias, residual, activation, compress, seed, given, keep_input):
         # Under autocast the parameters are cast here and again in backward: what is saved is the parameter itself, which hooks
         # know and leave alone.  (A copy that requires a gradient looks like an activation to them and would be quantized.)
         w, b = _autocast(weight, bias)
-        ck = None if given is None else Checkpoint8(given, x.shape, x.dtype)
-        y, s = fused.op_linear(x, w, b, activation, residual, compress=compress, seed=seed, checkpoint=ck)
+        # Only what a gradient will need: the input for the weight's, the weight for the input's, the pre-activation for any of the three.
+        n = ctx.needs_input_grad
+        if not (n[0] or n[1] or n[2]):
+            return fused.op_linear(x, w, b, activation, residual, save=False)[0]
+        keep_input = keep_input or n[1]
+        ck = None if given is None or not keep_input else Checkpoint8(given, x.shape, x.dtype)
+        y, s = fused.op_linear(x, w, b, activation, residual, compress=compress, seed=seed, checkpoint=ck, keep_input=keep_input)
         xt, *ctx.x = _flat(s.x)
         zt, *ctx.z = _flat(s.z)
-        ctx.save_for_backward(xt, zt, weight)
-        ctx.meta = (activation, s.out_shape, s.has_bias)
+        ctx.save_for_backward(xt, zt, weight if n[0] else None)
+        ctx.meta = (activation, s.out_shape, s.has_bias, s.in_features)
         ctx.param_dtypes = weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xt, zt, weight = ctx.saved_tensors
-        saved = LinearSaved(_unflat(xt, *ctx.x), _unflat(zt, *ctx.z), weight.to(dy.dtype), *ctx.meta)
         n = ctx.needs_input_grad
+        if not (n[0] or n[1] or n[2]):
+            return (None,) * 3 + (dy,) + (None,) * 5
+        xt, zt, weight = ctx.saved_tensors
+        saved = LinearSaved(_unflat(xt, *ctx.x), _unflat(zt, *ctx.z), None if weight is None else weight.to(dy.dtype), *ctx.meta)
         dx, dw, db = fused.op_linear_backward(dy, saved, (n[0], n[1], n[2]))
         wt, bt = ctx.param_dtypes
-        return dx, None if dw is None else dw.to(wt), None if db is None else db.to(bt), (dy if n[3] else None), None, None, None, None
+        return dx, None if dw is None else dw.to(wt), None if db is None else db.to(bt), (dy if n[3] else None), None, None, None, None, None
 
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
@@ -109,9 +116,11 @@ def _autocast(*tensors):
     return tuple(t if t is None or not t.is_floating_point() or t.dtype == torch.float64 else t.to(dt) for t in tensors)
 
 
-def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None):
+def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None, keep_input=None):
     """activation(input W^T + bias) + residual, differentiable; see ``gact.fused.op_linear``.  ``compress`` as in
-    ``layer_norm``; ``checkpoint``: a Checkpoint8 of the input (in the type it is computed in) to share."""
+    ``layer_norm``; ``checkpoint``: a Checkpoint8 of the input (in the type it is computed in) to share.  ``keep_input``: whether the
+    input is kept although the weight asks for no gradient; None: not for a frozen parameter, but for a plain tensor (whose
+    ``grad_fn.saved_tensors`` then hold it)."""
     input, residual = _autocast(input, residual)
     if input.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("gact.layers.linear computes in float16 or bfloat16: cast the model or use torch.autocast "
@@ -124,7 +133,8 @@ def linear(input, weight, bias=None, activation=None, residual=None, compress=No
         if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
             raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
         given = checkpoint.buf
-    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, given)
+    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, given,
+                         not isinstance(weight, nn.Parameter) if keep_input is None else keep_input)
 
 
 class LayerNorm(nn.LayerNorm):
@@ -169,7 +179,8 @@ def share_input(parent, children):
 
     def before(module, args):
         x = args[0] if args else None
-        if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(x, *(c.weight for c in children)):
+        # (frozen weights keep no input)
+        if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(*(c.weight for c in children)):
             cast = _autocast(x)[0]
             if cast.dtype in (torch.float16, torch.bfloat16):
                 ck = fused.op_checkpoint8(cast.detach(), _next_seed())

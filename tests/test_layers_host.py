@@ -109,3 +109,47 @@ def test_a_controller_without_compression_still_asks_for_lost_copies(monkeypatch
 def test_no_report_without_a_device():
     from gact import _native as nv
     assert nv.lib.gact_pipeline_reported() == 0
+
+
+@pytest.mark.parametrize("compress", [True, False])
+def test_only_what_a_gradient_needs_is_saved(plain, compress):
+    """A frozen weight keeps no input, a frozen input no weight, a residual alone nothing; gradients come out where they are asked for."""
+    for x_grad, w_grad, b_grad, r_grad in [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (1, 0, 1, 1), (0, 0, 0, 1), (1, 1, 1, 1)]:
+        x, w, b, r = (torch.randn(*s).bfloat16().requires_grad_(bool(g)) for s, g in (((5, 8), x_grad), ((4, 8), w_grad), ((4,), b_grad), ((5, 4), r_grad)))
+        w = torch.nn.Parameter(w.detach(), requires_grad=bool(w_grad))
+        y, seen = saved_by(lambda: layers.linear(x, w, b, residual=r, compress=compress))
+        assert plain[-1]["save"] == bool(x_grad or w_grad or b_grad) and plain[-1].get("keep_input", True) == bool(w_grad or not plain[-1]["save"])
+        assert any(t.data_ptr() == w.data_ptr() for t in seen) == bool(x_grad)
+        assert any(t.dtype == torch.int8 or t.data_ptr() == x.data_ptr() for t in seen) == bool(w_grad)
+        if not x_grad:
+            with torch.no_grad():
+                w.mul_(2)                       # (nobody needs the old one)
+        y.sum().backward()
+        assert [t.grad is not None for t in (x, w, b, r)] == [bool(g) for g in (x_grad, w_grad, b_grad, r_grad)]
+
+
+def test_a_plain_weight_without_gradient_says_whether_the_input_is_kept(plain):
+    x, w = torch.randn(5, 8).bfloat16().requires_grad_(), torch.randn(4, 8).bfloat16()
+    for asked, kept in ((None, True), (True, True), (False, False)):
+        layers.linear(x, w, keep_input=asked)
+        assert plain[-1]["keep_input"] == kept
+    layers.linear(x, w.clone().requires_grad_(), keep_input=False)           # (its gradient needs it)
+    assert plain[-1]["keep_input"]
+
+
+def test_share_input_of_frozen_layers_makes_no_checkpoint(plain, monkeypatch):
+    made = []
+    monkeypatch.setattr(fused, "op_checkpoint8", lambda x, seed=None: made.append(x))
+
+    class Two(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a, self.b = layers.Linear(8, 8), layers.Linear(8, 8)
+
+        def forward(self, x):
+            return self.a(x) + self.b(x)
+
+    m = Two().bfloat16().requires_grad_(False)
+    layers.share_input(m, (m.a, m.b))
+    m(torch.zeros(3, 8, dtype=torch.bfloat16, requires_grad=True))
+    assert not made and not any(c["keep_input"] for c in plain)
