@@ -10,8 +10,8 @@ both alone and go on compressing everything else the model saves.  Converted lay
 auto precision adapts the other tensors.  ``config.stochastic_checkpoints`` rounds the codes stochastically instead of to
 nearest.
 
-Linear layers compute in float16 / bfloat16 (under autocast the inputs are cast to its type, as torch does); layer norm keeps
-the type of its input.
+Linear layers compute in float16 / bfloat16 (under autocast input and parameters are cast to its type, as torch does); layer norm
+keeps the type of its input (torch's returns float32 under autocast).
 """
 import torch
 import torch.nn as nn
@@ -120,11 +120,18 @@ def linear(input, weight, bias=None, activation=None, residual=None, compress=No
     """activation(input W^T + bias) + residual, differentiable; see ``gact.fused.op_linear``.  ``compress`` as in
     ``layer_norm``; ``checkpoint``: a Checkpoint8 of the input (in the type it is computed in) to share.  ``keep_input``: whether the
     input is kept although the weight asks for no gradient; None: not for a frozen parameter, but for a plain tensor (whose
-    ``grad_fn.saved_tensors`` then hold it)."""
-    input, residual = _autocast(input, residual)
+    ``grad_fn.saved_tensors`` then hold it).  A residual of another type is an error, but under autocast it is added to the
+    result as torch adds it, in the wider of the two types."""
+    input, = _autocast(input)
     if input.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("gact.layers.linear computes in float16 or bfloat16: cast the model or use torch.autocast "
                            "(got an input of %s)" % input.dtype)
+    if residual is not None and residual.dtype != input.dtype and torch.is_autocast_enabled("cuda"):
+        # as torch's sum: the wider type (an fp32 residual stream keeps its bits)
+        y = linear(input, weight, bias, activation, None, compress, checkpoint, keep_input)
+        if residual.shape != y.shape:
+            raise ValueError("residual must have shape %s, got %s" % (tuple(y.shape), tuple(residual.shape)))
+        return y + residual
     if not _keeps_graph(input, weight, bias, residual):
         return fused.op_linear(input, *_autocast(weight, bias), activation, residual, save=False)[0]
     compress = config.compress_activation if compress is None else compress

@@ -153,3 +153,19 @@ def test_share_input_of_frozen_layers_makes_no_checkpoint(plain, monkeypatch):
     layers.share_input(m, (m.a, m.b))
     m(torch.zeros(3, 8, dtype=torch.bfloat16, requires_grad=True))
     assert not made and not any(c["keep_input"] for c in plain)
+
+
+def test_a_wider_residual_keeps_its_type_under_autocast(plain, autocast):
+    """torch's linear + residual gives the wider type; a residual stream in fp32 must not be lowered to 16 bits."""
+    x, w = torch.randn(5, 8), torch.nn.Parameter(torch.randn(4, 8))
+    for dt in (torch.float32, torch.float64):
+        r = torch.randn(5, 4, dtype=dt).requires_grad_()
+        y = layers.linear(x, w, residual=r)
+        assert y.dtype == dt and torch.equal(y, layers.linear(x, w) + r) and not plain[-1]["residual"]
+        y.sum().backward()
+        assert torch.equal(r.grad, torch.ones_like(r)) and w.grad.dtype == torch.float32
+    assert layers.linear(x, w, residual=torch.randn(5, 4).bfloat16()).dtype == torch.bfloat16 and plain[-1]["residual"]
+    with torch.no_grad():
+        assert layers.linear(x, w, residual=torch.randn(5, 4)).dtype == torch.float32
+    with pytest.raises(ValueError, match="residual must have shape"):
+        layers.linear(x, w, residual=torch.randn(4))
