@@ -36,10 +36,24 @@ __device__ __forceinline__ float scale_up8(uint32_t b) { return b == 255u ? 0.0f
 // 2^(b-127); NaN for b = 255
 __device__ __forceinline__ float scale_down8(uint32_t b) { return b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b << 23); }
 
-// Noise of stochastic rounding: Philox4x32-7 keyed by the seed, one call per 8 consecutive elements of the padded row
-// layout (counter = element index / 8), 16 bits each: u = (r + 0.5) / 65536.
-__device__ __forceinline__ uint4 noise8(const PhiloxKeys& rk, uint64_t chunk) {
-    return philox4x32<7>((uint32_t)chunk, (uint32_t)(chunk >> 32), 0u, 0u, rk);
+// Noise of stochastic rounding: Philox4x32-7, one call per 8 consecutive elements of the padded row layout (low half of the
+// counter = element index / 8), 16 bits each: u = (r + 0.5) / 65536.  A seed is the key; one that lies on the device (a captured
+// launch cannot be given another key) is the high half of the counter instead.
+struct Noise8 {
+    PhiloxKeys rk; const uint2* word;
+    static Noise8 of(uint64_t seed, bool on_device, uint64_t other) {
+        return {philox_round_keys((on_device ? 0 : seed) + other), on_device ? (const uint2*)(uintptr_t)seed : nullptr};
+    }
+    __device__ __forceinline__ uint2 high() const { return word ? __ldg(word) : make_uint2(0u, 0u); }
+};
+__device__ __forceinline__ uint4 noise8(const Noise8& n, uint2 high, uint64_t chunk) {
+    return philox4x32<7>((uint32_t)chunk, (uint32_t)(chunk >> 32), high.x, high.y, n.rk);
+}
+// the `rounding` argument of the entry points: a known combination, and a seed on the device that can be read
+static inline int rounding_status(int rounding, uint64_t seed, int known) {
+    if ((rounding & ~known) || ((rounding & GACT_CODES_DEVICE_SEED) && !(rounding & GACT_CODES_STOCHASTIC))) return GACT_ERR_MODE;
+    if (rounding & GACT_CODES_DEVICE_SEED) return !seed ? GACT_ERR_NULL : (seed & 7) ? GACT_ERR_ALIGN : GACT_OK;
+    return GACT_OK;
 }
 __device__ __forceinline__ float noise8_at(const uint4& r, int j) {
     const uint32_t w = word_of(r, j >> 1);
@@ -143,14 +157,14 @@ template <int DT> __device__ __forceinline__ uint32_t absmax8(const uint32_t (&r
 // lanes and every lane of the warp must call.  `m`: the lane's largest magnitude; `last`: top_byte8 of the type that the codes
 // are restored to.  Returns the scale byte too.
 template <bool STOCH>
-__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const PhiloxKeys& rk, uint64_t chunk, uint32_t& byte, uint32_t last) {
+__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], uint32_t m, const Noise8& noise, uint2 high, uint64_t chunk, uint32_t& byte, uint32_t last) {
     m = max(m, __shfl_xor_sync(kFull, m, 1));
     m = max(m, __shfl_xor_sync(kFull, m, 2));
     byte = scale_byte8(m);
     const float up = scale_up8(byte);
     uint32_t c[8];
     if constexpr (STOCH) {
-        const uint4 r = noise8(rk, chunk);
+        const uint4 r = noise8(noise, high, chunk);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             c[2 * i] = code8_noise(v[i].x, up, noise8_at(r, 2 * i));

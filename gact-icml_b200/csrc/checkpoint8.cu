@@ -12,7 +12,7 @@ struct Ckpt8Args {
     int chunks;               // chunks of 8 elements per padded row
     int tiles;                // tiles of 256 columns per row
     Divisor by;               // chunks or tiles of a row, by the way the kernel walks
-    PhiloxKeys rk;
+    Noise8 noise;
 };
 struct Restore8Args {
     const int8_t* codes; const uint8_t* scales;
@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kCThreads) checkpoint8_kernel(const __grid_con
     __shared__ __align__(16) uint8_t stage[VEC || FLAT ? 16 : kCThreads * 8 * Elem<DT>::kBytes];
     void* mine = stage + (VEC || FLAT ? 0 : (threadIdx.x >> 5) * Stage8<DT, false>::kBytes);
     const Walk<FLAT, U> w(a.rows, a.chunks, a.tiles, a.by);
+    const uint2 high = STOCH ? a.noise.high() : make_uint2(0u, 0u);
     Row8<DT, VEC, 32> x[U];
     uint32_t raw[U][RawRegs<DT>::N];
 #pragma unroll
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kCThreads) checkpoint8_kernel(const __grid_con
         float2 v[4];
         raw_to_pairs<DT>(raw[u], v);
         uint32_t byte;
-        const uint2 c = codes8<STOCH>(v, absmax8<DT>(raw[u]), a.rk, (uint64_t)w.chunk[u], byte, top_byte8<DT>());
+        const uint2 c = codes8<STOCH>(v, absmax8<DT>(raw[u]), a.noise, high, (uint64_t)w.chunk[u], byte, top_byte8<DT>());
         if (w.chunk[u] >= 0) {
             st_stream_u2(a.codes + w.chunk[u] * 8, c);
             if ((threadIdx.x & 3) == 0) a.scales[w.chunk[u] >> 2] = (uint8_t)byte;
@@ -168,18 +169,20 @@ using namespace gact;
 
 extern "C" int64_t gact_checkpoint8_pitch(int64_t cols) { return cols < 0 ? -1 : pitch8(cols); }
 
-extern "C" int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int stochastic, uint64_t seed,
+extern "C" int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int rounding, uint64_t seed,
                                 void* codes, void* scales, void* stream) {
     if (dtype < GACT_F32 || dtype > GACT_BF16) return GACT_ERR_DTYPE;
     if (rows < 0 || cols < 0 || cols > GACT_MAX_COLS || ld < cols || (cols && rows > GACT_MAX_ELEMENTS / pitch8(cols))) return GACT_ERR_SIZE;
     if (rows == 0 || cols == 0) return GACT_OK;
+    if (const int st = rounding_status(rounding, seed, GACT_CODES_STOCHASTIC | GACT_CODES_DEVICE_SEED)) return st;
     if (!x || !codes || !scales) return GACT_ERR_NULL;
     if (((uintptr_t)x & (uintptr_t)(elem_bytes_of(dtype) - 1)) || ((uintptr_t)codes & 31)) return GACT_ERR_ALIGN;
     Ckpt8Args a;
     a.x = x; a.ld = ld; a.rows = rows; a.cols = (int)cols;
     a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales; a.chunks = (int)(pitch8(cols) / 8);
     a.tiles = (int)((cols + 255) / 256);
-    a.rk = philox_round_keys(seed);
+    const bool stochastic = rounding & GACT_CODES_STOCHASTIC;
+    a.noise = Noise8::of(seed, rounding & GACT_CODES_DEVICE_SEED, 0);
     cudaStream_t s = (cudaStream_t)stream;
     switch (dtype) {
     case GACT_F32: return stochastic ? dispatch_ckpt<GACT_F32, true>(a, s) : dispatch_ckpt<GACT_F32, false>(a, s);

@@ -95,7 +95,8 @@ Rows as_operand(Rows r, int64_t cols, void* stream) {
     return {out, r.rows, pitch};
 }
 
-struct Seed { int stochastic = 0; uint64_t value = 0; };
+// how codes are rounded; `held` keeps a seed that lies on the device
+struct Seed { int rounding = 0; uint64_t value = 0; Tensor held; };
 
 // A checkpoint is one byte tensor: rows x pitch codes, then rows x pitch / 32 scales.
 struct Codes {
@@ -133,7 +134,7 @@ Codes checkpoint8(const Tensor& x, const Seed& seed) {
     const int64_t cols = x.size(-1);
     Codes c = empty_codes(r.rows, cols, x);
     if (x.numel() == 0) return c;
-    check(gact_checkpoint8(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, seed.stochastic, seed.value, c.codes(), c.scales(),
+    check(gact_checkpoint8(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, seed.rounding, seed.value, c.codes(), c.scales(),
                            stream_of(x)), "gact_checkpoint8");
     g_launches++;
     return c;
@@ -145,10 +146,17 @@ Tensor tensor_arg(PyObject* o, const char* name) {
     return THPVariable_Unpack(o);
 }
 Tensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor_arg(o, name); }
-Seed seed_arg(PyObject* o) {
+// None, a number, or a tensor beside `like` whose one int64 the kernels read
+Seed seed_arg(PyObject* o, const Tensor& like) {
     Seed s;
-    if (o != Py_None) {
-        s.stochastic = 1;
+    if (THPVariable_Check(o)) {
+        s.held = THPVariable_Unpack(o);
+        TORCH_CHECK(s.held.device() == like.device(), "seed is on ", s.held.device().str(), ", the input on ", like.device().str());
+        TORCH_CHECK_VALUE(s.held.scalar_type() == at::kLong && s.held.numel() == 1 && s.held.layout() == at::kStrided, "a seed tensor holds one int64");
+        s.rounding = GACT_CODES_STOCHASTIC | GACT_CODES_DEVICE_SEED;
+        s.value = (uint64_t)(uintptr_t)s.held.data_ptr();
+    } else if (o != Py_None) {
+        s.rounding = GACT_CODES_STOCHASTIC;
         s.value = PyLong_AsUnsignedLongLongMask(o);
         if (PyErr_Occurred()) throw python_error();
     }
@@ -187,7 +195,7 @@ PyObject* py_checkpoint8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(x.device());
-    return wrap(checkpoint8(x, seed_arg(args[1])).buf);
+    return wrap(checkpoint8(x, seed_arg(args[1], x)).buf);
     END_HANDLE_TH_ERRORS
 }
 
@@ -250,8 +258,8 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const double eps = PyFloat_AsDouble(args[3]);
     if (PyErr_Occurred()) throw python_error();
     const bool compress = bool_arg(args[4]), save = bool_arg(args[6]), center = bool_arg(args[7]);
-    const Seed seed = seed_arg(args[5]);
     check_tensor(x, "input", false, nullptr);
+    const Seed seed = seed_arg(args[5], x);
     TORCH_CHECK_VALUE(x.dim() > 0, "input needs at least one dimension");
     const int64_t cols = x.size(-1);
     TORCH_CHECK_VALUE(cols >= 1 && cols <= GACT_LAYER_NORM_MAX_COLS, "layer norm takes rows of 1 to ", GACT_LAYER_NORM_MAX_COLS, " elements, got ", cols);
@@ -271,7 +279,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (r.rows > 0) {
         check(gact_layer_norm(r.t.data_ptr(), type_code(x.scalar_type()), r.rows, cols, r.ld, ptr(w), ptr(b), type_code(pt), eps, y.data_ptr(),
                               (float*)ptr(stats), c.codes(), c.scales(),
-                              (seed.stochastic ? GACT_CODES_STOCHASTIC : 0) | (center ? GACT_CODES_CENTERED : 0), seed.value, stream_of(x)),
+                              seed.rounding | (center ? GACT_CODES_CENTERED : 0), seed.value, stream_of(x)),
               "gact_layer_norm");
         g_launches++;
     }
@@ -335,9 +343,9 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (PyErr_Occurred()) throw python_error();
     const Tensor res = optional_arg(args[4], "residual");
     const bool compress = bool_arg(args[5]), save = bool_arg(args[7]), keep = save && bool_arg(args[9]);
-    const Seed seed = seed_arg(args[6]);
     const Tensor given = optional_arg(args[8], "checkpoint");
     check_tensor(x, "input", true, nullptr);
+    const Seed seed = seed_arg(args[6], x);
     check_tensor(w, "weight", true, &x);
     TORCH_CHECK(w.scalar_type() == x.scalar_type(), "The type of weight is not correct!");
     TORCH_CHECK_VALUE(x.dim() > 0 && w.dim() == 2 && x.size(-1) == w.size(1), "input ", x.sizes(), " does not fit weight ", w.sizes());
@@ -377,7 +385,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const int64_t bytes = gact_linear_scratch_bytes(xr.rows, cin, cout, 0);
         const Tensor scr = scratch(bytes, x);
         check(gact_linear(xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, ptr(b), ptr(rr.t), rr.ld, type_code(x.scalar_type()), xr.rows, cin, cout, act,
-                          y.data_ptr(), xc.codes(), xc.scales(), ptr(z), zc.codes(), zc.scales(), seed.stochastic, seed.value, ptr(scr), s),
+                          y.data_ptr(), xc.codes(), xc.scales(), ptr(z), zc.codes(), zc.scales(), seed.rounding, seed.value, ptr(scr), s),
               "gact_linear");
         g_launches += 1 + (bytes > 0);
     }

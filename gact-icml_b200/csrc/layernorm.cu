@@ -22,7 +22,7 @@ struct LnArgs {
     int64_t rows; int cols; float inv_cols; float eps;
     void* y;
     float* stats;                                    // (mean, or 0 with `center`; 1 / deviation) per row, or null
-    int8_t* codes; uint8_t* scales; int chunks; int stochastic, center; PhiloxKeys rk;
+    int8_t* codes; uint8_t* scales; int chunks; int stochastic, center; Noise8 noise;
 };
 
 // 8 weights starting at column `col` (fp32 or the type of x); `none` without a weight, 0 past the end
@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(TPR > 128 ? TPR : 128) layer_norm_kernel(const
             if (a.codes) {
                 uint32_t byte;
                 const uint64_t chunk = (uint64_t)row * a.chunks + (t + c * TPR);
-                const uint2 q = a.stochastic ? codes8<true>(v[c], top[c], a.rk, chunk, byte, last) : codes8<false>(v[c], top[c], a.rk, chunk, byte, last);
+                const uint2 q = a.stochastic ? codes8<true>(v[c], top[c], a.noise, a.noise.high(), chunk, byte, last)
+                                             : codes8<false>(v[c], top[c], a.noise, make_uint2(0u, 0u), chunk, byte, last);
                 if (live && t + c * TPR < a.chunks) {
                     st_stream_u2(a.codes + chunk * 8, q);
                     if ((t & 3) == 0) a.scales[chunk >> 2] = (uint8_t)byte;
@@ -748,7 +749,7 @@ extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t c
     if (dtype < GACT_F32 || dtype > GACT_BF16 || (param_dtype != dtype && param_dtype != GACT_F32)) return GACT_ERR_DTYPE;
     if (!ln_sizes_ok(rows, cols) || ld < cols) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
-    if (rounding & ~(GACT_CODES_STOCHASTIC | GACT_CODES_CENTERED)) return GACT_ERR_MODE;
+    if (const int st = rounding_status(rounding, seed, GACT_CODES_STOCHASTIC | GACT_CODES_DEVICE_SEED | GACT_CODES_CENTERED)) return st;
     if (!x || !y || (codes && !scales)) return GACT_ERR_NULL;
     const uintptr_t em = (uintptr_t)(elem_bytes_of(dtype) - 1);
     if (((uintptr_t)x & em) || ((uintptr_t)y & em) || ((uintptr_t)codes & 31) || ((uintptr_t)stats & 7) || !param_ok(weight, param_dtype) ||
@@ -758,7 +759,7 @@ extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t c
     a.x = x; a.ldx = ld; a.w = weight; a.b = bias; a.wf32 = param_dtype == GACT_F32;
     a.rows = rows; a.cols = (int)cols; a.inv_cols = 1.0f / (float)cols; a.eps = (float)eps;
     a.y = y; a.stats = stats; a.codes = (int8_t*)codes; a.scales = (uint8_t*)scales;
-    a.chunks = (int)(pitch8(cols) / 8); a.rk = philox_round_keys(seed);
+    a.chunks = (int)(pitch8(cols) / 8); a.noise = Noise8::of(seed, rounding & GACT_CODES_DEVICE_SEED, 0);
     a.stochastic = (rounding & GACT_CODES_STOCHASTIC) != 0; a.center = codes && (rounding & GACT_CODES_CENTERED);
     const bool vec = rows_aligned(x, ld, cols, elem_bytes_of(dtype)) && rows_aligned(y, cols, cols, elem_bytes_of(dtype));
     cudaStream_t s = (cudaStream_t)stream;

@@ -32,7 +32,7 @@ enum { kEpiStore = 0, kEpiLinear = 1, kEpiPartial = 2 };
 // weight gradient that follows (kind 2), and the bias gradient's partial sums added up beside either gradient.
 struct SideJob {
     int kind;
-    const void* x; int64_t ld; int stochastic; PhiloxKeys rk;      // 1: rows of cols elements on 16-byte boundaries
+    const void* x; int64_t ld; int stochastic; Noise8 noise;       // 1: rows of cols elements on 16-byte boundaries
     int8_t* codes; uint8_t* scales;
     void* out;                                                     // 2: rows of the codes' pitch
     int64_t rows; int cols, chunks; Divisor by;
@@ -49,7 +49,7 @@ struct GemmArgs {
     int act;
     void* z; int zvec;                        // pre-activation in the operand type (row pitch N), or
     int8_t* zcodes; uint8_t* zscales; int64_t zpitch;   // as 8-bit checkpoint
-    int stochastic; PhiloxKeys rk;
+    int stochastic; Noise8 noise;
     float* partial;                           // [splits][M][pitchN] fp32
     int64_t ldp;
     SideJob side;
@@ -229,11 +229,12 @@ __device__ __forceinline__ void linear_epilogue32(const GemmArgs& a, int64_t row
                 w[i] = pack4(__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y));
             }
         } else {
+            const uint2 high = a.noise.high();
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 uint32_t c[4];
                 uint4 r = make_uint4(0u, 0u, 0u, 0u);
-                if (a.stochastic) r = noise8(a.rk, at / 8 + i / 2);
+                if (a.stochastic) r = noise8(a.noise, high, at / 8 + i / 2);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float z = (j & 1) ? v[2 * i + j / 2].y : v[2 * i + j / 2].x;
@@ -300,6 +301,7 @@ __device__ __forceinline__ void side_job(const SideJob& j, int w, int n) {
     }
     const int64_t total = j.rows * j.chunks;
     if (j.kind == 1) {
+        const uint2 high = j.noise.high();
         for (int64_t i0 = (int64_t)w * 32 * U; i0 < total; i0 += (int64_t)n * 32 * U) {
             uint32_t raw[U][4];
 #pragma unroll
@@ -324,7 +326,7 @@ __device__ __forceinline__ void side_job(const SideJob& j, int w, int n) {
                 raw_to_pairs<DT>(raw[u], v);
                 uint32_t byte;
                 const uint32_t m = absmax8<DT>(raw[u]);
-                const uint2 q = j.stochastic ? codes8<true>(v, m, j.rk, (uint64_t)i, byte, top_byte8<DT>()) : codes8<false>(v, m, j.rk, (uint64_t)i, byte, top_byte8<DT>());
+                const uint2 q = j.stochastic ? codes8<true>(v, m, j.noise, high, (uint64_t)i, byte, top_byte8<DT>()) : codes8<false>(v, m, j.noise, high, (uint64_t)i, byte, top_byte8<DT>());
                 if (i < total) {
                     st_stream_u2(j.codes + i * 8, q);
                     if ((lane & 3) == 0) j.scales[i >> 2] = (uint8_t)byte;
@@ -948,11 +950,12 @@ static bool beside(int kind, int64_t M, int64_t N, int64_t K, int64_t elements) 
 
 extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
                            int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* xcodes, void* xscales, void* z, void* zcodes,
-                           void* zscales, int stochastic, uint64_t seed, void* scratch, void* stream) {
+                           void* zscales, int rounding, uint64_t seed, void* scratch, void* stream) {
     if (dtype != GACT_F16 && dtype != GACT_BF16) return GACT_ERR_DTYPE;
     if (act < GACT_ACT_NONE || act > GACT_ACT_SILU) return GACT_ERR_MODE;
     if (!dims_ok(rows, cin, cout) || ld_x < cin || ld_w < cin || (residual && ld_res < cout)) return GACT_ERR_SIZE;
     if (rows == 0) return GACT_OK;
+    if (const int st = rounding_status(rounding, seed, GACT_CODES_STOCHASTIC | GACT_CODES_DEVICE_SEED)) return st;
     if (!x || !weight || !y || (xcodes && !xscales) || (zcodes && !zscales)) return GACT_ERR_NULL;
     if (!map_ok(x, ld_x) || !map_ok(weight, ld_w) || (((uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)residual) & 1) ||
         ((uintptr_t)zcodes & 31) || ((uintptr_t)xcodes & 31) || ((uintptr_t)scratch & 31))
@@ -965,15 +968,16 @@ extern "C" int gact_linear(const void* x, int64_t ld_x, const void* weight, int6
     a.act = act; a.z = z; a.zvec = vec_bytes(z, cout);
     a.zcodes = (int8_t*)zcodes; a.zscales = (uint8_t*)zscales; a.zpitch = pitch8(cout);
     // the codes of the pre-activation draw their noise from another key than those of the input
-    a.stochastic = stochastic; a.rk = philox_round_keys(seed + 0x9E3779B97F4A7C15ull);
+    const bool stochastic = rounding & GACT_CODES_STOCHASTIC, on_device = rounding & GACT_CODES_DEVICE_SEED;
+    a.stochastic = stochastic; a.noise = Noise8::of(seed, on_device, 0x9E3779B97F4A7C15ull);
     if (xcodes) {
         if (beside(1, rows, cout, cin, rows * cin)) {
             SideJob& j = a.side;
-            j.kind = 1; j.x = x; j.ld = ld_x; j.stochastic = stochastic; j.rk = philox_round_keys(seed);
+            j.kind = 1; j.x = x; j.ld = ld_x; j.stochastic = stochastic; j.noise = Noise8::of(seed, on_device, 0);
             j.codes = (int8_t*)xcodes; j.scales = (uint8_t*)xscales; j.rows = rows; j.cols = (int)cin; j.chunks = (int)(pitch8(cin) / 8);
             j.by = Divisor::of(j.chunks);
         } else {
-            const int st = gact_checkpoint8(x, dtype, rows, cin, ld_x, stochastic, seed, xcodes, xscales, stream);
+            const int st = gact_checkpoint8(x, dtype, rows, cin, ld_x, rounding, seed, xcodes, xscales, stream);
             if (st != GACT_OK) return st;
         }
     }

@@ -75,8 +75,9 @@ def _unwrap(kept):
 def op_checkpoint8(input, seed=None):
     """8-bit checkpoint of a float32 / float16 / bfloat16 tensor, blocks of 32 along its last dimension.
 
-    Rounds to nearest, or with a ``seed`` stochastically (unbiased; the same seed gives the same codes).  A block that
-    holds a NaN or an infinity restores to NaN throughout."""
+    Rounds to nearest, or with a ``seed`` stochastically (unbiased; the same seed gives the same codes).  A seed is a number, or
+    an int64 tensor of one element on the input's device, which the kernel reads: in a captured graph a number is repeated by
+    every replay, a tensor's value is that of the replay.  A block that holds a NaN or an infinity restores to NaN throughout."""
     return Checkpoint8(_fused.checkpoint8(input, seed), input.shape, input.dtype)
 
 

@@ -24,13 +24,17 @@ from gact.fused import Checkpoint8, LayerNormSaved, LinearSaved
 _calls = 0
 
 
-def _next_seed():
-    """None (round to nearest), or a seed of its own for every call: from torch's seed, the rank and a running number."""
+def _next_seed(device=None):
+    """None (round to nearest), or a seed of its own for every call: from torch's seed, the rank and a running number.  While the
+    device's stream is captured it is drawn on the device by torch's generator, whose state moves on from replay to replay."""
     if not config.stochastic_checkpoints:
         return None
     global _calls
     _calls += 1
     rank = torch.distributed.get_rank() if torch.distributed.is_available() and torch.distributed.is_initialized() else 0
+    if device is not None and torch.cuda.is_current_stream_capturing():
+        seed = torch.empty(1, dtype=torch.int64, device=device).random_()
+        return seed.add_(rank << 40) if rank else seed
     return (torch.initial_seed() * 0x9E3779B97F4A7C15 + (rank << 40) + 2 * _calls) & 0xFFFFFFFFFFFFFFFF
 
 
@@ -106,7 +110,7 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
     if not _keeps_graph(input, weight, bias):
         return fused.op_layer_norm(input, weight, bias, eps, save=False)[0]
     compress = config.compress_activation if compress is None else compress
-    return _LayerNorm.apply(input, weight, bias, eps, compress, _next_seed() if compress else None)
+    return _LayerNorm.apply(input, weight, bias, eps, compress, _next_seed(input.device) if compress else None)
 
 
 def _autocast(*tensors):
@@ -140,7 +144,7 @@ def linear(input, weight, bias=None, activation=None, residual=None, compress=No
         if checkpoint.shape != input.shape or checkpoint.dtype != input.dtype:
             raise ValueError("checkpoint is of a %s tensor of shape %s" % (checkpoint.dtype, tuple(checkpoint.shape)))
         given = checkpoint.buf
-    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed() if compress else None, given,
+    return _Linear.apply(input, weight, bias, residual, activation, compress, _next_seed(input.device) if compress else None, given,
                          not isinstance(weight, nn.Parameter) if keep_input is None else keep_input)
 
 
@@ -190,7 +194,7 @@ def share_input(parent, children):
         if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(*(c.weight for c in children)):
             cast = _autocast(x)[0]
             if cast.dtype in (torch.float16, torch.bfloat16):
-                ck = fused.op_checkpoint8(cast.detach(), _next_seed())
+                ck = fused.op_checkpoint8(cast.detach(), _next_seed(x.device))
                 for c in children:
                     c._shared = (ck, x, x._version)
 

@@ -248,8 +248,10 @@ int gact_calc_precision_host(int32_t* b, const float* C, const int64_t* w, int L
  * the largest |x| stays below 127 steps; b = 255 marks a block that held a NaN or an infinity, all of it restores to NaN.
  * codes: int8[rows][pitch], pitch = gact_checkpoint8_pitch(cols) = cols rounded up to 32, codes past `cols` are 0;
  * scales: uint8[rows][pitch / 32].  In the highest binade of the type codes stop at +-63 (64 would restore out of range).
- * stochastic != 0: code = floor(x * 2^(127-b) + u) with u in (0,1) from Philox4x32-7 keyed by `seed`, counter = index of
- * the element's group of 8 in the padded layout, 16 bits each; the restored value is then unbiased.
+ * rounding: 0, or GACT_CODES_STOCHASTIC: code = floor(x * 2^(127-b) + u) with u in (0,1) from Philox4x32-7 keyed by `seed`,
+ * low half of the counter = index of the element's group of 8 in the padded layout, 16 bits each; the restored value is then
+ * unbiased.  With GACT_CODES_DEVICE_SEED too, `seed` is the address of 8 bytes on the device (8-byte aligned), read by the kernel: they
+ * are the high half of the counter and the key is 0.  A captured launch repeats the seed that it was given, but reads new ones there.
  *
  * Sizes: cols (and the features of a linear layer) at most GACT_MAX_COLS, rows * pitch at most GACT_MAX_ELEMENTS, layer
  * norm rows of at most GACT_LAYER_NORM_MAX_COLS.  `ld` arguments are row pitches in elements (>= the row length).
@@ -261,14 +263,14 @@ int gact_calc_precision_host(int32_t* b, const float* C, const int64_t* w, int L
 #define GACT_MAX_ELEMENTS (1LL << 38)
 #define GACT_LAYER_NORM_MAX_COLS 16384
 
-/* how gact_layer_norm makes its codes */
-enum { GACT_CODES_STOCHASTIC = 1, GACT_CODES_CENTERED = 4 };
+/* how codes are made; GACT_CODES_CENTERED is gact_layer_norm's alone */
+enum { GACT_CODES_STOCHASTIC = 1, GACT_CODES_DEVICE_SEED = 2, GACT_CODES_CENTERED = 4 };
 
 /* activations of gact_linear; GELU is the erf form, GELU_TANH its tanh approximation */
 enum { GACT_ACT_NONE = 0, GACT_ACT_RELU = 1, GACT_ACT_GELU = 2, GACT_ACT_GELU_TANH = 3, GACT_ACT_SILU = 4 };
 
 int64_t gact_checkpoint8_pitch(int64_t cols);
-int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int stochastic, uint64_t seed,
+int gact_checkpoint8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int rounding, uint64_t seed,
                      void* codes, void* scales, void* stream);
 int gact_restore8(const void* codes, const void* scales, int64_t rows, int64_t cols, int dtype, void* out, int64_t ld,
                   void* stream);
@@ -280,7 +282,7 @@ int gact_repitch16(const void* src, int64_t ld, int64_t rows, int64_t cols, void
  * Layer norm over rows of `cols`: y = (x - mean) / sqrt(var + eps) * weight + bias; weight / bias may be null, their type
  * is `param_dtype` (that of x, or GACT_F32).  y is contiguous.  stats (optional, 8-byte aligned): (mean, 1 / deviation)
  * per row in fp32, for the backward pass.  codes / scales (optional): checkpoint of x, made in the same pass.
- * rounding: 0, or GACT_CODES_STOCHASTIC, and with GACT_CODES_CENTERED the codes are those of x - mean (an fp32 tensor) and
+ * rounding: as above, and with GACT_CODES_CENTERED the codes are those of x - mean (an fp32 tensor) and
  * stats hold (0, 1 / deviation): what the backward pass takes off the kept values.  Codes of x itself are as coarse as the
  * largest |x| of their block; in rows whose mean is large against their deviation that leaves little of x - mean.
  */
@@ -308,7 +310,7 @@ int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows, int64_t co
 int64_t gact_linear_scratch_bytes(int64_t rows, int64_t cin, int64_t cout, int direction);
 int gact_linear(const void* x, int64_t ld_x, const void* weight, int64_t ld_w, const void* bias, const void* residual, int64_t ld_res,
                 int dtype, int64_t rows, int64_t cin, int64_t cout, int act, void* y, void* xcodes, void* xscales, void* z, void* zcodes,
-                void* zscales, int stochastic, uint64_t seed, void* scratch, void* stream);
+                void* zscales, int rounding, uint64_t seed, void* scratch, void* stream);
 /*
  * dz = dy act'(z) with z given as a tensor or (z null) as a checkpoint; with GACT_ACT_NONE dz is a copy of dy (to another row
  * pitch), or null.  scratch (optional): partial sums of dz over the rows, added from the unrounded products;

@@ -169,3 +169,18 @@ def test_a_wider_residual_keeps_its_type_under_autocast(plain, autocast):
         assert layers.linear(x, w, residual=torch.randn(5, 4)).dtype == torch.float32
     with pytest.raises(ValueError, match="residual must have shape"):
         layers.linear(x, w, residual=torch.randn(4))
+
+
+def test_entry_points_refuse_unknown_ways_of_rounding():
+    import ctypes
+    from gact import _native as nv
+    b = ctypes.create_string_buffer(1 << 14)
+    p = (ctypes.addressof(b) + 255) & ~255
+    L = nv.lib
+    calls = [lambda r, seed: L.gact_checkpoint8(p, 0, 2, 32, 32, r, seed, p, p, None),
+             lambda r, seed: L.gact_layer_norm(p, 2, 2, 32, 32, p, p, 2, 1e-5, p, p, p, p, r, seed, None),
+             lambda r, seed: L.gact_linear(p, 64, p, 64, p, None, 0, 2, 4, 64, 32, 2, p, p, p, None, p, p, r, seed, p, None)]
+    for i, f in enumerate(calls):
+        for r in (2, 8, 6, -1) + (() if i == 1 else (4, 5)):
+            assert f(r, p) == 6
+        assert f(3, 0) == 3 and f(3, p + 4) == 4             # a seed on the device has an address of 8 bytes
