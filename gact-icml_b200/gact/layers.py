@@ -174,7 +174,8 @@ class Linear(nn.Linear):
     def forward(self, input, residual=None):
         shared, self._shared = self._shared, None
         checkpoint = None
-        if shared is not None and shared[1] is input and shared[2] == input._version:
+        # (made in the type that the parent was called under: a forward pass that enters autocast by itself computes in another)
+        if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast(input)[0].dtype:
             checkpoint = shared[0]
         return linear(input, self.weight, self.bias, self.activation, residual, checkpoint=checkpoint)
 

@@ -184,3 +184,43 @@ def test_entry_points_refuse_unknown_ways_of_rounding():
         for r in (2, 8, 6, -1) + (() if i == 1 else (4, 5)):
             assert f(r, p) == 6
         assert f(3, 0) == 3 and f(3, p + 4) == 4             # a seed on the device has an address of 8 bytes
+
+
+class Attention(torch.nn.Module):
+    """Two layers on one input, as query and key are."""
+
+    def __init__(self, inside=None):
+        super().__init__()
+        self.a, self.b, self.inside = layers.Linear(8, 8), layers.Linear(8, 8), inside
+
+    def forward(self, x):
+        if self.inside is not None:
+            self.inside()
+        return self.a(x) + self.b(x)
+
+
+@pytest.fixture
+def checkpoints(monkeypatch):
+    """op_checkpoint8 without a device; the checkpoints that were made."""
+    made = []
+
+    def op_checkpoint8(x, seed=None):
+        made.append(fused.Checkpoint8(torch.zeros(x.numel() * 33 // 32, dtype=torch.int8), x.shape, x.dtype))
+        return made[-1]
+
+    monkeypatch.setattr(fused, "op_checkpoint8", op_checkpoint8)
+    return made
+
+
+def test_share_input_when_the_forward_pass_enters_another_autocast(plain, checkpoints, monkeypatch):
+    """The shared checkpoint is of the type outside; layers that compute in another one keep their own instead of failing."""
+    def enter():
+        monkeypatch.setattr(torch, "is_autocast_enabled", lambda device: True)
+        monkeypatch.setattr(torch, "get_autocast_dtype", lambda device: torch.float16)
+
+    m = Attention(enter).bfloat16()
+    layers.share_input(m, (m.a, m.b))
+    x = torch.zeros(4, 8, dtype=torch.bfloat16, requires_grad=True)
+    assert m(x).dtype == torch.float16 and len(checkpoints) == 1
+    assert [c["checkpoint"] for c in plain] == [None, None]
+    monkeypatch.undo()
