@@ -175,7 +175,9 @@ class Linear(nn.Linear):
         shared, self._shared = self._shared, None
         checkpoint = None
         # (made in the type that the parent was called under: a forward pass that enters autocast by itself computes in another)
-        if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast(input)[0].dtype:
+        # and on its stream: a layer run on another one may come before it and outlive it
+        if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast(input)[0].dtype \
+                and shared[3] == _stream(input):
             checkpoint = shared[0]
         return linear(input, self.weight, self.bias, self.activation, residual, checkpoint=checkpoint)
 
@@ -183,10 +185,14 @@ class Linear(nn.Linear):
         return super().extra_repr() + ("" if self.activation is None else ", activation=%s" % self.activation)
 
 
+def _stream(x):
+    return torch.cuda.current_stream(x.device) if x.is_cuda else None
+
+
 def share_input(parent, children):
     """Lets linear layers that ``parent`` calls with its own first argument share one checkpoint of it (the query, key and
     value layers of an attention block): made when ``parent`` is called, used by the next call of each child that is given
-    that very tensor, unmodified, and dropped when ``parent`` returns."""
+    that very tensor, unmodified, on the same stream, and dropped when ``parent`` returns."""
     children = list(children)
 
     def before(module, args):
@@ -197,7 +203,7 @@ def share_input(parent, children):
             if cast.dtype in (torch.float16, torch.bfloat16):
                 ck = fused.op_checkpoint8(cast.detach(), _next_seed(x.device))
                 for c in children:
-                    c._shared = (ck, x, x._version)
+                    c._shared = (ck, x, x._version, _stream(x))
 
     def after(module, args, output):
         for c in children:
