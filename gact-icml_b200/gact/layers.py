@@ -189,28 +189,35 @@ def _stream(x):
     return torch.cuda.current_stream(x.device) if x.is_cuda else None
 
 
+class _SharedInput:
+    """The hooks of ``share_input``: an object whose methods they are, so that a copied or pickled parent has its own, with its own
+    layers."""
+
+    def __init__(self, children):
+        self.children = list(children)
+
+    def before(self, module, args):
+        x = args[0] if args else None
+        # (frozen weights keep no input)
+        if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(*(c.weight for c in self.children)):
+            cast = _autocast(x)[0]
+            if cast.dtype in (torch.float16, torch.bfloat16):
+                ck = fused.op_checkpoint8(cast.detach(), _next_seed(x.device))
+                for c in self.children:
+                    c._shared = (ck, x, x._version, _stream(x))
+
+    def after(self, module, args, output):
+        for c in self.children:
+            c._shared = None
+
+
 def share_input(parent, children):
     """Lets linear layers that ``parent`` calls with its own first argument share one checkpoint of it (the query, key and
     value layers of an attention block): made when ``parent`` is called, used by the next call of each child that is given
     that very tensor, unmodified, on the same stream, and dropped when ``parent`` returns."""
-    children = list(children)
-
-    def before(module, args):
-        x = args[0] if args else None
-        # (frozen weights keep no input)
-        if isinstance(x, torch.Tensor) and config.compress_activation and _keeps_graph(*(c.weight for c in children)):
-            cast = _autocast(x)[0]
-            if cast.dtype in (torch.float16, torch.bfloat16):
-                ck = fused.op_checkpoint8(cast.detach(), _next_seed(x.device))
-                for c in children:
-                    c._shared = (ck, x, x._version, _stream(x))
-
-    def after(module, args, output):
-        for c in children:
-            c._shared = None
-
-    parent.register_forward_pre_hook(before)
-    parent.register_forward_hook(after, always_call=True)
+    shared = _SharedInput(children)
+    parent.register_forward_pre_hook(shared.before)
+    parent.register_forward_hook(shared.after, always_call=True)
 
 
 def activation_name(module):

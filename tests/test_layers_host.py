@@ -224,3 +224,24 @@ def test_share_input_when_the_forward_pass_enters_another_autocast(plain, checkp
     assert m(x).dtype == torch.float16 and len(checkpoints) == 1
     assert [c["checkpoint"] for c in plain] == [None, None]
     monkeypatch.undo()
+
+
+@pytest.mark.parametrize("way", ["deepcopy", "pickle"])
+def test_a_copy_shares_among_its_own_layers(plain, checkpoints, way):
+    import copy
+    import io
+    m = Attention().bfloat16()
+    layers.share_input(m, (m.a, m.b))
+    if way == "deepcopy":
+        twin = copy.deepcopy(m)
+    else:
+        file = io.BytesIO()
+        torch.save(m, file)
+        file.seek(0)
+        twin = torch.load(file, weights_only=False)
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    twin(x)
+    assert len(checkpoints) == 1 and [c["checkpoint"].buf.data_ptr() for c in plain] == [checkpoints[0].buf.data_ptr()] * 2
+    assert all(c._shared is None for c in (m.a, m.b, twin.a, twin.b))
+    m(x)
+    assert len(checkpoints) == 2 and [c["checkpoint"].buf.data_ptr() for c in plain[2:]] == [checkpoints[1].buf.data_ptr()] * 2
