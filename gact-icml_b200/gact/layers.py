@@ -13,6 +13,8 @@ nearest.
 Linear layers compute in float16 / bfloat16 (under autocast input and parameters are cast to its type, as torch does); layer norm
 keeps the type of its input (torch's returns float32 under autocast).
 """
+import math
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -248,10 +250,11 @@ def _as_layer_norm(m):
 def convert(module):
     """Replaces, in place, every nn.LayerNorm and nn.Linear under ``module`` by the layers above, which take over the very
     parameters; a GELU / ReLU / SiLU that follows a Linear inside an nn.Sequential moves into its epilogue.  Subclasses of
-    nn.Linear / nn.LayerNorm, and layers that carry hooks, stay as they are.  Returns ``module`` (or its replacement)."""
+    nn.Linear / nn.LayerNorm, layers that carry hooks, and norms over more elements than the operator takes (16384) stay as they are.
+    Returns ``module`` (or its replacement)."""
     if type(module) is nn.Linear and not _hooked(module):
         return _as_linear(module)
-    if type(module) is nn.LayerNorm and not _hooked(module):
+    if type(module) is nn.LayerNorm and not _hooked(module) and math.prod(module.normalized_shape) <= fused.LAYER_NORM_MAX_COLS:
         return _as_layer_norm(module)
     names = list(module._modules)
     for i, name in enumerate(names):

@@ -245,3 +245,12 @@ def test_a_copy_shares_among_its_own_layers(plain, checkpoints, way):
     assert all(c._shared is None for c in (m.a, m.b, twin.a, twin.b))
     m(x)
     assert len(checkpoints) == 2 and [c["checkpoint"].buf.data_ptr() for c in plain[2:]] == [checkpoints[1].buf.data_ptr()] * 2
+
+
+def test_convert_leaves_norms_that_are_too_long():
+    """What ran before conversion runs after it: the operator takes rows of at most 16384."""
+    m = torch.nn.Sequential(torch.nn.LayerNorm(16385), torch.nn.LayerNorm((128, 129)), torch.nn.LayerNorm((128, 128)), torch.nn.LayerNorm(16384))
+    layers.convert(m)
+    assert [type(c) is layers.LayerNorm for c in m] == [False, False, True, True]
+    x = torch.randn(2, 16385)
+    assert torch.equal(m[0](x), torch.nn.functional.layer_norm(x, (16385,)))
