@@ -1,4 +1,6 @@
 """Bounded waits of the products and of layer norm's rings: the limit that is asked for, and who learns of a wait that ran out."""
+import gc
+
 import pytest
 import torch
 
@@ -59,10 +61,12 @@ def test_the_next_call_says_that_a_copy_was_lost(withheld, first, second):
     calls = {"checkpoint": lambda: fused.op_checkpoint8(x[:4]).buf, "restore": lambda: fused.op_restore8(c), "norm": lambda: fused.op_layer_norm(x[:4])[0],
              "norm backward": lambda: fused.op_layer_norm_backward(x, norm)[0], "linear": lambda: fused.op_linear(x, w)[0],
              "linear backward": lambda: fused.op_linear_backward(y, lin)[1]}
+    gc.collect()                                   # (no graph of another test may be collected inside the capture)
     graph = torch.cuda.CUDAGraph()
+    norm_call = calls["norm"]
     with torch.cuda.graph(graph):
-        captured = calls["norm"]()
-    calls["replay"] = lambda: (graph.replay(), calls["norm"](), captured)[2]
+        captured = norm_call()
+    calls["replay"] = lambda: (graph.replay(), norm_call(), captured)[2]
     want = {k: f().clone() for k, f in calls.items()}
     torch.cuda.synchronize()
     withheld(2000)

@@ -1,4 +1,5 @@
 """Seeds of stochastic checkpoints that lie on the device, and captured steps whose replays draw new noise."""
+import gc
 import math
 
 import pytest
@@ -109,6 +110,7 @@ def test_replays_of_a_captured_step_draw_new_noise():
     with torch.cuda.stream(side):
         step()
     torch.cuda.current_stream().wait_stream(side)
+    gc.collect()                                   # (no graph of another test may be collected inside the capture)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         out = step()
