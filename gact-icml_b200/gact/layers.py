@@ -108,7 +108,11 @@ class _Linear(torch.autograd.Function):
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
     """Layer norm over the last dimension, differentiable; what it keeps is decided by ``compress`` (None: by the level,
-    ``config.compress_activation``): the checkpoint of the input minus its row's mean, or the input itself."""
+    ``config.compress_activation``): the checkpoint of the input minus its row's mean, or the input itself.  Parameters are of
+    the input's type or float32; under autocast others (bfloat16 ones with a float32 input, say) are widened to float32."""
+    params = [p for p in (weight, bias) if p is not None]
+    if torch.is_autocast_enabled("cuda") and any(p.dtype not in (input.dtype, torch.float32) or p.dtype != params[0].dtype for p in params):
+        weight, bias = (p if p is None or p.dtype == torch.float64 else p.float() for p in (weight, bias))
     if not _keeps_graph(input, weight, bias):
         return fused.op_layer_norm(input, weight, bias, eps, save=False)[0]
     compress = config.compress_activation if compress is None else compress
