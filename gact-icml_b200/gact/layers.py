@@ -254,11 +254,13 @@ def _as_layer_norm(m):
 def convert(module):
     """Replaces, in place, every nn.LayerNorm and nn.Linear under ``module`` by the layers above, which take over the very
     parameters; a GELU / ReLU / SiLU that follows a Linear inside an nn.Sequential moves into its epilogue.  Subclasses of
-    nn.Linear / nn.LayerNorm, layers that carry hooks, and norms over more elements than the operator takes (16384) stay as they are.
-    Returns ``module`` (or its replacement)."""
-    if type(module) is nn.Linear and not _hooked(module):
+    nn.Linear / nn.LayerNorm, layers that carry hooks, layers in float64 and norms over more elements than the operator takes (16384) stay as
+    they are.  Returns ``module`` (or its replacement)."""
+    if _hooked(module) or any(p.dtype == torch.float64 for p in module._parameters.values() if p is not None):
+        pass
+    elif type(module) is nn.Linear:
         return _as_linear(module)
-    if type(module) is nn.LayerNorm and not _hooked(module) and math.prod(module.normalized_shape) <= fused.LAYER_NORM_MAX_COLS:
+    elif type(module) is nn.LayerNorm and math.prod(module.normalized_shape) <= fused.LAYER_NORM_MAX_COLS:
         return _as_layer_norm(module)
     names = list(module._modules)
     for i, name in enumerate(names):

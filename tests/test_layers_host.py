@@ -254,3 +254,11 @@ def test_convert_leaves_norms_that_are_too_long():
     assert [type(c) is layers.LayerNorm for c in m] == [False, False, True, True]
     x = torch.randn(2, 16385)
     assert torch.equal(m[0](x), torch.nn.functional.layer_norm(x, (16385,)))
+
+
+def test_convert_leaves_float64_layers():
+    """The operators have no float64: a head in double precision under a converted body goes on running."""
+    m = torch.nn.Sequential(torch.nn.Linear(4, 4), torch.nn.Sequential(torch.nn.LayerNorm(4), torch.nn.Linear(4, 2), torch.nn.ReLU()).double())
+    layers.convert(m)
+    assert type(m[0]) is layers.Linear and type(m[1][0]) is torch.nn.LayerNorm and type(m[1][1]) is torch.nn.Linear and type(m[1][2]) is torch.nn.ReLU
+    assert m[1](torch.randn(3, 4, dtype=torch.float64)).dtype == torch.float64
