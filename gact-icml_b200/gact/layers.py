@@ -268,7 +268,8 @@ def convert(module):
         if child is None:
             continue
         new = convert(child)
-        if type(module) is nn.Sequential and type(new) is Linear and new.activation is None and i + 1 < len(names):
+        # (a layer that was one of these before may be used, or watched by hooks, elsewhere too: it keeps its output)
+        if type(module) is nn.Sequential and new is not child and type(new) is Linear and i + 1 < len(names):
             act = activation_name(module._modules[names[i + 1]])
             if act is not None and not _hooked(module._modules[names[i + 1]]):
                 new.activation = act

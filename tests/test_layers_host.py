@@ -262,3 +262,16 @@ def test_convert_leaves_float64_layers():
     layers.convert(m)
     assert type(m[0]) is layers.Linear and type(m[1][0]) is torch.nn.LayerNorm and type(m[1][1]) is torch.nn.Linear and type(m[1][2]) is torch.nn.ReLU
     assert m[1](torch.randn(3, 4, dtype=torch.float64)).dtype == torch.float64
+
+
+def test_convert_does_not_move_an_activation_into_a_layer_that_is_used_elsewhere():
+    own = layers.Linear(4, 4)
+    seen = []
+    own.register_forward_hook(lambda m, a, y: seen.append(y))
+    m = torch.nn.ModuleList([torch.nn.Sequential(own, torch.nn.ReLU()), own])
+    layers.convert(m)
+    assert m[0][0] is own is m[1] and own.activation is None and type(m[0][1]) is torch.nn.ReLU
+    lin = torch.nn.Linear(4, 4)
+    m = torch.nn.ModuleList([torch.nn.Sequential(lin, torch.nn.ReLU()), lin])
+    layers.convert(m)
+    assert m[0][0].activation == "relu" and m[1].activation is None and m[0][0].weight is m[1].weight is lin.weight
