@@ -232,7 +232,7 @@ struct LnBwdArgs {
     uint32_t wait_limit; int withhold; int* report;    // rings: bounded waits; diagnostics; the host's word
 };
 
-// For short rows, few rows and rows that do not start on 16-byte boundaries.  A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
+// Wherever the rings below were not measured to be faster.  A thread owns CH fixed chunks of 8 columns, so the weight gradients of a block's rows stay in its registers; a block
 // walks the rows, R of them (per row group) side by side: one barrier serves 2 R sums, and the next R rows' loads are issued
 // before the current ones are worked on.  Block sums go to `partial`, added up in a fixed order afterwards: no atomics.
 template <int DT, int TPR, int CH, int R, bool VEC, bool COMP>
@@ -456,13 +456,13 @@ template <int DT> __device__ __forceinline__ void take_raw(const uint8_t* row, i
     }
 }
 
-// dy and the codes of a row (or x) are read twice, before and after the sums; the weight gradients of a thread's columns stay
-// in its registers.
-template <int DT, int TPR, int CH, bool COMP>
+// dy and the codes of a row are read twice, before and after the sums; the weight gradients of a thread's columns stay in its
+// registers.
+template <int DT, int TPR, int CH>
 __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __grid_constant__ LnBwdArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int W = TPR * CH * 8, WARPS = TPR / 32, N = RawRegs<DT>::N;
-    constexpr int YROW = W * Elem<DT>::kBytes, XROW = COMP ? W : YROW, ROW = YROW + XROW;
+    constexpr int YROW = W * Elem<DT>::kBytes, ROW = YROW + W;
     extern __shared__ __align__(128) uint8_t dyn[];               // weights (fp32), rings
     float* pw = (float*)dyn;
     __shared__ __align__(8) uint64_t bars[kRingStages];
@@ -479,15 +479,14 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
     RowRing r{smem_addr(bars), a.wait_limit, &dead, 0, 0};
     const int64_t step = gridDim.x;
     int64_t row = blockIdx.x;
-    const uint32_t ybytes = (uint32_t)a.cols * Elem<DT>::kBytes, xbytes = COMP ? (uint32_t)a.chunks * 8 : ybytes;
+    const uint32_t ybytes = (uint32_t)a.cols * Elem<DT>::kBytes, xbytes = (uint32_t)a.chunks * 8;
     auto issue = [&](int64_t w) {
         // (a ring that gave up issues nothing more: announcing bytes on a phase that never completed would be a second arrival
         // on it, which faults)
         if (w < a.rows && !dead) {
             const uint32_t s = r.announce(ybytes + xbytes), to = smem_addr(ring + s * ROW), bar = r.bar + 8 * s;
             if (!(a.withhold && w == 0)) bulk_copy(to, (const T*)a.dy + w * a.ldy, ybytes, bar);      // (withhold: diagnostics)
-            if (COMP) bulk_copy(to + YROW, a.codes + w * a.chunks * 8, xbytes, bar);
-            else bulk_copy(to + YROW, (const T*)a.x + w * a.ldx, xbytes, bar);
+            bulk_copy(to + YROW, a.codes + w * a.chunks * 8, xbytes, bar);
         }
     };
     if (t == 0)
@@ -498,12 +497,10 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
     auto fetch = [&](int64_t w) {
         if (w < a.rows) {
             ps = ld_ahead_float2((const float2*)a.stats + w);
-            if (COMP) {
-                const uint8_t* p = a.scales + ((w * a.chunks + t) >> 2);
+            const uint8_t* p = a.scales + ((w * a.chunks + t) >> 2);
 #pragma unroll
-                for (int c = 0; c < CH; c++)
-                    if (t + c * TPR < a.chunks) pe[c] = ld_ahead_byte(p + c * (TPR / 4));
-            }
+            for (int c = 0; c < CH; c++)
+                if (t + c * TPR < a.chunks) pe[c] = ld_ahead_byte(p + c * (TPR / 4));
         }
     };
 #pragma unroll
@@ -521,7 +518,7 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
         const float rs = ps.y, off = -ps.x * ps.y;
         float up[CH];
 #pragma unroll
-        for (int c = 0; c < CH; c++) up[c] = COMP ? scale_down8(pe[c]) * rs : rs;
+        for (int c = 0; c < CH; c++) up[c] = scale_down8(pe[c]) * rs;
         fetch(row + step);
         const uint8_t* in = ring + r.take() * ROW;
         // dy and x^ of chunk c: x^ = x' r - mean r; a code is a small integer and its scale a power of two, so x' r is one product
@@ -529,12 +526,7 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
             uint32_t raw[N];
             take_raw<DT>(in, t + c * TPR, raw);
             raw_to_pairs<DT>(raw, g);
-            if constexpr (COMP) {
-                code_pairs(*(const uint2*)(in + YROW + (t + c * TPR) * 8), xh);
-            } else {
-                take_raw<DT>(in + YROW, t + c * TPR, raw);
-                raw_to_pairs<DT>(raw, xh);
-            }
+            code_pairs(*(const uint2*)(in + YROW + (t + c * TPR) * 8), xh);
 #pragma unroll
             for (int i = 0; i < 4; i++) xh[i] = fma2(xh[i], splat2(up[c]), splat2(off));
         };
@@ -606,35 +598,40 @@ __global__ void __launch_bounds__(TPR) layer_norm_backward_ring_kernel(const __g
     }
 }
 
-// Rings need rows long enough to be worth a copy each, and several rows per block to run ahead.
-static bool ln_ring(bool vec, int64_t rows, int64_t cols) { return vec && cols > 1024 && cols <= 8192 && rows > (int64_t)sm_count() * 8; }
+// Rings take the place of the plain kernel's shape of 512 threads a row, where many rows let a block run ahead.  Measured, ring / plain
+// in us, from codes: bf16 4800 x 2056 21.7 / 27.6, 4800 x 4096 31.9 / 30.7, 8192 x 3200 38.3 / 44.2, 65536 x 4096 266 / 316; fp32 (twice
+// the bytes per row) 8192 x 4096 67 / 63, 16384 x 4096 115 / 116, 65536 x 4096 408 / 467.  At 2400 rows they lose (4096 columns
+// 25.5 / 21), with other shapes of the plain kernel too (65536 x 2048 175 / 140, x 1024 127 / 72, x 8192 693 / 522), and from x
+// itself (65536 x 4096 329 / 290).  The diagnostics hook, which is there to see a copy lost, takes them wherever they fit.
+constexpr int kRingCols = 4096;
+static bool ln_ring(bool vec, bool codes, int dtype, int64_t rows, int64_t cols, bool forced) {
+    if (!vec || !codes || cols > kRingCols) return false;
+    return forced || (cols > 2048 && rows > (int64_t)sm_count() * (dtype == GACT_F32 ? 96 : 32));
+}
 
 // Shapes and blocks of the backward pass.  The number of blocks decides how many partial sums there are (2 x cols floats per
 // block), so it must not depend on anything but the sizes: 512 threads per SM for the plain kernel, and for the rings as many
 // blocks as their registers and shared memory let an SM hold.
-struct LnBwdShape { bool ring; int tpr, block, rows_per_step, per_sm; };
-static LnBwdShape ln_bwd_shape(bool vec, int64_t rows, int64_t cols) {
-    if (ln_ring(vec, rows, cols)) return cols <= 4096 ? LnBwdShape{true, 128, 128, 1, 4} : LnBwdShape{true, 512, 512, 1, 1};
+struct LnBwdShape { int block, rows_per_step, per_sm; };
+static LnBwdShape ln_bwd_shape(bool ring, int64_t cols) {
+    if (ring) return {128, 1, 4};
     const int tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
     const int block = tpr > 32 ? tpr : 128;
-    return {false, tpr, block, block / tpr * (cols <= 4096 ? kLnBwdRows : 1), 512 / block};
+    return {block, block / tpr * (cols <= 4096 ? kLnBwdRows : 1), 512 / block};
 }
-static int64_t ln_bwd_blocks(bool vec, int64_t rows, int64_t cols) {
-    const LnBwdShape p = ln_bwd_shape(vec, rows, cols);
+static int64_t ln_bwd_blocks(bool ring, int64_t rows, int64_t cols) {
+    const LnBwdShape p = ln_bwd_shape(ring, cols);
     const int64_t want = (rows + p.rows_per_step - 1) / p.rows_per_step, most = (int64_t)sm_count() * p.per_sm;
     return want < most ? want : most;
 }
 
-template <int DT, int TPR, int CH, bool COMP> static int launch_ln_bwd_ring_kernel(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
-    auto* k = layer_norm_backward_ring_kernel<DT, TPR, CH, COMP>;
-    constexpr int W = TPR * CH * 8, E = Elem<DT>::kBytes, kSmem = W * (int)sizeof(float) + kRingStages * W * (E + (COMP ? 1 : E));
+template <int DT> static int launch_ln_bwd_ring(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
+    constexpr int TPR = 128, kSmem = kRingCols * ((int)sizeof(float) + kRingStages * (Elem<DT>::kBytes + 1));
+    auto* k = layer_norm_backward_ring_kernel<DT, TPR, kRingCols / (TPR * 8)>;
     static std::atomic<bool> allowed[kMaxDevices];
     if (!allow_smem(k, kSmem, allowed)) return GACT_ERR_LAUNCH;
     k<<<(unsigned)blocks, TPR, kSmem, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
-}
-template <int DT, int TPR, int CH> static int launch_ln_bwd_ring(const LnBwdArgs& a, int64_t blocks, cudaStream_t s) {
-    return a.codes ? launch_ln_bwd_ring_kernel<DT, TPR, CH, true>(a, blocks, s) : launch_ln_bwd_ring_kernel<DT, TPR, CH, false>(a, blocks, s);
 }
 template <int DT, int TPR, int CH, int R> static int launch_ln_bwd(const LnBwdArgs& a, bool vec, int64_t blocks, cudaStream_t s) {
     const int block = TPR > 32 ? TPR : 128;
@@ -647,13 +644,9 @@ template <int DT, int TPR, int CH, int R> static int launch_ln_bwd(const LnBwdAr
     }
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
-template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, int64_t blocks, cudaStream_t s) {
+template <int DT> static int dispatch_ln_bwd(const LnBwdArgs& a, bool vec, bool ring, int64_t blocks, cudaStream_t s) {
     const int h = a.cols;
-    if (ln_bwd_shape(vec, a.rows, h).ring) {
-        if (h <= 2048) return launch_ln_bwd_ring<DT, 128, 2>(a, blocks, s);
-        if (h <= 4096) return launch_ln_bwd_ring<DT, 128, 4>(a, blocks, s);
-        return launch_ln_bwd_ring<DT, 512, 2>(a, blocks, s);
-    }
+    if (ring) return launch_ln_bwd_ring<DT>(a, blocks, s);
     if (h <= 32) return launch_ln_bwd<DT, 4, 1, kLnBwdRows>(a, vec, blocks, s);
     if (h <= 64) return launch_ln_bwd<DT, 8, 1, kLnBwdRows>(a, vec, blocks, s);
     if (h <= 128) return launch_ln_bwd<DT, 16, 1, kLnBwdRows>(a, vec, blocks, s);
@@ -772,8 +765,8 @@ extern "C" int gact_layer_norm(const void* x, int dtype, int64_t rows, int64_t c
 
 extern "C" int64_t gact_layer_norm_backward_scratch_bytes(int64_t rows, int64_t cols) {
     if (!ln_sizes_ok(rows, cols)) return -1;
-    // (whichever kernel the operands' alignment picks)
-    const int64_t a = ln_bwd_blocks(true, rows, cols), b = ln_bwd_blocks(false, rows, cols);
+    // (whichever kernel the operands' type and alignment pick)
+    const int64_t a = cols <= kRingCols ? ln_bwd_blocks(true, rows, cols) : 0, b = ln_bwd_blocks(false, rows, cols);
     return (a > b ? a : b) * 2 * ((cols + 7) / 8 * 8) * (int64_t)sizeof(float);
 }
 
@@ -806,12 +799,13 @@ extern "C" int gact_layer_norm_backward(const void* dy, int dtype, int64_t rows,
     a.wait_limit = hook.limit; a.withhold = hook.withhold; a.report = pipeline_report_word();
     const int eb = elem_bytes_of(dtype);
     const bool vec = rows_aligned(dy, ld_dy, cols, eb) && (!x || rows_aligned(x, ld_x, cols, eb)) && (!dx || rows_aligned(dx, cols, cols, eb));
-    const int64_t blocks = ln_bwd_blocks(vec, rows, cols);
+    const bool ring = ln_ring(vec, a.codes != nullptr, dtype, rows, cols, hook.withhold != 0);
+    const int64_t blocks = ln_bwd_blocks(ring, rows, cols);
     int st;
     switch (dtype) {
-    case GACT_F32: st = dispatch_ln_bwd<GACT_F32>(a, vec, blocks, s); break;
-    case GACT_F16: st = dispatch_ln_bwd<GACT_F16>(a, vec, blocks, s); break;
-    default: st = dispatch_ln_bwd<GACT_BF16>(a, vec, blocks, s); break;
+    case GACT_F32: st = dispatch_ln_bwd<GACT_F32>(a, vec, ring, blocks, s); break;
+    case GACT_F16: st = dispatch_ln_bwd<GACT_F16>(a, vec, ring, blocks, s); break;
+    default: st = dispatch_ln_bwd<GACT_BF16>(a, vec, ring, blocks, s); break;
     }
     if (st != GACT_OK || !params) return st;
     // both halves are summed; a gradient nobody asked for is not stored

@@ -112,7 +112,8 @@ int gact_pipeline_reported(void);
  * Diagnostics, no counterpart in the reference.  wait_limit: polls after which a wait of the pipeline above gives
  * up (0 restores the default, 2^20).  withhold_one_copy != 0: warp 0 of block 0 leaves its first bulk copy
  * unissued, so that its wait runs out after wait_limit polls - the only way to see the give-up path work without
- * a broken GPU.  The products of gact_linear* and gact_layer_norm_backward take the same knobs (default there 2^23).
+ * a broken GPU.  The products of gact_linear* and gact_layer_norm_backward take the same knobs (default there 2^23); the
+ * latter then takes its kernel with copies for all aligned rows of up to 4096 elements with codes.
  * Process-wide, read at launch; meant for the test-suite.
  */
 void gact_pipeline_test_hook(uint32_t wait_limit, int withhold_one_copy);
