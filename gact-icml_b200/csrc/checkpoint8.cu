@@ -127,8 +127,17 @@ __global__ void __launch_bounds__(kCThreads) repitch16_kernel(const uint16_t* __
     }
 }
 
-// Four chunks a thread once that still fills the GPU, else one (a small tensor is bound by latency).  Rows that do not
-// start on 16-byte boundaries are walked along the row once a warp's 256 columns are at least half full.
+// Four chunks a thread once that still fills the GPU, else one (a small tensor is bound by latency).  Measured, four / one in us,
+// bf16 rows of 1024: 1024 rows 2.6 / 2.0, 4096 3.8 / 3.5, 9472 (where the rule changes) 6.5 / 7.2, 65536 33.8 / 39.7; back 2.2 / 1.9,
+// 3.5 / 3.3, 6.3 / 7.0, 32.1 / 36.9.
+// Rows that do not start on 16-byte boundaries are walked along the row where the warps' 256 columns are full enough: the element-wise
+// accesses then run side by side, but lanes past the end of a row idle.  Measured on 8 M elements, along the row / flat in us,
+// bf16 (fp32): 127 columns 12.9 / 7.2 (13.9 / 10.1), 161 10.9 / 8.1 (12.1 / 10.2), 255 7.8 / 7.4 (9.0 / 11.1), 257 12.8 / 7.9
+// (13.6 / 10.5); on 16 M: 513 17.4 / 16.6 (18.7 / 20.1), 771 16.1 / 16.2 (17.5 / 20.3), 1003 14.1 / 16.5 (16.0 / 21.0).  Restoring, where
+// the stores are the element-wise side, pays sooner: 65 columns 21.8 / 23.1 (26.5 / 21.1), 73 19.8 / 24.7 (24.4 / 26.2), 97
+// 15.7 / 24.7 (20.2 / 26.2), 257 12.0 / 23.8 (13.9 / 30.5).
+static bool along_row_ckpt(int cols, int tiles) { return 4 * (int64_t)cols >= 3 * 256 * (int64_t)tiles; }
+static bool along_row_restore(int cols) { return cols >= 72; }
 template <bool FLAT> static int64_t walk_blocks(int64_t rows, int chunks, int tiles, int u) {
     const int64_t per = (int64_t)(FLAT ? kCThreads : kCThreads / 32) * u;
     return (rows * (FLAT ? chunks : tiles) + per - 1) / per;
@@ -144,7 +153,7 @@ template <int DT, bool VEC, bool FLAT, bool STOCH> static void launch_ckpt(Ckpt8
 }
 template <int DT, bool STOCH> static int dispatch_ckpt(const Ckpt8Args& a, cudaStream_t s) {
     if (rows_aligned(a.x, a.ld, a.cols, Elem<DT>::kBytes)) launch_ckpt<DT, true, true, STOCH>(a, s);
-    else if (a.cols >= 128) launch_ckpt<DT, false, false, STOCH>(a, s);
+    else if (along_row_ckpt(a.cols, a.tiles)) launch_ckpt<DT, false, false, STOCH>(a, s);
     else launch_ckpt<DT, false, true, STOCH>(a, s);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }
@@ -158,7 +167,7 @@ template <int DT, bool VEC, bool FLAT> static void launch_restore(Restore8Args a
 }
 template <int DT> static int dispatch_restore(const Restore8Args& a, cudaStream_t s) {
     if (rows_aligned(a.out, a.ld, a.cols, Elem<DT>::kBytes)) launch_restore<DT, true, true>(a, s);
-    else if (a.cols >= 128) launch_restore<DT, false, false>(a, s);
+    else if (along_row_restore(a.cols)) launch_restore<DT, false, false>(a, s);
     else launch_restore<DT, false, true>(a, s);
     return cudaGetLastError() == cudaSuccess ? GACT_OK : GACT_ERR_LAUNCH;
 }

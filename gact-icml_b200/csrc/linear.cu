@@ -868,8 +868,10 @@ __global__ void __launch_bounds__(kAWarps * 32, 4) act_backward_kernel(const __g
     if (c < a.width) a.partial[(int64_t)blockIdx.y * a.width + c] = sum;
 }
 
-// Filling the table takes about a microsecond: worth it from 64 rows per warp on (with the grid below).
-static bool act_bwd_table(int64_t rows, int64_t cols) { return rows * ((cols + 255) / 256) >= (int64_t)sm_count() * 4 * kAWarps * 4; }
+// Filling the table takes about a microsecond: worth it from 5 rows per warp on (with the grid below).  Measured, table / computed in us,
+// 4096 columns, GELU (SiLU): 1184 rows 8.0 / 7.6 (7.4 / 6.7), 1400 9.0 / 9.4 (8.7 / 8.5), 2048 11.4 / 12.4 (11.1 / 11.7), 8192
+// 32 / 39 (31 / 37).
+static bool act_bwd_table(int64_t rows, int64_t cols) { return rows * ((cols + 255) / 256) >= (int64_t)sm_count() * 4 * kAWarps * 5; }
 // Parts of the rows (blocks per strip of 256 columns): four blocks per SM.  The count must not depend on anything but the sizes.
 static int64_t act_bwd_parts(int64_t rows, int64_t cols) {
     const int64_t strips = (cols + 255) / 256;
