@@ -119,11 +119,15 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5, compress=None):
     return _LayerNorm.apply(input, weight, bias, eps, compress, _next_seed(input.device) if compress else None)
 
 
+def _autocast_dtype(t):
+    """The type that a linear layer computes a tensor in."""
+    if not torch.is_autocast_enabled("cuda") or not t.is_floating_point() or t.dtype == torch.float64:
+        return t.dtype
+    return torch.get_autocast_dtype("cuda")
+
+
 def _autocast(*tensors):
-    if not torch.is_autocast_enabled("cuda"):
-        return tensors
-    dt = torch.get_autocast_dtype("cuda")
-    return tuple(t if t is None or not t.is_floating_point() or t.dtype == torch.float64 else t.to(dt) for t in tensors)
+    return tuple(t if t is None else t.to(_autocast_dtype(t)) for t in tensors)
 
 
 def linear(input, weight, bias=None, activation=None, residual=None, compress=None, checkpoint=None, keep_input=None):
@@ -182,7 +186,7 @@ class Linear(nn.Linear):
         checkpoint = None
         # (made in the type that the parent was called under: a forward pass that enters autocast by itself computes in another)
         # and on its stream: a layer run on another one may come before it and outlive it
-        if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast(input)[0].dtype \
+        if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast_dtype(input) \
                 and shared[3] == _stream(input):
             checkpoint = shared[0]
         return linear(input, self.weight, self.bias, self.activation, residual, checkpoint=checkpoint)
