@@ -76,8 +76,9 @@ class _LayerNorm(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, compress, seed, given, keep_input):
-        # Under autocast the parameters are cast here and again in backward: what is saved is the parameter itself, which hooks
-        # know and leave alone.  (A copy that requires a gradient looks like an activation to them and would be quantized.)
+        # Under autocast the parameters are cast here and again in backward.  What is saved is the weight itself, detached: saved-tensor
+        # hooks take a tensor that requires a gradient and is no parameter they know (a cast copy, a computed weight) for an activation,
+        # and would quantize it.
         w, b = _autocast(weight, bias)
         # Only what a gradient will need: the input for the weight's, the weight for the input's, the pre-activation for any of the three.
         n = ctx.needs_input_grad
@@ -88,7 +89,7 @@ class _Linear(torch.autograd.Function):
         y, s = fused.op_linear(x, w, b, activation, residual, compress=compress, seed=seed, checkpoint=ck, keep_input=keep_input)
         xt, *ctx.x = _flat(s.x)
         zt, *ctx.z = _flat(s.z)
-        ctx.save_for_backward(xt, zt, weight if n[0] else None)
+        ctx.save_for_backward(xt, zt, weight.detach() if n[0] else None)
         ctx.meta = (activation, s.out_shape, s.has_bias, s.in_features)
         ctx.param_dtypes = weight.dtype, None if bias is None else bias.dtype
         return y
@@ -184,8 +185,8 @@ class Linear(nn.Linear):
     def forward(self, input, residual=None):
         shared, self._shared = self._shared, None
         checkpoint = None
-        # (made in the type that the parent was called under: a forward pass that enters autocast by itself computes in another)
-        # and on its stream: a layer run on another one may come before it and outlive it
+        # It was made in the type that the parent was called under (a forward pass that enters autocast by itself computes in
+        # another) and on its stream (a layer on another one could read it before it is there, and outlive it).
         if shared is not None and shared[1] is input and shared[2] == input._version and shared[0].dtype == _autocast_dtype(input) \
                 and shared[3] == _stream(input):
             checkpoint = shared[0]

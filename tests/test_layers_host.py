@@ -275,3 +275,21 @@ def test_convert_does_not_move_an_activation_into_a_layer_that_is_used_elsewhere
     m = torch.nn.ModuleList([torch.nn.Sequential(lin, torch.nn.ReLU()), lin])
     layers.convert(m)
     assert m[0][0].activation == "relu" and m[1].activation is None and m[0][0].weight is m[1].weight is lin.weight
+
+
+@pytest.mark.parametrize("compress", [True, False])
+def test_a_computed_weight_is_no_activation(plain, compress):
+    """A weight that is computed from parameters (a norm, an adapter's product) reaches the hooks without requiring a gradient, and a
+    change in place is still noticed."""
+    a, b = torch.randn(4, 2).bfloat16().requires_grad_(), torch.randn(2, 8).bfloat16().requires_grad_()
+    x = torch.randn(5, 8).bfloat16().requires_grad_()
+    w = a @ b
+    y, seen = saved_by(lambda: layers.linear(x, w, compress=compress))
+    assert not any(t.requires_grad for t in seen if t.is_floating_point() and t.data_ptr() != x.data_ptr())
+    y.sum().backward(retain_graph=True)
+    assert a.grad is not None and torch.equal(x.grad, torch.ones(5, 4).bfloat16() @ w.detach())
+    y = layers.linear(x, w, compress=compress)          # (hooks do without the version check)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
