@@ -1,5 +1,6 @@
 // 8-bit activation checkpoints: rows -> codes + scales, and back (format: blocks8.cuh).  Bound by HBM: bf16 65536 x 4096 takes
-// 125 us (0.99 of the copy bandwidth), back 120; with stochastic rounding 199 (the generator's instructions).
+// 126 us (0.99 of the copy bandwidth), back 121; with stochastic rounding 200 (the generator: 20.4 instructions an element instead of
+// 12.7, issue slots 74 % busy).
 #include "blocks8.cuh"
 
 namespace gact {

@@ -3,14 +3,16 @@
 //   mean = sum(x) / H,  r = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) r w + b
 //   x^ = (x' - mean) r with x' the kept input (restored codes, or x itself),  g = dy w
 //   centred codes keep x - mean instead:  x^ = x' r.  Half a code's step is then at most 1/127 of the largest deviation from the
-//   mean; that of x grows with the mean, and seen through r it has no bound (rows of 100 +- 1: dw 28 % off, centred 0.8 %)
+//   mean; that of x grows with the mean, and seen through r it has no bound (fp32 rows of 100 +- 1: dw 30 % off, centred 0.9 %)
 //   dx = r (g - sum(g)/H - x^ sum(g x^)/H),  dw = sum over rows of dy x^,  db = sum over rows of dy
 //
 // Both passes are bound by HBM: forward reads x and writes y and 33/32 bytes of codes per element, backward reads dy and
 // the codes and writes dx.  Statistics, sums and the weight gradients are fp32; the variance is taken around the mean
-// (x stays in registers, so the second look at it is free).  Measured in bf16: 65536 x 4096 forward 258 us, backward 248 (0.80
-// and 0.83 of the copy bandwidth); 65536 x 1024 64 and 72; 8192 x 1024 11.5 and 15 (of which 4 the sum of the partials);
-// 128 x 1024 2.5 and 4.7 (launches).
+// (x stays in registers, so the second look at it is free); 1 / H is a factor, r comes from rsqrtf, and (x' - mean) r is one
+// multiply-add x' r - mean r in the backward pass: fp32 outputs are off by 1.7e-7, half again as much as with a division, a square
+// root and a subtraction.  Measured in bf16: 65536 x 4096 forward 262 us (centred 271), backward 252 (0.79 and 0.82 of the copy
+// bandwidth); 65536 x 1024 66 to 70 and 74; 8192 x 1024 11.9 and 15.6 (of which 4 the sum of the partials), fp32 16.2 and 19.9;
+// 128 x 1024 2.7 and 5.0 (launches).
 #include "blocks8.cuh"
 #include "tcgen05.cuh"
 

@@ -9,8 +9,8 @@
 // MN-major tiles), persistent, one block per SM: warp 0 feeds a ring of operand tiles with tensor-map copies, one thread of
 // warp 1 issues tcgen05.mma into one of two TMEM accumulators, eight warps work on the other one (epilogue), and the two warps
 // that are left do side jobs.  Bounds, measured on 8192 rows, 1024 -> 4096 features, bf16 (68.7 GFLOP a product, 41.5 us at the
-// measured 1655 TFLOP/s): forward 55 us, with GELU and the pre-activation's checkpoint 67 (the epilogue's instructions and
-// TMEM reads, hidden from a reduction of about 1500 on), data gradient 53, weight gradient 52; the tensor pipe is busy 83 % of
+// measured 1655 TFLOP/s): forward 54 us, with GELU and the pre-activation's checkpoint 68 (the epilogue's instructions and
+// TMEM reads; at a reduction of 4096, 32768 rows, 75 to 160 of 860 to 945), data gradient 53, weight gradient 54; the tensor pipe is busy 83 % of
 // the cycles in which the SMs work, and 64 or 512 tiles over 74 pairs of SMs leave 7 to 14 % of them idle at the end.
 // Widening the codes inside the weight gradient instead of restoring x beside the data gradient was built and measured: 80 us
 // instead of 52 + 2.
@@ -744,11 +744,13 @@ constexpr int kAWarps = 8;
 
 // A warp owns 256 columns (8 per lane) and walks rows, kARows of them side by side.  A block takes eight such sets at a time.
 // 64 registers and four blocks per SM: loading the next rows ahead instead took 84 registers and was a quarter slower.
+// dz is rounded to the operands' 16 bits, for the tensor cores read it: against 64 bits the products' error is then 0.0023 instead of
+// 0.0017 in bf16 (0.0003 instead of 0.0002 in fp16).  The bias gradient sums the products before they are rounded.
 constexpr int kARows = 2;
 //
 // TABLE: a pre-activation from a checkpoint is an 8-bit code times a power of two, so there are 256 slopes per exponent.  Those
 // of the exponents -14 .. 4 are computed once per block; a slope is then one shared-memory read instead of about 20
-// instructions (the kernel was bound by issuing them: GELU on 8192 x 4096 took 59 us, with the table 32; floor 26).  Larger exponents
+// instructions (the kernel was bound by issuing them: GELU on 8192 x 4096 took 59 us, with the table 32 to 34; floor 26).  Larger exponents
 // equal the last row (a code's step is past the bend); below, |z| < 0.004 and the slope is its tangent at 0 (the next term,
 // z^3 / 4, is below 2^-25); a NaN block's tangent is NaN.
 constexpr int kLowExp = -14, kHighExp = 4, kTableRows = kHighExp - kLowExp + 1;
